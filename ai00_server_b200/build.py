@@ -16,8 +16,13 @@ ORACLE_C = os.path.join(ROOT, "oracle", "liboracle_ref.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-    "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-shared",
+    "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
 ]
+# translation units of the engine library and the sources each is made of (None: every header)
+UNITS = {
+    "engine.cu": None,
+    "operators.cu": ["adapters.cuh", "logits.cuh", "operators.cuh", "common.cuh", "host.cuh"],
+}
 
 
 def _newer(target: str, sources: list[str]) -> bool:
@@ -33,14 +38,27 @@ def _run(cmd: list[str]) -> None:
 
 
 def build_engine(force: bool = False, verbose_ptxas: bool = False, debug: bool = False) -> str:
-    srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh"))]
-    srcs.append(os.path.join(ROOT, "include", "b200rwkv.h"))
+    header = os.path.join(ROOT, "include", "b200rwkv.h")
     target = LIB_DEBUG if debug else LIB
-    if force or not _newer(target, srcs):
-        nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-        cmd = [nvcc] + NVCC_FLAGS + (["-DB200RWKV_DEBUG"] if debug else []) + (["-Xptxas", "-v"] if verbose_ptxas else []) + [
-            os.path.join(CSRC, "engine.cu"), "-o", target]
-        _run(cmd)
+    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+    objects, jobs = [], []
+    for unit, parts in UNITS.items():
+        if parts is None:
+            parts = [f for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh")]
+        srcs = [os.path.join(CSRC, f) for f in [unit, *parts]] + [header]
+        obj = os.path.join(CSRC, unit[:-3] + ("_dbg.o" if debug else ".o"))
+        objects.append(obj)
+        if force or not _newer(obj, srcs):
+            jobs.append([nvcc] + NVCC_FLAGS + (["-DB200RWKV_DEBUG"] if debug else []) + (["-Xptxas", "-v"] if verbose_ptxas else []) + [
+                "-c", os.path.join(CSRC, unit), "-o", obj])
+    for cmd in jobs:
+        print("+", " ".join(cmd), flush=True)
+    running = [subprocess.Popen(cmd) for cmd in jobs]
+    failed = [cmd for cmd, p in zip(jobs, running) if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    if jobs or not _newer(target, objects):
+        _run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", *objects, "-o", target])
     return target
 
 

@@ -41,6 +41,32 @@ class Options(C.Structure):
                 ("config_json", C.c_void_p), ("config_len", C.c_size_t), ("kv_tokens", C.c_int32), ("kv_page", C.c_int32)]
 
 
+class AdapterPart(C.Structure):
+    """b200rwkv_adapter_part (include/b200rwkv.h)."""
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("base", C.c_void_p), ("base_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("in_features", C.c_int32), ("out_features", C.c_int32), ("rank", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class Adapters(C.Structure):
+    """b200rwkv_adapters."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("out_type", C.c_int32), ("tokens", C.c_int32), ("adapters", C.c_int32),
+                ("num_parts", C.c_int32), ("index", C.c_void_p), ("scale", C.c_void_p), ("parts", C.POINTER(AdapterPart)), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Logits(C.Structure):
+    """b200rwkv_logits."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("kind", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32),
+                ("allow_rows", C.c_int32), ("logits", C.c_void_p), ("logits_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("controls", C.c_void_p), ("history_offset", C.c_void_p), ("history", C.c_void_p), ("history_from", C.c_void_p),
+                ("allow", C.c_void_p), ("allow_row", C.c_void_p), ("bias_offset", C.c_void_p), ("bias_token", C.c_void_p),
+                ("bias_value", C.c_void_p)]
+
+
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+LOGITS, PROBS, LOG_PROBS = 0, 1, 2
+MAX_PARTS, MAX_RANK, MAX_ADAPTERS = 8, 256, 1024
 QUANT_NONE, QUANT_INT8, QUANT_NF4 = 0, 1, 2
 ARCH_KEMIRAX = 100          # Info.version of the config.json-described families
 ARCH_DEGAVIK = 101
@@ -90,6 +116,9 @@ SYMBOLS = [
     ("b200rwkv_profile_insitu", C.c_int32, [_P, C.c_int32, _P, _P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, C.POINTER(C.c_double)]),
     ("b200rwkv_op_quantize", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     ("b200rwkv_op_wkv", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32] + [_P] * 14),
+    ("b200rwkv_op_adapters_workspace", C.c_int64, [C.c_int32, C.c_int32]),
+    ("b200rwkv_op_adapters", C.c_int32, [C.c_int32, _P, C.POINTER(Adapters)]),
+    ("b200rwkv_op_logits", C.c_int32, [C.c_int32, _P, C.POINTER(Logits)]),
     ("b200rwkv_launch_count", C.c_int32, [_P, C.POINTER(C.c_int64)]),
     ("b200rwkv_keep_hidden", C.c_int32, [_P, C.c_int32]),
     ("b200rwkv_last_hidden", C.c_int32, [_P, _P, C.c_size_t]),

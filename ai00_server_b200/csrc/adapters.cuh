@@ -1,0 +1,433 @@
+// Low-rank adapters of many requests beside their shared projection: token t of a request with adapter a adds to the projection's output
+//     out[t, n] = base[t, n] + scale[a] * sum_r S[t, r] B[a][n, r],      S[t, r] = sum_k x[t, k] A[a][r, k]
+// and a token without one (an index that names no adapter) keeps its base.  The reference blends such pairs into the weights when a model is loaded
+// (lib.rs:466-485); here they stay apart, so that the requests of a batch can have different ones.
+//
+// Tokens are taken in groups that share an adapter (tokens of a batch lie in any order).  Bound: a decode batch reads every adapter of its requests
+// once, 2 R (K + N) bytes each, beside rows of a few KB, so what counts is how soon the two dependent products are through.
+//
+// adapter_few_kernel: a cluster of eight CTAs takes eight tokens of one adapter.  Each CTA has an eighth of k for the first product and an eighth of n for
+// the second; between them the eight partial S (R x 8 floats) go to every CTA of the cluster in one exchange, so that nothing but x, A, B, base and out
+// touches memory.  Both products are m16n8k16 with the adapter's rows as M and the eight tokens as N: a lane reads 16 bytes of a row at a time, which
+// is two steps of k for it (the order of k within 32 is the same permutation on both sides of a product, so it is never undone).
+// S is f32; the second product takes it as two or three 16-bit parts, enough for the output's type, scaled per token by a power of two.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int ADP_CTAS = 8, ADP_THREADS = 256, ADP_WARPS = ADP_THREADS / 32;
+constexpr int ADP_TOK = 8;                       // tokens of a group: the N of the products
+constexpr int ADP_MAX_PARTS = 8, ADP_MAX_RANK = 256, ADP_MAX_ADAPTERS = 1024;
+constexpr int ADP_INLINE = ADP_THREADS;          // tokens of a call whose groups every CTA finds by itself; more take adapter_plan_kernel
+constexpr int ADP_PLAN_THREADS = 1024;
+
+// one adapter of one projection, where adapters lie apart
+struct AdapterEntry {
+    const void* a;
+    const void* b;
+    int rank;                    // 0: the adapter leaves this projection alone
+    float scale;
+};
+
+struct AdapterPart {
+    const void* x;               // rows of K, or (x_a16) the A16 layout of common.cuh with x_th as its height
+    long long x_stride;          // elements
+    int x_a16, x_th;
+    int x_lo;                    // rows to the low half of split operands (0: none)
+    const void* a;               // [adapters][R][K]
+    const void* b;               // [adapters][N][R]
+    const AdapterEntry* table;   // instead of a and b
+    const void* base;
+    long long base_stride;
+    void* out;
+    long long out_stride;
+    int K, N, R;                 // R: the largest rank
+    int vec;                     // rows of base and out take accesses of four elements
+};
+
+// groups of more tokens than ADP_INLINE: [0] = groups, then {adapter, first place} of each, then tokens by place
+struct AdapterPlan {
+    int* base;
+    int tokens, most;            // most: groups there can be
+    __host__ __device__ int* count() const { return base; }
+    __host__ __device__ int2* group() const { return reinterpret_cast<int2*>(base + 4); }
+    __host__ __device__ int* place() const { return base + 4 + 2 * (size_t)most; }
+    __host__ __device__ static size_t ints(int tokens, int most) { return 4 + 2 * (size_t)most + tokens; }
+};
+
+struct AdapterParams {
+    int tokens, adapters;
+    int copy;                    // tokens without an adapter have their base copied (base and out differ)
+    const int* index;
+    const float* scale;
+    AdapterPlan plan;
+    AdapterPart part[ADP_MAX_PARTS];
+};
+
+// groups of up to ADP_TOK tokens that `tokens` tokens can need: all with their own adapter, or full groups and a broken one for each adapter (and for none)
+__host__ __device__ inline int adapter_groups(int tokens, int adapters) {
+    const long long full = (long long)adapters + 1 + tokens / ADP_TOK;
+    return (int)(full < tokens ? full : tokens);
+}
+
+template <typename E> struct AdpType;
+template <> struct AdpType<__half> {
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        mma_16816(c, a0, a1, a2, a3, b0, b1);
+    }
+    static __device__ __forceinline__ __half round(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+};
+template <> struct AdpType<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+};
+
+// 16-bit parts of S in the second product: what they leave out is far below half a step of the output's type (two parts of f16 leave 2^-22, of bf16 2^-17,
+// three of bf16 2^-25)
+template <typename E, typename O> struct AdpParts { static constexpr int N = 2; };
+template <> struct AdpParts<__nv_bfloat16, float> { static constexpr int N = 3; };
+
+__device__ __forceinline__ uint4 adp_ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
+
+__device__ __forceinline__ void adp_load4(const float* p, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+template <typename O>
+__device__ __forceinline__ void adp_load4(const O* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const O* e = reinterpret_cast<const O*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = AdpType<O>::widen(e[i]);
+}
+__device__ __forceinline__ void adp_store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <typename O>
+__device__ __forceinline__ void adp_store4(O* p, const float (&v)[4]) {
+    uint2 u;
+    O* e = reinterpret_cast<O*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = AdpType<O>::round(v[i]);
+    *reinterpret_cast<uint2*>(p) = u;
+}
+__device__ __forceinline__ float adp_widen(float v) { return v; }
+__device__ __forceinline__ float adp_widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ float adp_widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void adp_put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void adp_put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void adp_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+struct AdpGroup {
+    int tok[ADP_TOK];            // tokens, -1 behind the last
+    int adapter;                 // -1: none
+    int found;
+};
+
+// group `want` of a call of up to ADP_INLINE tokens, found by all threads of a CTA: a group starts at a token whose number of earlier tokens with
+// the same adapter is a multiple of ADP_TOK, groups count in the order of their first tokens
+__device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const int want, AdpGroup& g, int* s_idx, int* s_cnt) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int id = -2;
+    if (tid < p.tokens) {
+        id = p.index[tid];
+        if (id < 0 || id >= p.adapters) id = p.copy ? -1 : -2;
+    }
+    s_idx[tid] = id;
+    if (tid < ADP_TOK) g.tok[tid] = -1;
+    if (tid == 0) g.found = 0;
+    __syncthreads();
+    const unsigned before = (1u << lane) - 1u;
+    int rank = __popc(__match_any_sync(0xffffffffu, id) & before);
+    for (int w = 0; w < warp * 32; w += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(s_idx + w);
+        rank += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+    }
+    const bool start = id >= -1 && rank % ADP_TOK == 0;
+    const unsigned starts = __ballot_sync(0xffffffffu, start);
+    if (lane == 0) s_cnt[warp] = __popc(starts);
+    __syncthreads();
+    int number = __popc(starts & before);
+    for (int w = 0; w < warp; ++w) number += s_cnt[w];
+    if (start && number == want) {
+        g.adapter = id;
+        g.found = rank + 1;
+    }
+    __syncthreads();
+    if (g.found && id >= -1 && id == g.adapter && rank >= g.found - 1 && rank < g.found - 1 + ADP_TOK) g.tok[rank - (g.found - 1)] = tid;
+    __syncthreads();
+}
+
+template <typename E, typename O>
+__global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) adapter_few_kernel(const __grid_constant__ AdapterParams p) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    __shared__ AdpGroup g;
+    __shared__ __align__(16) int s_idx[ADP_THREADS];
+    __shared__ int s_cnt[ADP_WARPS];
+    __shared__ float s_back[ADP_TOK];
+    constexpr int NP = AdpParts<E, O>::N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = lane >> 2, quad = lane & 3;
+    const int cta = blockIdx.x % ADP_CTAS, want = blockIdx.x / ADP_CTAS;
+    const AdapterPart& q = p.part[blockIdx.y];
+    pdl_wait();
+    if (p.plan.base) {
+        if (want >= *p.plan.count()) return;
+        const int2 gr = p.plan.group()[want];
+        if (tid < ADP_TOK) {
+            // places of a group: up to the next group's first
+            const int last = want + 1 < *p.plan.count() ? p.plan.group()[want + 1].y : p.plan.count()[1];
+            g.tok[tid] = gr.y + tid < last ? p.plan.place()[gr.y + tid] : -1;
+        }
+        if (tid == 0) g.adapter = gr.x;
+        __syncthreads();
+    } else {
+        adapter_find_group(p, want, g, s_idx, s_cnt);
+        if (!g.found) return;
+    }
+    const int adapter = g.adapter, K = q.K, N = q.N;
+    O* const out = reinterpret_cast<O*>(q.out);
+    const O* const base = reinterpret_cast<const O*>(q.base);
+    const E *A = nullptr, *B = nullptr;
+    int R = 0;
+    float scale = 0.f;
+    if (adapter >= 0) {
+        if (q.table) {
+            const AdapterEntry e = q.table[adapter];
+            A = reinterpret_cast<const E*>(e.a); B = reinterpret_cast<const E*>(e.b); R = e.rank; scale = e.scale;
+        } else {
+            R = q.R;
+            A = reinterpret_cast<const E*>(q.a) + (size_t)adapter * R * K;
+            B = reinterpret_cast<const E*>(q.b) + (size_t)adapter * N * R;
+            scale = p.scale[adapter];
+        }
+    }
+    const int units = (N + 31) / 32, u0 = (int)((long long)units * cta / ADP_CTAS), u1 = (int)((long long)units * (cta + 1) / ADP_CTAS);
+    if (R == 0) {
+        if (!p.copy || (q.base == q.out && q.base_stride == q.out_stride)) return;
+        for (int j = warp; j < ADP_TOK; j += ADP_WARPS) {
+            const int t = g.tok[j];
+            if (t < 0) continue;
+            for (int n = u0 * 32 + lane; n < min(u1 * 32, N); n += 32)
+                adp_put(out + (size_t)t * q.out_stride + n, base ? adp_widen(base[(size_t)t * q.base_stride + n]) : 0.f);
+        }
+        return;
+    }
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+
+    const int R8 = R * ADP_TOK, Rp = (R + 31) & ~31, pitch = Rp + 8;
+    float* const part = reinterpret_cast<float*>(smem_raw);                      // [warp][R][8]: partial sums of the CTA's warps
+    float* const all = part + (size_t)ADP_WARPS * q.R * ADP_TOK;                 // [CTA][R][8]
+    E* const frag = reinterpret_cast<E*>(all + (size_t)ADP_CTAS * q.R * ADP_TOK);        // [part][token][pitch]
+
+    // ---- S: this CTA's k, a run of 32 of them to a warp at a time ----
+    {
+        const int tok = g.tok[row];
+        const E* const x = reinterpret_cast<const E*>(q.x);
+        auto xat = [&](int k, int lo) {
+            return q.x_a16 ? x + a16_index(tok + lo, k, q.x_th) : x + (size_t)(tok + lo) * q.x_stride + k;
+        };
+        const int nk = (K + 31) / 32, c0 = (int)((long long)nk * cta / ADP_CTAS), c1 = (int)((long long)nk * (cta + 1) / ADP_CTAS);
+        for (int m0 = 0; m0 < R; m0 += 64) {
+            float acc[4][4] = {};
+            for (int c = c0 + warp; c < c1; c += ADP_WARPS) {
+                const int k = c * 32 + quad * 8;
+                const bool in = k < K;
+                uint4 xv = make_uint4(0, 0, 0, 0), xl = xv, lo[4], hi[4];
+                if (in && tok >= 0) {
+                    xv = adp_ld16(xat(k, 0));
+                    if (q.x_lo) xl = adp_ld16(xat(k, q.x_lo));
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    const int r = m0 + m * 16 + row;
+                    lo[m] = hi[m] = make_uint4(0, 0, 0, 0);
+                    if (in && r < R) lo[m] = adp_ld16(A + (size_t)r * K + k);
+                    if (in && r + 8 < R) hi[m] = adp_ld16(A + (size_t)(r + 8) * K + k);
+                }
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                    AdpType<E>::mma(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xv.x, xv.y);
+                    AdpType<E>::mma(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xv.z, xv.w);
+                    if (q.x_lo) {
+                        AdpType<E>::mma(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xl.x, xl.y);
+                        AdpType<E>::mma(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xl.z, xl.w);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int r = m0 + m * 16 + row;
+                float* const d = part + (size_t)warp * R8 + r * ADP_TOK + quad * 2;
+                if (r < R) *reinterpret_cast<float2*>(d) = make_float2(acc[m][0], acc[m][1]);
+                if (r + 8 < R) *reinterpret_cast<float2*>(d + 8 * ADP_TOK) = make_float2(acc[m][2], acc[m][3]);
+            }
+        }
+    }
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");          // every CTA of the cluster has started
+    for (int i = tid * 4; i < R8; i += ADP_THREADS * 4) {
+        float4 s = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll
+        for (int w = 1; w < ADP_WARPS; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(part + (size_t)w * R8 + i);
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+        }
+        const uint32_t local = smem_u32(all + (size_t)cta * R8 + i);
+#pragma unroll
+        for (int c = 0; c < ADP_CTAS; ++c) {
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(c));
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(s.x), "f"(s.y), "f"(s.z), "f"(s.w) : "memory");
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+
+    // ---- S of a token (one to a warp): sum over the CTAs in their order, scale, 16-bit parts relative to the token's largest ----
+    {
+        float v[ADP_MAX_RANK / 32], top = 0.f;
+#pragma unroll
+        for (int i = 0; i < ADP_MAX_RANK / 32; ++i) {
+            const int r = i * 32 + lane;
+            v[i] = 0.f;
+            if (r < R) {
+#pragma unroll
+                for (int c = 0; c < ADP_CTAS; ++c) v[i] += all[(size_t)c * R8 + r * ADP_TOK + warp];
+                v[i] *= scale;
+            }
+            top = fmaxf(top, fabsf(v[i]));
+        }
+        top = warp_max(top);
+        // a power of two near the largest (its exponent field alone; the smallest and the largest few stay within normal numbers)
+        const unsigned ex = min(max((__float_as_uint(top) >> 23) & 255u, 2u), 252u);
+        const float down = __uint_as_float((254u - ex) << 23), back = __uint_as_float(ex << 23);
+        if (lane == 0) s_back[warp] = back;
+#pragma unroll
+        for (int i = 0; i < ADP_MAX_RANK / 32; ++i) {
+            const int r = i * 32 + lane;
+            if (r < Rp) {
+                float left = v[i] * down;
+#pragma unroll
+                for (int k = 0; k < NP; ++k) {
+                    const E h = AdpType<E>::round(left);
+                    const float w = AdpType<E>::widen(h);
+                    frag[((size_t)k * ADP_TOK + warp) * pitch + r] = h;
+                    left = fabsf(w) < INFINITY ? left - w : 0.f;
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- out: 32 columns to a warp at a time, four neighbours of them to a lane ----
+    const int ta = g.tok[quad * 2], tb = g.tok[quad * 2 + 1];
+    const float backa = s_back[quad * 2], backb = s_back[quad * 2 + 1];
+    for (int u = u0 + warp; u < u1; u += ADP_WARPS) {
+        const int n = u * 32 + row * 4;
+        float acc[2][4] = {};
+        for (int r0 = 0; r0 < R; r0 += 32) {
+            const int r = r0 + quad * 8;
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = make_uint4(0, 0, 0, 0);
+                if (n + i < N && r < R) w[i] = adp_ld16(B + (size_t)(n + i) * R + r);
+            }
+#pragma unroll
+            for (int k = 0; k < NP; ++k) {
+                const uint4 s = adp_ld16(frag + ((size_t)k * ADP_TOK + row) * pitch + r);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    AdpType<E>::mma(acc[i], w[2 * i].x, w[2 * i + 1].x, w[2 * i].y, w[2 * i + 1].y, s.x, s.y);
+                    AdpType<E>::mma(acc[i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, s.z, s.w);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int t = h ? tb : ta;
+            if (t < 0) continue;
+            const float back = h ? backb : backa;
+            const float d[4] = {acc[0][h] * back, acc[0][2 + h] * back, acc[1][h] * back, acc[1][2 + h] * back};
+            O* const o = out + (size_t)t * q.out_stride + n;
+            const O* const y = base ? base + (size_t)t * q.base_stride + n : nullptr;
+            if (q.vec && n + 3 < N) {
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                if (y) adp_load4(y, v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += d[i];
+                adp_store4(o, v);
+            } else {
+                for (int i = 0; i < 4 && n + i < N; ++i) adp_put(o + i, (y ? adp_widen(y[i]) : 0.f) + d[i]);
+            }
+        }
+    }
+}
+
+inline size_t adapter_few_smem(int R, int elem_parts) {
+    return (size_t)(ADP_WARPS + ADP_CTAS) * R * ADP_TOK * 4 + (size_t)elem_parts * ADP_TOK * (((R + 31) & ~31) + 8) * 2;
+}
+
+// Tokens of a longer call ordered by adapter, and its groups: one CTA, a counting sort.  Where a token lands within its adapter depends on the order of the
+// atomics, its result does not: columns of a product do not see each other.
+__global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __grid_constant__ AdapterParams p) {
+    __shared__ int s_count[ADP_MAX_ADAPTERS + 1], s_first[ADP_MAX_ADAPTERS + 1], s_warp[2][ADP_PLAN_THREADS / 32], s_total[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = p.adapters + (p.copy ? 1 : 0);
+    for (int i = tid; i <= ADP_MAX_ADAPTERS; i += ADP_PLAN_THREADS) s_count[i] = 0;
+    if (tid < 2) s_total[tid] = 0;
+    pdl_wait();
+    __syncthreads();
+    auto bin_of = [&](int t) {
+        const int id = p.index[t];
+        return id >= 0 && id < p.adapters ? id : (p.copy ? p.adapters : -1);
+    };
+    for (int t0 = 0; t0 < p.tokens; t0 += ADP_PLAN_THREADS) {
+        const int b = t0 + tid < p.tokens ? bin_of(t0 + tid) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, b);
+        if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&s_count[b], __popc(same));
+    }
+    __syncthreads();
+    // exclusive sums over the bins of tokens and of groups, ADP_PLAN_THREADS bins at a time
+    for (int b0 = 0; b0 < bins; b0 += ADP_PLAN_THREADS) {
+        const int b = b0 + tid, c = b < bins ? s_count[b] : 0, gr = (c + ADP_TOK - 1) / ADP_TOK;
+        int st = c, sg = gr;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int vt = __shfl_up_sync(0xffffffffu, st, o), vg = __shfl_up_sync(0xffffffffu, sg, o);
+            if (lane >= o) { st += vt; sg += vg; }
+        }
+        if (lane == 31) { s_warp[0][warp] = st; s_warp[1][warp] = sg; }
+        __syncthreads();
+        int at = s_total[0] + st - c, ag = s_total[1] + sg - gr;
+        for (int w = 0; w < warp; ++w) { at += s_warp[0][w]; ag += s_warp[1][w]; }
+        if (b < bins) {
+            s_first[b] = at;
+            for (int i = 0; i < gr; ++i) p.plan.group()[ag + i] = make_int2(b == p.adapters ? -1 : b, at + i * ADP_TOK);
+        }
+        __syncthreads();
+        if (tid == ADP_PLAN_THREADS - 1) { s_total[0] = at + c; s_total[1] = ag + gr; }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        p.plan.count()[0] = s_total[1];
+        p.plan.count()[1] = s_total[0];
+    }
+    for (int t0 = 0; t0 < p.tokens; t0 += ADP_PLAN_THREADS) {
+        const int b = t0 + tid < p.tokens ? bin_of(t0 + tid) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, b);
+        int at = 0;
+        const int leader = __ffs(same) - 1;
+        if (b >= 0 && lane == leader) at = atomicAdd(&s_first[b], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
+        if (b >= 0) p.plan.place()[at] = t0 + tid;
+    }
+}
+
+}  // namespace b200

@@ -20,6 +20,7 @@
 #include <string>
 #include <vector>
 
+#include "host.cuh"
 #include "kx_rows.cuh"
 #include "gemm.cuh"
 #include "gemm_wide.cuh"
@@ -60,23 +61,8 @@ namespace b200 {
 // =========================================================================================
 // errors
 // =========================================================================================
-struct Error : std::runtime_error {
-    int code;
-    Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-#define CK(call)                                                                                         \
-    do {                                                                                                 \
-        cudaError_t e_ = (call);                                                                         \
-        if (e_ != cudaSuccess)                                                                           \
-            throw Error(B200RWKV_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_) + " @" +   \
-                                               __FILE__ + ":" + std::to_string(__LINE__) + watchdog_report()); \
-    } while (0)
-#define REQUIRE(cond, code, msg)                 \
-    do {                                         \
-        if (!(cond)) throw Error((code), (msg)); \
-    } while (0)
-
 static thread_local std::string g_err;
+std::string& last_error_text() { return g_err; }
 
 // Bring-up switches exist only in the debug build (-DB200RWKV_DEBUG, `python -m ai00_server_b200.build --debug` ->
 // libb200rwkv_dbg.so): the product library ignores the environment entirely.
@@ -98,7 +84,7 @@ static void watchdog_setup() {
     memset(h, 0, 64);
     g_wd_host = h;
 }
-static std::string watchdog_report() {
+std::string watchdog_report() {
     if (!g_wd_host || (g_wd_host[0] >> 16) != 0xDEADu) return "";
     char buf[256];
     snprintf(buf, sizeof buf, " [device watchdog: code=%u block=%u thread=%u a0=0x%x a1=%u a2=%u]", g_wd_host[0] & 0xFFFFu, g_wd_host[1],
@@ -386,17 +372,6 @@ static bool state_from_st(const StFile& st, int L, int H, int N, int C, std::vec
 // =========================================================================================
 static inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 static inline int rup(int a, int b) { return cdiv(a, b) * b; }
-
-// dynamic shared memory a kernel may be launched with.  The limit belongs to the process, not to an engine: it is only ever raised, so that a
-// narrower model loaded later leaves the launches of a wider one valid
-template <typename K>
-static void allow_smem(K* kern, size_t bytes) {
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lk(mu);
-    cudaFuncAttributes a;
-    CK(cudaFuncGetAttributes(&a, kern));
-    if ((size_t)a.maxDynamicSharedSizeBytes < bytes) CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-}
 
 enum KClass { KC_GEMM = 0, KC_WKV = 1, KC_LN = 2, KC_OTHER = 3 };
 
@@ -2394,28 +2369,6 @@ int32_t Group::spmd(const std::function<int32_t(int)>& fn) {
 // =========================================================================================
 // C ABI
 // =========================================================================================
-// Error text is thread-local: the reference makes engine calls from two tasks (infer / softmax, run.rs:1232-1237) and a
-// per-engine string would race between them.  b200rwkv_last_error() returns the message of the calling thread's last failure.
-#define API_BEGIN(e)                            \
-    std::string* errp_ = &g_err;                \
-    (void)(e);                                  \
-    try {
-#define API_END                                  \
-    }                                            \
-    catch (const Error& ex) {                    \
-        *errp_ = ex.what();                      \
-        return ex.code;                          \
-    }                                            \
-    catch (const std::exception& ex) {           \
-        *errp_ = ex.what();                      \
-        return B200RWKV_ERR_INVALID;             \
-    }                                            \
-    catch (...) {                                \
-        *errp_ = "unknown exception";            \
-        return B200RWKV_ERR_INVALID;             \
-    }                                            \
-    return B200RWKV_OK;
-
 extern "C" {
 
 int32_t b200rwkv_info_from_st(const uint8_t* st, size_t len, b200rwkv_info* out) {

@@ -1,0 +1,193 @@
+// Operators on device memory: adapters of many requests (adapters.cuh) and adjusted logits (logits.cuh), their C entries and the launches
+// the engine makes of them.
+#include "operators.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+
+namespace b200 {
+
+// a kernel's dynamic shared memory, once for every device that launches it
+template <auto KERN>
+static void prepare(size_t bytes) {
+    static std::atomic<unsigned long long> done{0};
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return;
+    allow_smem(KERN, bytes);
+    done.fetch_or(bit, std::memory_order_release);
+}
+
+template <typename P>
+static void launch(void (*kern)(P), dim3 grid, int threads, size_t smem, cudaStream_t s, const P& p) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    // starts while the kernel in front drains; every kernel here waits for that one's end before it reads anything
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    CK(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+size_t adapters_workspace(int tokens, int adapters) {
+    if (tokens <= ADP_INLINE) return 0;
+    return AdapterPlan::ints(tokens, adapter_groups(tokens, adapters)) * 4;
+}
+
+void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan_kernel, dim3(1), ADP_PLAN_THREADS, 0, s, p); }
+
+template <typename E, typename O>
+static void apply(cudaStream_t s, const AdapterParams& p, int nparts) {
+    int R = 0;
+    for (int i = 0; i < nparts; ++i) R = std::max(R, p.part[i].R);
+    const size_t smem = adapter_few_smem(R, AdpParts<E, O>::N);
+    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
+    launch(adapter_few_kernel<E, O>, dim3(ADP_CTAS * adapter_groups(p.tokens, p.adapters), nparts), ADP_THREADS, smem, s, p);
+}
+
+void adapters_apply(cudaStream_t s, const AdapterParams& p, int nparts, int type, int out_type) {
+    if (type == B200RWKV_TYPE_F16) {
+        if (out_type == B200RWKV_TYPE_F32) apply<__half, float>(s, p, nparts);
+        else apply<__half, __half>(s, p, nparts);
+    } else {
+        if (out_type == B200RWKV_TYPE_F32) apply<__nv_bfloat16, float>(s, p, nparts);
+        else apply<__nv_bfloat16, __nv_bfloat16>(s, p, nparts);
+    }
+}
+
+template <typename E>
+static void logits_launch(cudaStream_t s, const LogitsParams& p, int rows, size_t smem) {
+    prepare<logits_kernel<E>>(LOGITS_SMEM_MAX);
+    launch(logits_kernel<E>, dim3(rows * LOGITS_CTAS), LOGITS_THREADS, smem, s, p);
+}
+
+void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type) {
+    const int size = type == B200RWKV_TYPE_F32 ? 4 : 2;
+    p.slice = ((p.V + LOGITS_CTAS - 1) / LOGITS_CTAS + 3) & ~3;
+    p.sub = p.hist_off || p.bias_off ? std::min(p.slice, LOGITS_SUB) : 0;
+    const size_t lists = (size_t)p.sub * 8, slice = (size_t)p.slice * 4;
+    p.buffered = slice + lists <= LOGITS_SMEM_MAX;
+    p.vec = (uintptr_t)p.in % (4 * size) == 0 && p.in_stride % 4 == 0 && (uintptr_t)p.out % 16 == 0 && p.out_stride % 4 == 0;
+    const size_t smem = lists + (p.buffered ? slice : 0);
+    if (type == B200RWKV_TYPE_F32) logits_launch<float>(s, p, rows, smem);
+    else if (type == B200RWKV_TYPE_F16) logits_launch<__half>(s, p, rows, smem);
+    else logits_launch<__nv_bfloat16>(s, p, rows, smem);
+}
+
+// the calling thread's device for the length of a call
+struct OnDevice {
+    int before = 0;
+    explicit OnDevice(int device) {
+        CK(cudaGetDevice(&before));
+        if (before != device) CK(cudaSetDevice(device));
+        else before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters) {
+    if (tokens < 0 || adapters < 1 || adapters > B200RWKV_MAX_ADAPTERS) {
+        last_error_text() = "op_adapters_workspace: bad argument";
+        return B200RWKV_ERR_INVALID;
+    }
+    return (int64_t)adapters_workspace(tokens, adapters);
+}
+
+int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* q) {
+    API_BEGIN((b200rwkv_engine*)nullptr)
+    static_assert(B200RWKV_MAX_PARTS == ADP_MAX_PARTS && B200RWKV_MAX_RANK == ADP_MAX_RANK && B200RWKV_MAX_ADAPTERS == ADP_MAX_ADAPTERS, "limits");
+    REQUIRE(q && q->struct_bytes == sizeof(*q), B200RWKV_ERR_INVALID, "op_adapters: struct_bytes must be sizeof(b200rwkv_adapters)");
+    REQUIRE(q->type == B200RWKV_TYPE_F16 || q->type == B200RWKV_TYPE_BF16, B200RWKV_ERR_UNSUPPORTED, "op_adapters: x, a and b are f16 or bf16");
+    REQUIRE(q->out_type == q->type || q->out_type == B200RWKV_TYPE_F32, B200RWKV_ERR_UNSUPPORTED, "op_adapters: out is f32 or of the type of x");
+    REQUIRE(q->tokens >= 0 && q->tokens <= (1 << 20), B200RWKV_ERR_INVALID, "op_adapters: tokens must be in [0, 2^20]");
+    REQUIRE(q->adapters >= 1 && q->adapters <= B200RWKV_MAX_ADAPTERS, B200RWKV_ERR_INVALID, "op_adapters: adapters must be in [1, 1024]");
+    REQUIRE(q->num_parts >= 1 && q->num_parts <= B200RWKV_MAX_PARTS && q->parts, B200RWKV_ERR_INVALID, "op_adapters: num_parts must be in [1, 8]");
+    REQUIRE(q->tokens == 0 || (q->index && q->scale), B200RWKV_ERR_INVALID, "op_adapters: null index or scale");
+    AdapterParams p;
+    memset(&p, 0, sizeof(p));
+    p.tokens = q->tokens;
+    p.adapters = q->adapters;
+    p.index = q->index;
+    p.scale = q->scale;
+    const int osize = q->out_type == B200RWKV_TYPE_F32 ? 4 : 2;
+    for (int i = 0; i < q->num_parts; ++i) {
+        const b200rwkv_adapter_part& s = q->parts[i];
+        AdapterPart& d = p.part[i];
+        REQUIRE(s.in_features >= 8 && s.in_features % 8 == 0 && s.in_features <= (1 << 24), B200RWKV_ERR_UNSUPPORTED, "op_adapters: in_features must be a multiple of 8");
+        REQUIRE(s.out_features >= 1 && s.out_features <= (1 << 24), B200RWKV_ERR_INVALID, "op_adapters: out_features must be positive");
+        REQUIRE(s.rank >= 8 && s.rank % 8 == 0 && s.rank <= B200RWKV_MAX_RANK, B200RWKV_ERR_UNSUPPORTED, "op_adapters: rank must be a multiple of 8, at most 256");
+        if (q->tokens == 0) continue;
+        REQUIRE(s.x && s.a && s.b && s.out, B200RWKV_ERR_INVALID, "op_adapters: null x, a, b or out");
+        REQUIRE(s.x_stride >= s.in_features && s.out_stride >= s.out_features && (!s.base || s.base_stride >= s.out_features), B200RWKV_ERR_INVALID,
+                "op_adapters: rows overlap (a stride is smaller than a row)");
+        REQUIRE(s.x_stride % 8 == 0 && ((uintptr_t)s.x | (uintptr_t)s.a | (uintptr_t)s.b) % 16 == 0, B200RWKV_ERR_INVALID,
+                "op_adapters: rows of x, a and b must start on 16-byte boundaries");
+        REQUIRE(((uintptr_t)s.out | (uintptr_t)s.base) % osize == 0, B200RWKV_ERR_INVALID, "op_adapters: misaligned base or out");
+        d.x = s.x; d.x_stride = s.x_stride;
+        d.a = s.a; d.b = s.b;
+        d.base = s.base; d.base_stride = s.base_stride;
+        d.out = s.out; d.out_stride = s.out_stride;
+        d.K = s.in_features; d.N = s.out_features; d.R = s.rank;
+        d.vec = ((uintptr_t)s.out | (uintptr_t)s.base) % (4 * osize) == 0 && s.out_stride % 4 == 0 && (!s.base || s.base_stride % 4 == 0);
+        if (s.base != s.out || s.base_stride != s.out_stride) p.copy = 1;
+    }
+    if (q->tokens == 0) return B200RWKV_OK;
+    const size_t need = adapters_workspace(q->tokens, q->adapters);
+    REQUIRE(need == 0 || (q->workspace && (uintptr_t)q->workspace % 16 == 0 && q->workspace_bytes >= need), B200RWKV_ERR_INVALID,
+            "op_adapters: workspace is missing, misaligned or smaller than b200rwkv_op_adapters_workspace");
+    OnDevice on(device);
+    if (need) {
+        p.plan.base = (int*)q->workspace;
+        p.plan.tokens = q->tokens;
+        p.plan.most = adapter_groups(q->tokens, q->adapters);
+        adapters_plan((cudaStream_t)stream, p);
+    }
+    adapters_apply((cudaStream_t)stream, p, q->num_parts, q->type, q->out_type);
+    API_END
+}
+
+int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* q) {
+    API_BEGIN((b200rwkv_engine*)nullptr)
+    REQUIRE(q && q->struct_bytes == sizeof(*q), B200RWKV_ERR_INVALID, "op_logits: struct_bytes must be sizeof(b200rwkv_logits)");
+    REQUIRE(q->type >= B200RWKV_TYPE_F32 && q->type <= B200RWKV_TYPE_BF16, B200RWKV_ERR_UNSUPPORTED, "op_logits: logits are f32, f16 or bf16");
+    REQUIRE(q->kind >= B200RWKV_LOGITS && q->kind <= B200RWKV_LOG_PROBS, B200RWKV_ERR_INVALID, "op_logits: kind must be logits, probabilities or log-probabilities");
+    REQUIRE(q->rows >= 0 && q->rows <= (1 << 24) && q->vocab >= 1 && q->vocab <= (1 << 28), B200RWKV_ERR_INVALID, "op_logits: rows or vocab out of range");
+    if (q->rows == 0) return B200RWKV_OK;
+    const int size = q->type == B200RWKV_TYPE_F32 ? 4 : 2;
+    REQUIRE(q->logits && q->out, B200RWKV_ERR_INVALID, "op_logits: null logits or out");
+    REQUIRE(q->logits_stride >= q->vocab && q->out_stride >= q->vocab, B200RWKV_ERR_INVALID, "op_logits: rows overlap (a stride is smaller than the vocabulary)");
+    REQUIRE((uintptr_t)q->logits % size == 0 && (uintptr_t)q->out % 4 == 0, B200RWKV_ERR_INVALID, "op_logits: misaligned logits or out");
+    REQUIRE(!q->history_offset || q->history, B200RWKV_ERR_INVALID, "op_logits: history offsets without tokens");
+    REQUIRE(!q->bias_offset || (q->bias_token && q->bias_value), B200RWKV_ERR_INVALID, "op_logits: bias offsets without tokens or values");
+    REQUIRE(!q->allow || q->allow_rows >= (q->allow_row ? 0 : q->rows), B200RWKV_ERR_INVALID, "op_logits: fewer masks than rows");
+    LogitsParams p;
+    memset(&p, 0, sizeof(p));
+    p.in = q->logits; p.in_stride = q->logits_stride;
+    p.out = q->out; p.out_stride = q->out_stride;
+    p.V = q->vocab; p.kind = q->kind;
+    p.controls = q->controls;
+    p.hist_off = q->history_offset; p.hist = q->history; p.hist_from = q->history_from;
+    p.allow = q->allow; p.words = (q->vocab + 31) / 32; p.allow_rows = q->allow_rows; p.allow_row = q->allow_row;
+    p.bias_off = q->bias_offset; p.bias_tok = q->bias_token; p.bias_val = q->bias_value;
+    OnDevice on(device);
+    logits_rows((cudaStream_t)stream, p, q->rows, q->type);
+    API_END
+}
+
+}  // extern "C"

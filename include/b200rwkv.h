@@ -274,6 +274,90 @@ int32_t b200rwkv_op_wkv(int32_t device, int32_t version, int32_t T, int32_t H, c
                         const float* w, const float* u, const float* a, const float* k_k, const float* k_a, const float* r_k,
                         const float* g, const float* lnx_w, const float* lnx_b, float* state, float* out);
 
+/* ---- Operators on device memory --------------------------------------------------------------------------------------------
+ * What the engine runs on its own buffers for the requests of a batch, for callers that hold theirs on the GPU.  All pointers
+ * in the two structs are device memory of `device` (the parts array and the structs themselves are host memory, read
+ * during the call).  A call only enqueues kernels on `stream` (a cudaStream_t of that device; NULL: its default stream): it neither
+ * allocates nor synchronises, can be captured into a graph, and leaves the calling thread's current device as it was.  Calls
+ * on different streams may overlap; each needs its own workspace for that long, and so does every graph that may run beside
+ * another.  Wrong arguments that the host can see are refused (B200RWKV_ERR_INVALID, _UNSUPPORTED) before anything is
+ * enqueued.  Set struct_bytes = sizeof(the struct) and zero what is not used. */
+#define B200RWKV_TYPE_F32 0
+#define B200RWKV_TYPE_F16 1
+#define B200RWKV_TYPE_BF16 2
+
+/* Low-rank adapters of many requests beside shared projections: for every part (a projection) and token t with a = index[t]
+ *     out[t, n] = base[t, n] + scale[a] * sum_r (sum_k x[t, k] A[a][r, k]) B[a][n, r]
+ * A token whose index names no adapter (negative, or >= adapters) keeps its base (zeros without one).  Sums are f32, the result is
+ * rounded once to out_type.  The load-time counterpart is b200rwkv_options.lora_st (reference lib.rs:466-485). */
+#define B200RWKV_MAX_PARTS 8
+#define B200RWKV_MAX_RANK 256
+#define B200RWKV_MAX_ADAPTERS 1024
+typedef struct {
+    const void* x;               /* [tokens, in] of `type`; rows x_stride elements apart (a multiple of 8) */
+    int64_t x_stride;
+    const void* a;               /* [adapters, rank, in] of `type` */
+    const void* b;               /* [adapters, out_features, rank] of `type` */
+    const void* base;            /* [tokens, out_features] of `out_type`, or NULL; may be `out` itself, else apart from it */
+    int64_t base_stride;
+    void* out;                   /* [tokens, out_features] of `out_type`; nothing else is written */
+    int64_t out_stride;
+    int32_t in_features;         /* a multiple of 8 */
+    int32_t out_features;
+    int32_t rank;                /* a multiple of 8, at most B200RWKV_MAX_RANK (pad smaller adapters with zero rows) */
+    int32_t reserved;
+} b200rwkv_adapter_part;
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t type;                /* B200RWKV_TYPE_F16 or _BF16: x, a, b */
+    int32_t out_type;            /* `type`, or B200RWKV_TYPE_F32: base, out */
+    int32_t tokens;
+    int32_t adapters;            /* 1 .. B200RWKV_MAX_ADAPTERS */
+    int32_t num_parts;           /* 1 .. B200RWKV_MAX_PARTS */
+    const int32_t* index;        /* [tokens] */
+    const float* scale;          /* [adapters] */
+    const b200rwkv_adapter_part* parts;      /* host array */
+    void* workspace;             /* b200rwkv_op_adapters_workspace bytes, 16-byte aligned; contents before and after do not matter */
+    size_t workspace_bytes;
+} b200rwkv_adapters;
+int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters);      /* 0: none is needed; negative: a status */
+int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* args);
+
+/* Rows of logits adjusted for their requests, as logits, probabilities or log-probabilities.  For row i, token t, with the row's
+ * controls (repetition, presence, frequency, decay, temperature; 1, 0, 0, 1, 1 without them) and its history h_0 .. h_{n-1}, oldest first:
+ *     l = in[i, t];   where t is in the history   l = l > 0 ? l / repetition : l * repetition
+ *     where h_j = t for some j >= history_from[i]   l -= presence + frequency * sum over those j of decay^(n - 1 - j)
+ *     l += the last bias value listed for t;   l = -inf where bit t of the row's mask is 0;   l /= temperature
+ * A row of which the mask leaves nothing has probabilities 0 and log-probabilities -inf; a NaN that the mask leaves makes a row of
+ * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number makes any row NaN; decay is
+ * taken into [0, 1].  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
+ * sampler/bnf.rs:35-38, run.rs:679-681 and softmax (run.rs:1179) of the samplers that need whole rows. */
+#define B200RWKV_LOGITS 0
+#define B200RWKV_PROBS 1
+#define B200RWKV_LOG_PROBS 2
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t type;                /* B200RWKV_TYPE_*: logits */
+    int32_t kind;                /* B200RWKV_LOGITS, _PROBS, _LOG_PROBS */
+    int32_t rows;
+    int32_t vocab;
+    int32_t allow_rows;          /* rows of `allow` */
+    const void* logits;          /* [rows, vocab], logits_stride elements apart */
+    int64_t logits_stride;
+    float* out;                  /* [rows, vocab], out_stride apart; may be `logits` itself where those are f32 rows of the same stride */
+    int64_t out_stride;
+    const float* controls;       /* [rows, 5] or NULL */
+    const int32_t* history_offset;   /* [rows + 1], ascending, or NULL: row i's history is history[offset[i] .. offset[i+1]) */
+    const int32_t* history;
+    const int32_t* history_from;     /* [rows] or NULL: everything counts for presence and frequency */
+    const uint32_t* allow;       /* [allow_rows, (vocab + 31) / 32] or NULL: bit t % 32 of word t / 32 */
+    const int32_t* allow_row;    /* [rows] or NULL: row i has mask i; a row outside [0, allow_rows) has none */
+    const int32_t* bias_offset;  /* [rows + 1] or NULL */
+    const int32_t* bias_token;
+    const float* bias_value;
+} b200rwkv_logits;
+int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* args);
+
 /* Kernels launched by this engine's forward steps since creation (graph replays counted by their kernel nodes). */
 int32_t b200rwkv_launch_count(b200rwkv_engine*, int64_t* total);
 

@@ -1,0 +1,91 @@
+"""Refusals of the operators on device memory: every wrong argument that the host can see is an error before anything is enqueued (no GPU needed)."""
+import ctypes as C
+
+import pytest
+
+from ai00_server_b200 import capi
+
+
+def _adapters(**change):
+    part = capi.AdapterPart(x=4096, x_stride=64, a=4096, b=4096, base=4096, base_stride=32, out=8192, out_stride=32, in_features=64, out_features=32, rank=16)
+    q = capi.Adapters(struct_bytes=C.sizeof(capi.Adapters), type=capi.TYPE_F16, out_type=capi.TYPE_F32, tokens=4, adapters=2, num_parts=1, index=4096, scale=4096)
+    for k, v in change.items():
+        setattr(part if hasattr(part, k) else q, k, v)
+    q.parts = (capi.AdapterPart * 1)(part) if change.get("parts", 1) else None
+    q._keep = q.parts
+    return q
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"struct_bytes": 8}, capi.ERR_INVALID), ({"type": capi.TYPE_F32}, capi.ERR_UNSUPPORTED), ({"type": 9}, capi.ERR_UNSUPPORTED),
+    ({"out_type": capi.TYPE_BF16}, capi.ERR_UNSUPPORTED), ({"tokens": -1}, capi.ERR_INVALID), ({"tokens": (1 << 20) + 1}, capi.ERR_INVALID),
+    ({"adapters": 0}, capi.ERR_INVALID), ({"adapters": 1025}, capi.ERR_INVALID), ({"num_parts": 0}, capi.ERR_INVALID), ({"num_parts": 9}, capi.ERR_INVALID),
+    ({"parts": None}, capi.ERR_INVALID), ({"index": None}, capi.ERR_INVALID), ({"scale": None}, capi.ERR_INVALID),
+    ({"in_features": 60}, capi.ERR_UNSUPPORTED), ({"in_features": 0}, capi.ERR_UNSUPPORTED), ({"out_features": 0}, capi.ERR_INVALID),
+    ({"rank": 12}, capi.ERR_UNSUPPORTED), ({"rank": 264}, capi.ERR_UNSUPPORTED), ({"rank": 0}, capi.ERR_UNSUPPORTED), ({"x": None}, capi.ERR_INVALID),
+    ({"a": None}, capi.ERR_INVALID), ({"b": None}, capi.ERR_INVALID), ({"out": None}, capi.ERR_INVALID), ({"x": 4098}, capi.ERR_INVALID),
+    ({"a": 4104}, capi.ERR_INVALID), ({"b": 4104}, capi.ERR_INVALID), ({"x_stride": 68}, capi.ERR_INVALID), ({"x_stride": 56}, capi.ERR_INVALID),
+    ({"out_stride": 31}, capi.ERR_INVALID), ({"base_stride": 31}, capi.ERR_INVALID), ({"out": 8194}, capi.ERR_INVALID),
+    ({"tokens": 300}, capi.ERR_INVALID),                                             # no workspace
+    ({"tokens": 300, "workspace": 4096, "workspace_bytes": 64}, capi.ERR_INVALID),
+    ({"tokens": 300, "workspace": 4100, "workspace_bytes": 1 << 20}, capi.ERR_INVALID)])
+def test_op_adapters_refuses(change, code):
+    q = _adapters(**change)
+    with pytest.raises(capi.B200Error) as ei:
+        capi.check(capi.lib().b200rwkv_op_adapters(0, None, C.byref(q)))
+    assert ei.value.code == code
+    assert "op_adapters" in str(ei.value)
+
+
+def test_op_adapters_null_struct_and_no_tokens():
+    assert capi.lib().b200rwkv_op_adapters(0, None, None) == capi.ERR_INVALID
+    assert capi.lib().b200rwkv_op_adapters(0, None, C.byref(_adapters(tokens=0, index=None, scale=None, x=None, out=None))) == 0
+
+
+def test_op_adapters_workspace():
+    lib = capi.lib()
+    assert lib.b200rwkv_op_adapters_workspace(256, 4) == 0
+    assert lib.b200rwkv_op_adapters_workspace(257, 4) > 257 * 4
+    assert lib.b200rwkv_op_adapters_workspace(-1, 4) == capi.ERR_INVALID
+    assert lib.b200rwkv_op_adapters_workspace(8, 0) == capi.ERR_INVALID
+    assert lib.b200rwkv_op_adapters_workspace(8, 1025) == capi.ERR_INVALID
+
+
+def _logits(**change):
+    q = capi.Logits(struct_bytes=C.sizeof(capi.Logits), type=capi.TYPE_F32, kind=capi.PROBS, rows=2, vocab=100, logits=4096, logits_stride=100, out=8192, out_stride=100)
+    for k, v in change.items():
+        setattr(q, k, v)
+    return q
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"struct_bytes": 4}, capi.ERR_INVALID), ({"type": 3}, capi.ERR_UNSUPPORTED), ({"type": -1}, capi.ERR_UNSUPPORTED), ({"kind": 3}, capi.ERR_INVALID),
+    ({"kind": -1}, capi.ERR_INVALID), ({"rows": -1}, capi.ERR_INVALID), ({"vocab": 0}, capi.ERR_INVALID), ({"logits": None}, capi.ERR_INVALID),
+    ({"out": None}, capi.ERR_INVALID), ({"logits_stride": 99}, capi.ERR_INVALID), ({"out_stride": 99}, capi.ERR_INVALID), ({"logits": 4098}, capi.ERR_INVALID),
+    ({"out": 8194}, capi.ERR_INVALID), ({"history_offset": 4096}, capi.ERR_INVALID), ({"bias_offset": 4096}, capi.ERR_INVALID),
+    ({"bias_offset": 4096, "bias_token": 4096}, capi.ERR_INVALID), ({"allow": 4096, "allow_rows": 1}, capi.ERR_INVALID),
+    ({"allow": 4096, "allow_rows": -1, "allow_row": 4096}, capi.ERR_INVALID)])
+def test_op_logits_refuses(change, code):
+    with pytest.raises(capi.B200Error) as ei:
+        capi.check(capi.lib().b200rwkv_op_logits(0, None, C.byref(_logits(**change))))
+    assert ei.value.code == code
+    assert "op_logits" in str(ei.value)
+
+
+def test_op_logits_null_struct_and_no_rows():
+    assert capi.lib().b200rwkv_op_logits(0, None, None) == capi.ERR_INVALID
+    assert capi.lib().b200rwkv_op_logits(0, None, C.byref(_logits(rows=0, logits=None, out=None))) == 0
+
+
+def test_tensors_that_do_not_fit():
+    torch = pytest.importorskip("torch")
+    from ai00_server_b200 import device_ops
+    x, a, b = torch.zeros(4, 64), torch.zeros(2, 8, 64), torch.zeros(2, 16, 8)
+    with pytest.raises(capi.B200Error):              # not in GPU memory
+        device_ops.low_rank(x, a, b, torch.zeros(4, dtype=torch.int32), torch.ones(2))
+    with pytest.raises(capi.B200Error):
+        device_ops.low_rank([x], [a, a], [b], torch.zeros(4, dtype=torch.int32), torch.ones(2))
+    with pytest.raises(capi.B200Error):
+        device_ops.logits(torch.zeros(2, 10))
+    with pytest.raises(capi.B200Error):
+        device_ops.logits(torch.zeros(20))
