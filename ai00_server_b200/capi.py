@@ -64,6 +64,13 @@ class Logits(C.Structure):
                 ("bias_value", C.c_void_p)]
 
 
+class RowControls(C.Structure):
+    """b200rwkv_row_controls."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("kind", C.c_int32), ("slots", C.c_void_p), ("controls", C.c_void_p), ("history_offset", C.c_void_p),
+                ("history", C.c_void_p), ("history_from", C.c_void_p), ("allow_bits", C.c_void_p), ("bias_offset", C.c_void_p), ("bias_token", C.c_void_p),
+                ("bias_value", C.c_void_p)]
+
+
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 LOGITS, PROBS, LOG_PROBS = 0, 1, 2
 MAX_PARTS, MAX_RANK, MAX_ADAPTERS = 8, 256, 1024
@@ -109,6 +116,10 @@ SYMBOLS = [
     ("b200rwkv_read_state", C.c_int32, [C.POINTER(Info), _P, C.c_size_t, _P]),
     ("b200rwkv_softmax", C.c_int32, [_P, C.c_int32, _P, _P]),
     ("b200rwkv_sample_topk", C.c_int32, [_P, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P]),
+    ("b200rwkv_sample_rows", C.c_int32, [_P, C.c_int32, C.POINTER(RowControls), _P]),
+    ("b200rwkv_adapter_load", C.c_int32, [_P, _P, C.c_size_t, C.c_float, C.POINTER(C.c_uint64)]),
+    ("b200rwkv_adapter_free", C.c_int32, [_P, C.c_uint64]),
+    ("b200rwkv_slot_adapter", C.c_int32, [_P, C.c_int32, C.c_uint64]),
     ("b200rwkv_host_alloc", C.c_int32, [C.c_size_t, C.POINTER(_P)]),
     ("b200rwkv_host_free", None, [_P]),
     ("b200rwkv_bench_decode", C.c_int32, [_P, C.c_int32, _P, _P, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_float), C.POINTER(C.c_int64), _P]),

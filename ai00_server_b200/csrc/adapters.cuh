@@ -14,64 +14,9 @@
 #pragma once
 #include <cuda_bf16.h>
 
-#include "common.cuh"
+#include "operators.cuh"
 
 namespace b200 {
-
-constexpr int ADP_CTAS = 8, ADP_THREADS = 256, ADP_WARPS = ADP_THREADS / 32;
-constexpr int ADP_TOK = 8;                       // tokens of a group: the N of the products
-constexpr int ADP_MAX_PARTS = 8, ADP_MAX_RANK = 256, ADP_MAX_ADAPTERS = 1024;
-constexpr int ADP_INLINE = ADP_THREADS;          // tokens of a call whose groups every CTA finds by itself; more take adapter_plan_kernel
-constexpr int ADP_PLAN_THREADS = 1024;
-
-// one adapter of one projection, where adapters lie apart
-struct AdapterEntry {
-    const void* a;
-    const void* b;
-    int rank;                    // 0: the adapter leaves this projection alone
-    float scale;
-};
-
-struct AdapterPart {
-    const void* x;               // rows of K, or (x_a16) the A16 layout of common.cuh with x_th as its height
-    long long x_stride;          // elements
-    int x_a16, x_th;
-    int x_lo;                    // rows to the low half of split operands (0: none)
-    const void* a;               // [adapters][R][K]
-    const void* b;               // [adapters][N][R]
-    const AdapterEntry* table;   // instead of a and b
-    const void* base;
-    long long base_stride;
-    void* out;
-    long long out_stride;
-    int K, N, R;                 // R: the largest rank
-    int vec;                     // rows of base and out take accesses of four elements
-};
-
-// groups of more tokens than ADP_INLINE: [0] = groups, then {adapter, first place} of each, then tokens by place
-struct AdapterPlan {
-    int* base;
-    int tokens, most;            // most: groups there can be
-    __host__ __device__ int* count() const { return base; }
-    __host__ __device__ int2* group() const { return reinterpret_cast<int2*>(base + 4); }
-    __host__ __device__ int* place() const { return base + 4 + 2 * (size_t)most; }
-    __host__ __device__ static size_t ints(int tokens, int most) { return 4 + 2 * (size_t)most + tokens; }
-};
-
-struct AdapterParams {
-    int tokens, adapters;
-    int copy;                    // tokens without an adapter have their base copied (base and out differ)
-    const int* index;
-    const float* scale;
-    AdapterPlan plan;
-    AdapterPart part[ADP_MAX_PARTS];
-};
-
-// groups of up to ADP_TOK tokens that `tokens` tokens can need: all with their own adapter, or full groups and a broken one for each adapter (and for none)
-__host__ __device__ inline int adapter_groups(int tokens, int adapters) {
-    const long long full = (long long)adapters + 1 + tokens / ADP_TOK;
-    return (int)(full < tokens ? full : tokens);
-}
 
 template <typename E> struct AdpType;
 template <> struct AdpType<__half> {

@@ -55,6 +55,7 @@
 #include "sink_attn.cuh"
 #include "prompt_attn.cuh"
 #include "short_attn.cuh"
+#include "slot_adapters.cuh"
 
 namespace b200 {
 
@@ -388,6 +389,7 @@ struct GemmLaunch {
     int total_tiles = 0;
     size_t weight_bytes = 0;   // algorithmic (unpadded) weight bytes streamed (f16, or codes + block parameters)
     int qtype = QT_NONE;       // weight format of every segment of the launch (qgemm.cuh)
+    int site[GEMM_MAX_SEG];    // projection matrix that slots may have adapters for (-1: none)
 };
 
 struct SegDesc {
@@ -641,7 +643,36 @@ struct b200rwkv_engine {
                      const uint32_t* allow_bits, const int32_t* bias_off, const uint32_t* bias_tok, const float* bias_val,
                      int top_k, uint32_t* ids_out, float* probs_out);
 
+    float* sr_out = nullptr;           // device rows of sample_rows
+    int sr_cap = 0;
+    void sample_rows(int nrows, const b200rwkv_row_controls& q, float* out);
+
     std::mutex mu, sm_mu;
+
+    // adapters of slots (slot_adapters.cuh; RWKV models on one GPU): made with the first one that is loaded
+    struct AdapterSite { std::string base; int K, N; };
+    struct LoadedAdapter { uint64_t id = 0; void* buf = nullptr; };
+    std::vector<AdapterSite> sites;            // projection matrices, in the order of their launches
+    std::vector<LoadedAdapter> pool;
+    std::vector<int> slot_adapter;             // place in the pool of each slot's adapter, -1: none
+    uint64_t next_adapter = 1;
+    int adapter_rank = 0;                      // the largest loaded so far: what the launches of a step reserve
+    bool adapters_on = false;                  // some slot of the step being enqueued has one
+    AdapterEntry* d_entries = nullptr;         // [site][pool]
+    int *d_slot_adapter = nullptr, *d_index_tok = nullptr;
+    uint8_t* adapter_ws = nullptr;             // plans of a long step's tokens and logits rows
+    float* adapter_tmp = nullptr;              // sums of projections that end in an activation
+    int adapter_site(const SegDesc& d);
+    void adapter_setup();
+    size_t adapter_ws_bytes() const;
+    uint64_t adapter_load(const StFile& st, float alpha);
+    int adapter_place(uint64_t id) const;
+    void adapter_free(uint64_t id);
+    void adapter_bind(int slot, uint64_t id);
+    AdapterParams adapter_params(int rows, bool out_rows) const;
+    void adapter_begin(cudaStream_t s, const MetaView& mv, int rows, int out_rows, Profiler* prof);
+    void adapter_redirect(const GemmLaunch& g, GemmParams& gp, int rows);
+    void adapter_add(const GemmLaunch& g, const GemmParams& was, const GemmParams& gp, int rows, int th, bool tiles, bool split, cudaStream_t s, Profiler* prof);
 
     // families that come with a config.json (Kemirax: kemirax.cuh, Degavik: degavik.cuh): set instead of `layers`; one model object,
     // step function, page pool and slot memory for all of them
@@ -753,6 +784,8 @@ b200rwkv_engine::~b200rwkv_engine() {
     if (tk_out) cudaFreeHost(tk_out);
     if (tk_dev) cudaFree(tk_dev);
     if (tk_host) cudaFreeHost(tk_host);
+    if (sr_out) cudaFree(sr_out);
+    for (auto& a : pool) if (a.buf) cudaFree(a.buf);
     if (step_done) cudaEventDestroy(step_done);
     for (auto& ev : meta_ev) if (ev) cudaEventDestroy(ev);
     if (d_hidden_all) cudaFree(d_hidden_all);
@@ -907,10 +940,12 @@ GemmLaunch b200rwkv_engine::make_launch(std::vector<SegDesc>& segs, int force_gr
     g.qtype = qtype;
     const size_t blk_bytes = (size_t)q_block_bytes(qtype);
     int blk = 0, tile = 0, kbmax = 0;
+    std::fill(g.site, g.site + GEMM_MAX_SEG, -1);
     for (size_t i = 0; i < segs.size(); ++i) {
         SegDesc& d = segs[i];
         GemmSeg& sg = g.p.seg[i];
         sg = d.proto;
+        g.site[i] = adapter_site(d);
         // A16 outputs are written as whole 16-byte chunks of 8 rows (gemm.cuh epilogue)
         REQUIRE(sg.out_mode == OUT_F32 || (d.N % 8 == 0 && sg.grp % 8 == 0), B200RWKV_ERR_UNSUPPORTED,
                 "LoRA ranks / hidden size must be multiples of 8");
@@ -1740,6 +1775,8 @@ void b200rwkv_engine::enqueue_step(cudaStream_t s, int MT, int MTR, Profiler* pr
         }
         for (int i = 0; i < g2.p.nseg; ++i)
             if (g2.p.seg[i].out_mode != OUT_F32) g2.p.seg[i].ldo = th_of(g2.p.seg[i].out_tile);      // A16 outputs feed a projection of this step
+        const GemmParams before = g2.p;
+        if (adapters_on) adapter_redirect(g, g2.p, mt * 16);
         const bool pairs = mt >= 8 && maxT > 128;
         if (pairs && g.short_k && !g.chain && mt > 8) {
             // one-block tiles, a CTA per weight tile and 128 tokens
@@ -1750,8 +1787,13 @@ void b200rwkv_engine::enqueue_step(cudaStream_t s, int MT, int MTR, Profiler* pr
         } else {
             launch_gemm(g2, mt, s, prof, split_on && MT == 1);      // split operands only when the whole step is decode-shaped
         }
+        if (adapters_on) {
+            const bool rows_of_head = &g == &head;
+            adapter_add(g, before, g2.p, mt * 16, rows_of_head ? th_rows : th, rows_of_head ? MTR > 8 : tiled, split_on && MT == 1, s, prof);
+        }
     };
     auto gemm = [&](const GemmLaunch& g) { launch_gemm_chained(g, MT); };
+    if (adapters_on) adapter_begin(s, mv, rows, MTR * 16, prof);
     {
         EmbedParams ep = embed;
         ep.meta = mv;
@@ -1916,7 +1958,9 @@ void b200rwkv_engine::run_step(int MT, int MTR, bool runs) {
         launch_total += launches_last_step;
         return;
     }
-    const int key = (((MT * 256 + MTR) * 2 + (runs ? 1 : 0)) * 2 + (scan_alone ? 1 : 0)) * 2 + (runs && scan_few() ? 1 : 0);
+    // (steps with adapters: a graph for each largest rank, whose shared memory it has)
+    const int64_t key = (int64_t)((((MT * 256 + MTR) * 2 + (runs ? 1 : 0)) * 2 + (scan_alone ? 1 : 0)) * 2 + (runs && scan_few() ? 1 : 0)) |
+                        (int64_t)(adapters_on ? adapter_rank : 0) << 32;
     auto it = graphs.find(key);
     if (it == graphs.end()) {
         cudaGraph_t g = nullptr;
@@ -2090,7 +2134,11 @@ void b200rwkv_engine::infer(int nslot, const int32_t* slot, const int32_t* ntok,
         CK(cudaEventRecord(meta_ev[mb], stream));
         step_seqs = (int)s_slots.size();
         if (kx) kx_run_step(T, R, kx_decode, kx_split);
-        else run_step(mt_bucket(T), R > 0 ? mt_bucket(R) : 0, *std::max_element(s_counts.begin(), s_counts.end()) > WKV_STAGE_TOK);
+        else {
+            struct Flag { bool& f; ~Flag() { f = false; } } flag{adapters_on};
+            for (int sl : s_slots) adapters_on = adapters_on || (!slot_adapter.empty() && slot_adapter[sl] >= 0);
+            run_step(mt_bucket(T), R > 0 ? mt_bucket(R) : 0, *std::max_element(s_counts.begin(), s_counts.end()) > WKV_STAGE_TOK);
+        }
         if (hidden_keep) {       // hidden rows of every token of this call (b200rwkv_last_hidden), in entry order
             int t0 = 0;
             for (size_t j = 0; j < s_entry.size(); ++j) {
@@ -2289,6 +2337,7 @@ void b200rwkv_engine::state_xform(int slot, bool import, float* snap) {
 #include "pasopel_engine.cuh"
 #include "panupel_engine.cuh"
 #include "fufipel_engine.cuh"
+#include "slot_adapters_engine.cuh"
 
 // =========================================================================================
 // in-process tensor-parallel group
@@ -2820,6 +2869,45 @@ int32_t b200rwkv_sample_topk(b200rwkv_engine* e, int32_t nrows, const int32_t* s
     CK(cudaSetDevice(e->dev));
     e->sample_topk(nrows, slots, penalty_offset, penalty_token, penalty_value, allow_bits, bias_offset, bias_token, bias_value, top_k,
                    ids_out, probs_out);
+    API_END
+}
+
+int32_t b200rwkv_sample_rows(b200rwkv_engine* e, int32_t nrows, const b200rwkv_row_controls* q, float* out) {
+    API_BEGIN(e)
+    REQUIRE(e && q && q->struct_bytes == sizeof(*q), B200RWKV_ERR_INVALID, "sample_rows: null engine, or struct_bytes is not sizeof(b200rwkv_row_controls)");
+    std::lock_guard<std::mutex> lk(e->sm_mu);
+    CK(cudaSetDevice(e->dev));
+    e->sample_rows(nrows, *q, out);
+    API_END
+}
+
+int32_t b200rwkv_adapter_load(b200rwkv_engine* e, const uint8_t* st, size_t len, float alpha, uint64_t* id) {
+    API_BEGIN(e)
+    REQUIRE(e && st && len > 8 && id, B200RWKV_ERR_INVALID, "adapter_load: null argument");
+    *id = 0;
+    REQUIRE(!e->group, B200RWKV_ERR_UNSUPPORTED, "adapters of slots: RWKV models on one GPU");
+    StFile f(st, len);
+    std::lock_guard<std::mutex> lk(e->mu);
+    CK(cudaSetDevice(e->dev));
+    *id = e->adapter_load(f, alpha);
+    API_END
+}
+
+int32_t b200rwkv_adapter_free(b200rwkv_engine* e, uint64_t id) {
+    API_BEGIN(e)
+    REQUIRE(e, B200RWKV_ERR_INVALID, "null engine");
+    std::lock_guard<std::mutex> lk(e->mu);
+    CK(cudaSetDevice(e->dev));
+    e->adapter_free(id);
+    API_END
+}
+
+int32_t b200rwkv_slot_adapter(b200rwkv_engine* e, int32_t slot, uint64_t id) {
+    API_BEGIN(e)
+    REQUIRE(e, B200RWKV_ERR_INVALID, "null engine");
+    std::lock_guard<std::mutex> lk(e->mu);
+    CK(cudaSetDevice(e->dev));
+    e->adapter_bind(slot, id);
     API_END
 }
 

@@ -16,37 +16,9 @@
 #pragma once
 #include <cuda_bf16.h>
 
-#include "common.cuh"
+#include "operators.cuh"
 
 namespace b200 {
-
-constexpr int LOGITS_CTAS = 8, LOGITS_THREADS = 256;
-constexpr int LOGITS_SUB = 8192;                 // tokens of a slice that a pass over the lists covers
-constexpr size_t LOGITS_SMEM_MAX = 220 * 1024;
-enum LogitsKind : int { LOGITS_ROWS = 0, LOGITS_PROBS = 1, LOGITS_LOGPROBS = 2 };
-
-struct LogitsParams {
-    const void* in;
-    long long in_stride;         // elements
-    float* out;
-    long long out_stride;
-    int V, slice;                // slice: tokens of a CTA, a multiple of 4
-    int kind;
-    int vec;                     // rows start on 16-byte boundaries (in and out)
-    int buffered;                // the slice fits shared memory; else it waits in `out`
-    int sub;                     // tokens of a pass over the lists (0: no lists)
-    const int* in_row;           // row of `in` of each output row (null: the same)
-    const float* controls;       // [rows][5]: repetition, presence, frequency, decay, temperature
-    const int* hist_off;
-    const int* hist;
-    const int* hist_from;
-    const unsigned* allow;
-    int words, allow_rows;
-    const int* allow_row;
-    const int* bias_off;
-    const int* bias_tok;
-    const float* bias_val;
-};
 
 template <typename E> __device__ __forceinline__ float logit_of(E v);
 template <> __device__ __forceinline__ float logit_of<float>(float v) { return v; }

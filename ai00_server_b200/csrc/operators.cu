@@ -1,6 +1,8 @@
 // Operators on device memory: adapters of many requests (adapters.cuh) and adjusted logits (logits.cuh), their C entries and the launches
 // the engine makes of them.
 #include "operators.cuh"
+#include "adapters.cuh"
+#include "logits.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -45,22 +47,33 @@ size_t adapters_workspace(int tokens, int adapters) {
 void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan_kernel, dim3(1), ADP_PLAN_THREADS, 0, s, p); }
 
 template <typename E, typename O>
+static void ready() {
+    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
+}
+
+template <typename E, typename O>
 static void apply(cudaStream_t s, const AdapterParams& p, int nparts) {
     int R = 0;
     for (int i = 0; i < nparts; ++i) R = std::max(R, p.part[i].R);
     const size_t smem = adapter_few_smem(R, AdpParts<E, O>::N);
-    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
+    ready<E, O>();
     launch(adapter_few_kernel<E, O>, dim3(ADP_CTAS * adapter_groups(p.tokens, p.adapters), nparts), ADP_THREADS, smem, s, p);
 }
 
+// f(element, output) of the types of a call
+template <typename F>
+static void with_types(int type, int out_type, F&& f) {
+    const bool wide = out_type == B200RWKV_TYPE_F32;
+    if (type == B200RWKV_TYPE_F16) wide ? f(__half{}, float{}) : f(__half{}, __half{});
+    else wide ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
+}
+
+void adapters_prepare(int type, int out_type) {
+    with_types(type, out_type, [](auto e, auto o) { ready<decltype(e), decltype(o)>(); });
+}
+
 void adapters_apply(cudaStream_t s, const AdapterParams& p, int nparts, int type, int out_type) {
-    if (type == B200RWKV_TYPE_F16) {
-        if (out_type == B200RWKV_TYPE_F32) apply<__half, float>(s, p, nparts);
-        else apply<__half, __half>(s, p, nparts);
-    } else {
-        if (out_type == B200RWKV_TYPE_F32) apply<__nv_bfloat16, float>(s, p, nparts);
-        else apply<__nv_bfloat16, __nv_bfloat16>(s, p, nparts);
-    }
+    with_types(type, out_type, [&](auto e, auto o) { apply<decltype(e), decltype(o)>(s, p, nparts); });
 }
 
 template <typename E>

@@ -1,17 +1,105 @@
-// Launches of the operators on device memory (operators.cu), as the C entries and the engine make them.
+// Operators on device memory: their parameters, and their launches as the C entries and the engine make them (operators.cu; the kernels are in
+// adapters.cuh and logits.cuh).
 #pragma once
-#include "adapters.cuh"
+#include "common.cuh"
 #include "host.cuh"
-#include "logits.cuh"
 
 namespace b200 {
 
+// ---- low-rank adapters ----
+constexpr int ADP_CTAS = 8, ADP_THREADS = 256, ADP_WARPS = ADP_THREADS / 32;
+constexpr int ADP_TOK = 8;                       // tokens of a group: the N of the products
+constexpr int ADP_MAX_PARTS = 8, ADP_MAX_RANK = 256, ADP_MAX_ADAPTERS = 1024;
+constexpr int ADP_INLINE = ADP_THREADS;          // tokens of a call whose groups every CTA finds by itself; more take adapter_plan_kernel
+constexpr int ADP_PLAN_THREADS = 1024;
+
+// one adapter of one projection, where adapters lie apart
+struct AdapterEntry {
+    const void* a;
+    const void* b;
+    int rank;                    // 0: the adapter leaves this projection alone
+    float scale;
+};
+
+struct AdapterPart {
+    const void* x;               // rows of K, or (x_a16) the A16 layout of common.cuh with x_th as its height
+    long long x_stride;          // elements
+    int x_a16, x_th;
+    int x_lo;                    // rows to the low half of split operands (0: none)
+    const void* a;               // [adapters][R][K]
+    const void* b;               // [adapters][N][R]
+    const AdapterEntry* table;   // instead of a and b
+    const void* base;
+    long long base_stride;
+    void* out;
+    long long out_stride;
+    int K, N, R;                 // R: the largest rank
+    int vec;                     // rows of base and out take accesses of four elements
+};
+
+// groups of more tokens than ADP_INLINE: [0] = groups, then {adapter, first place} of each, then tokens by place
+struct AdapterPlan {
+    int* base;
+    int tokens, most;            // most: groups there can be
+    __host__ __device__ int* count() const { return base; }
+    __host__ __device__ int2* group() const { return reinterpret_cast<int2*>(base + 4); }
+    __host__ __device__ int* place() const { return base + 4 + 2 * (size_t)most; }
+    __host__ __device__ static size_t ints(int tokens, int most) { return 4 + 2 * (size_t)most + tokens; }
+};
+
+struct AdapterParams {
+    int tokens, adapters;
+    int copy;                    // tokens without an adapter have their base copied (base and out differ)
+    const int* index;
+    const float* scale;
+    AdapterPlan plan;
+    AdapterPart part[ADP_MAX_PARTS];
+};
+
+// groups of up to ADP_TOK tokens that `tokens` tokens can need: all with their own adapter, or full groups and a broken one for each adapter (and for none)
+__host__ __device__ inline int adapter_groups(int tokens, int adapters) {
+    const long long full = (long long)adapters + 1 + tokens / ADP_TOK;
+    return (int)(full < tokens ? full : tokens);
+}
+
 // bytes of the plan that a call of this many tokens needs (0: none)
 B200_HIDDEN size_t adapters_workspace(int tokens, int adapters);
+// sets up the kernels of a type; a captured call needs it beforehand
+B200_HIDDEN void adapters_prepare(int type, int out_type);
 // orders the tokens of a longer call by adapter; its groups serve any number of adapters_apply calls with the same tokens
 B200_HIDDEN void adapters_plan(cudaStream_t s, const AdapterParams& p);
 // parts [0, nparts) of p; type: B200RWKV_TYPE_F16 / _BF16, out_type: that or _F32
 B200_HIDDEN void adapters_apply(cudaStream_t s, const AdapterParams& p, int nparts, int type, int out_type);
+
+// ---- rows of logits ----
+constexpr int LOGITS_CTAS = 8, LOGITS_THREADS = 256;
+constexpr int LOGITS_SUB = 8192;                 // tokens of a slice that a pass over the lists covers
+constexpr size_t LOGITS_SMEM_MAX = 220 * 1024;
+enum LogitsKind : int { LOGITS_ROWS = 0, LOGITS_PROBS = 1, LOGITS_LOGPROBS = 2 };
+
+struct LogitsParams {
+    const void* in;
+    long long in_stride;         // elements
+    float* out;
+    long long out_stride;
+    int V, slice;                // slice: tokens of a CTA, a multiple of 4
+    int kind;
+    int vec;                     // rows start on 16-byte boundaries (in and out)
+    int buffered;                // the slice fits shared memory; else it waits in `out`
+    int sub;                     // tokens of a pass over the lists (0: no lists)
+    const int* in_row;           // row of `in` of each output row (null: the same)
+    const float* controls;       // [rows][5]: repetition, presence, frequency, decay, temperature
+    const int* hist_off;
+    const int* hist;
+    const int* hist_from;
+    const unsigned* allow;
+    int words, allow_rows;
+    const int* allow_row;
+    const int* bias_off;
+    const int* bias_tok;
+    const float* bias_val;
+};
+
 // slice, sub, buffered and vec of p are filled in here
 B200_HIDDEN void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type);
 

@@ -81,6 +81,18 @@ class TensorGpu:
             self.id = 0
 
 
+class Adapter:
+    """A LoRA file that the model holds beside its weights, for slots that ask for it (Model.set_adapter)."""
+
+    def __init__(self, model: "Model", adapter_id: int):
+        self._model, self.id = model, adapter_id
+
+    def free(self):
+        if self.id:
+            capi.check(capi.lib().b200rwkv_adapter_free(self._model._h, self.id), self._model._h)
+            self.id = 0
+
+
 class State:
     def __init__(self, model: "Model"):
         self._m = model
@@ -146,6 +158,15 @@ class State:
         n, used, free = C.c_int64(0), C.c_int64(0), C.c_int64(0)
         capi.check(capi.lib().b200rwkv_cache_stats(self._m._h, C.byref(n), C.byref(used), C.byref(free)), self._m._h)
         return {"snapshots": n.value, "bytes_used": used.value, "bytes_free": free.value}
+
+
+def pack_allow(allow, n: int, vocab: int) -> np.ndarray:
+    """[n, vocab] truth values -> words of 32 tokens, the first in the lowest bit."""
+    a = np.asarray(allow, bool).reshape(n, vocab)
+    words = (vocab + 31) // 32
+    padded = np.zeros((n, words * 32), bool)
+    padded[:, :vocab] = a
+    return np.ascontiguousarray(np.packbits(padded.reshape(n, words, 32), axis=2, bitorder="little").view(np.uint32).reshape(n, words))
 
 
 class NucleusSampler:
@@ -328,6 +349,61 @@ class Model:
         capi.check(capi.lib().b200rwkv_softmax(self._h, x.shape[0], capi.ptr(x), capi.ptr(y)), self._h)
         return [y[i] for i in range(y.shape[0])]
 
+    # ---- adapters of requests ----
+    def load_adapter(self, st: np.ndarray, alpha: float = 1.0) -> Adapter:
+        """A LoRA file for slots (b200rwkv_adapter_load): the files that `lora=` blends, kept apart from the weights."""
+        st = np.ascontiguousarray(st, dtype=np.uint8)
+        aid = C.c_uint64(0)
+        capi.check(capi.lib().b200rwkv_adapter_load(self._h, capi.ptr(st), st.size, alpha, C.byref(aid)), self._h)
+        return Adapter(self, aid.value)
+
+    def set_adapter(self, slot: int, adapter: Adapter | None) -> None:
+        """Tokens of the slot use the adapter (None: the weights alone) from the next infer call on."""
+        capi.check(capi.lib().b200rwkv_slot_adapter(self._h, slot, adapter.id if adapter is not None else 0), self._h)
+
+    def sample_rows(self, slots, kind: str = "probs", controls=None, history=None, history_from=None, allow=None, bias=None, out: np.ndarray | None = None):
+        """Whole rows for samplers (b200rwkv_sample_rows): the slots' last logits rows as [n, V] "logits", "probs" or "log_probs" after
+        controls [n, 5] (repetition, presence, frequency, decay, temperature), each row's token history (a list per row, oldest first; tokens
+        before history_from[i] count for repetition alone), its bias dict and its [V] mask of allowed tokens."""
+        kinds = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
+        if kind not in kinds:
+            raise capi.B200Error(capi.ERR_INVALID, "kind must be logits, probs or log_probs")
+        n, V = len(slots), self.info["num_vocab"]
+        keep = {}
+
+        def give(name, x, dtype, size=None):
+            if x is not None:
+                keep[name] = np.ascontiguousarray(x, dtype)
+                if size is not None and keep[name].size != size:
+                    raise capi.B200Error(capi.ERR_INVALID, f"{name} has the wrong number of elements")
+                setattr(q, name, keep[name].ctypes.data)
+
+        q = capi.RowControls()
+        q.struct_bytes, q.kind = C.sizeof(capi.RowControls), kinds[kind]
+        give("slots", slots, np.int32)
+        give("controls", controls, np.float32, n * 5)
+        if history is not None:
+            if len(history) != n:
+                raise capi.B200Error(capi.ERR_INVALID, "history: a list of tokens for each slot")
+            give("history_offset", np.concatenate([[0], np.cumsum([len(h) for h in history])]) if n else [0], np.int32)
+            give("history", [t for h in history for t in h], np.uint32)
+            give("history_from", history_from, np.int32, n)
+        if bias is not None:
+            maps = [m or {} for m in bias]
+            if len(maps) != n:
+                raise capi.B200Error(capi.ERR_INVALID, "bias: a dict (or None) for each slot")
+            give("bias_offset", np.concatenate([[0], np.cumsum([len(m) for m in maps])]) if n else [0], np.int32)
+            give("bias_token", [int(t) for m in maps for t in m], np.uint32)
+            give("bias_value", [float(v) for m in maps for v in m.values()], np.float32)
+        if allow is not None:
+            give("allow_bits", pack_allow(allow, n, V), np.uint32)
+        if out is None:
+            out = np.empty((n, V), np.float32)
+        elif out.dtype != np.float32 or out.shape != (n, V) or not out.flags.c_contiguous:
+            raise capi.B200Error(capi.ERR_INVALID, "out must be a contiguous f32 [slots, vocabulary] array")
+        capi.check(capi.lib().b200rwkv_sample_rows(self._h, n, C.byref(q), out.ctypes.data), self._h)
+        return out
+
     def sample_topk(self, slots, penalties=None, bias=None, allow=None, top_k: int = 128):
         """GPU front half of sampling (b200rwkv_sample_topk): for each slot the `top_k` most probable tokens of its last
         logits row after penalties / grammar mask / bias, as (ids [n, top_k] uint32, probs [n, top_k] f32).
@@ -351,12 +427,7 @@ class Model:
         bo, bt, bv = pack(bias)
         bits = None
         if allow is not None:
-            V = self.info["num_vocab"]
-            a = np.asarray(allow, bool).reshape(n, V)
-            words = (V + 31) // 32
-            padded = np.zeros((n, words * 32), bool)
-            padded[:, :V] = a
-            bits = np.ascontiguousarray(np.packbits(padded.reshape(n, words, 32), axis=2, bitorder="little").view(np.uint32).reshape(n, words))
+            bits = pack_allow(allow, n, self.info["num_vocab"])
         ids = np.empty((n, top_k), np.uint32)
         probs = np.empty((n, top_k), np.float32)
         a_slot = np.asarray(slots, np.int32)

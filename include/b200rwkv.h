@@ -221,11 +221,47 @@ int32_t b200rwkv_softmax(b200rwkv_engine*, int32_t rows, const float* in, float*
  * probs = softmax over the whole adjusted row.  Order: logit descending, token id ascending on ties.  ids_out / probs_out:
  * [nrows][top_k].  The draw itself (top_p cut, temperature, RNG, penalty update; nucleus.rs:81-123) stays in the host
  * sampler, now over <= 128 pairs.  Samplers that need the whole distribution (Mirostat, Typical) keep using
- * b200rwkv_infer with a logits buffer + b200rwkv_softmax.  Thread contract: the softmax task's (run.rs:1237). */
+ * b200rwkv_infer with a logits buffer + b200rwkv_softmax, or take whole rows from b200rwkv_sample_rows.  Thread contract: the softmax task's (run.rs:1237). */
 int32_t b200rwkv_sample_topk(b200rwkv_engine*, int32_t nrows, const int32_t* slots, const int32_t* penalty_offset,
                              const uint32_t* penalty_token, const float* penalty_value, const uint32_t* allow_bits,
                              const int32_t* bias_offset, const uint32_t* bias_token, const float* bias_value, int32_t top_k,
                              uint32_t* ids_out, float* probs_out);
+
+/* The same for samplers that need the whole row (Mirostat sampler/mirostat.rs:44-90, Typical sampler/typical.rs:70-131, or any
+ * top_k): the listed slots' most recent logits rows, adjusted on the device as b200rwkv_op_logits states it and written to
+ * out [nrows, num_vocab] (host memory; pinned memory of b200rwkv_host_alloc is filled at full rate) as logits, probabilities
+ * or log-probabilities.  Replaces a logits copy to the host, the adjustments there and the softmax round trip (run.rs:664-697,
+ * 1164-1190); penalties come from each request's token history, or, kept by the caller, as negative biases.  A slot may be listed
+ * more than once (its row under several controls).  All arrays are host memory, in b200rwkv_op_logits' layouts.  Thread contract:
+ * the softmax task's (run.rs:1237). */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t kind;                    /* B200RWKV_LOGITS, _PROBS, _LOG_PROBS */
+    const int32_t* slots;            /* [nrows] */
+    const float* controls;           /* [nrows, 5] or NULL: repetition, presence, frequency, decay, temperature */
+    const int32_t* history_offset;   /* [nrows + 1] or NULL */
+    const uint32_t* history;
+    const int32_t* history_from;     /* [nrows] or NULL */
+    const uint32_t* allow_bits;      /* [nrows, (num_vocab + 31) / 32] or NULL */
+    const int32_t* bias_offset;      /* [nrows + 1] or NULL */
+    const uint32_t* bias_token;
+    const float* bias_value;
+} b200rwkv_row_controls;
+#define B200RWKV_LOGITS 0
+#define B200RWKV_PROBS 1
+#define B200RWKV_LOG_PROBS 2
+int32_t b200rwkv_sample_rows(b200rwkv_engine*, int32_t nrows, const b200rwkv_row_controls* controls, float* out);
+
+/* Adapters of requests: LoRA files that stay apart from the weights, so that the slots of a batch can have different ones
+ * (b200rwkv_options.lora_st blends a file into the weights for all).  Same files: `<name>.lora.1` [out, r] and `<name>.lora.0` [in, r] in F16
+ * on att.{receptance,key,value,gate,output} / ffn.{key,value,receptance} / head, r <= 256; every projection of a slot's tokens is then
+ * W x + alpha * lora.1 (lora.0^T x).  A model holds up to 64 of them.  RWKV models on one GPU (also with quantised layers and at
+ * precision 1); others answer B200RWKV_ERR_UNSUPPORTED.  b200rwkv_slot_adapter: tokens of the slot use the adapter from the next
+ * b200rwkv_infer call on (id 0: none), until the next call for that slot -- resetting or writing the slot's state does not change it.
+ * b200rwkv_adapter_free refuses (B200RWKV_ERR_STATE) while a slot has the adapter.  The image is borrowed during the call only. */
+int32_t b200rwkv_adapter_load(b200rwkv_engine*, const uint8_t* st, size_t len, float alpha, uint64_t* adapter_id);
+int32_t b200rwkv_adapter_free(b200rwkv_engine*, uint64_t adapter_id);
+int32_t b200rwkv_slot_adapter(b200rwkv_engine*, int32_t slot, uint64_t adapter_id);
 
 /* Pinned host memory for logits / state buffers (full-rate DMA); optional. */
 int32_t b200rwkv_host_alloc(size_t bytes, void** out);
@@ -332,9 +368,6 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
  * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number makes any row NaN; decay is
  * taken into [0, 1].  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
  * sampler/bnf.rs:35-38, run.rs:679-681 and softmax (run.rs:1179) of the samplers that need whole rows. */
-#define B200RWKV_LOGITS 0
-#define B200RWKV_PROBS 1
-#define B200RWKV_LOG_PROBS 2
 typedef struct {
     uint32_t struct_bytes;
     int32_t type;                /* B200RWKV_TYPE_*: logits */

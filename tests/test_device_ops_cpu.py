@@ -89,3 +89,37 @@ def test_tensors_that_do_not_fit():
         device_ops.logits(torch.zeros(2, 10))
     with pytest.raises(capi.B200Error):
         device_ops.logits(torch.zeros(20))
+
+
+def test_structs_match_the_header(tmp_path):
+    """Sizes and offsets of the operators' structs, as a C compiler has them."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    pairs = {"b200rwkv_adapter_part": capi.AdapterPart, "b200rwkv_adapters": capi.Adapters, "b200rwkv_logits": capi.Logits, "b200rwkv_row_controls": capi.RowControls}
+    lines = []
+    for name, cls in pairs.items():
+        lines.append(f'printf("%zu ", sizeof({name}));')
+        lines += [f'printf("%zu ", offsetof({name}, {f[0]}));' for f in cls._fields_]
+    src = tmp_path / "s.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "b200rwkv.h"\nint main(void) { ' + "\n".join(lines) + " return 0; }\n")
+    exe = tmp_path / "s"
+    subprocess.check_call(["gcc", "-std=c99", "-Wall", "-Werror", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)])
+    got = [int(x) for x in subprocess.check_output([str(exe)]).split()]
+    want = []
+    for cls in pairs.values():
+        want += [C.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
+    assert got == want
+    header = open(os.path.join(root, "include", "b200rwkv.h")).read()
+    for name, value in [("MAX_PARTS", capi.MAX_PARTS), ("MAX_RANK", capi.MAX_RANK), ("MAX_ADAPTERS", capi.MAX_ADAPTERS), ("TYPE_F32", capi.TYPE_F32), ("TYPE_F16", capi.TYPE_F16),
+                        ("TYPE_BF16", capi.TYPE_BF16), ("LOGITS", capi.LOGITS), ("PROBS", capi.PROBS), ("LOG_PROBS", capi.LOG_PROBS)]:
+        assert f"#define B200RWKV_{name} {value}\n" in header, name
+
+
+def test_engine_calls_refuse_null():
+    lib = capi.lib()
+    aid = C.c_uint64(5)
+    assert lib.b200rwkv_adapter_load(None, None, 0, 1.0, C.byref(aid)) == capi.ERR_INVALID
+    assert lib.b200rwkv_adapter_free(None, 1) == capi.ERR_INVALID
+    assert lib.b200rwkv_slot_adapter(None, 0, 1) == capi.ERR_INVALID
+    assert lib.b200rwkv_sample_rows(None, 1, C.byref(capi.RowControls()), None) == capi.ERR_INVALID
