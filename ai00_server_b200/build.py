@@ -18,10 +18,11 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
     "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
 ]
-# translation units of the engine library and the sources each is made of (None: every header)
+# translation units of the engine library and the headers each is made of
+KERNELS_OF_OPERATORS = ["adapters.cuh", "adapter_tiles.cuh", "logits.cuh"]
 UNITS = {
-    "engine.cu": None,
-    "operators.cu": ["adapters.cuh", "logits.cuh", "operators.cuh", "common.cuh", "host.cuh"],
+    "engine.cu": [f for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh") and f not in KERNELS_OF_OPERATORS],
+    "operators.cu": [*KERNELS_OF_OPERATORS, "operators.cuh", "common.cuh", "host.cuh"],
 }
 
 
@@ -43,8 +44,6 @@ def build_engine(force: bool = False, verbose_ptxas: bool = False, debug: bool =
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     objects, jobs = [], []
     for unit, parts in UNITS.items():
-        if parts is None:
-            parts = [f for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh")]
         srcs = [os.path.join(CSRC, f) for f in [unit, *parts]] + [header]
         obj = os.path.join(CSRC, unit[:-3] + ("_dbg.o" if debug else ".o"))
         objects.append(obj)

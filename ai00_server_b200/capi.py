@@ -127,7 +127,7 @@ SYMBOLS = [
     ("b200rwkv_profile_insitu", C.c_int32, [_P, C.c_int32, _P, _P, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, C.POINTER(C.c_double)]),
     ("b200rwkv_op_quantize", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     ("b200rwkv_op_wkv", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32] + [_P] * 14),
-    ("b200rwkv_op_adapters_workspace", C.c_int64, [C.c_int32, C.c_int32]),
+    ("b200rwkv_op_adapters_workspace", C.c_int64, [C.c_int32] * 4),
     ("b200rwkv_op_adapters", C.c_int32, [C.c_int32, _P, C.POINTER(Adapters)]),
     ("b200rwkv_op_logits", C.c_int32, [C.c_int32, _P, C.POINTER(Logits)]),
     ("b200rwkv_launch_count", C.c_int32, [_P, C.POINTER(C.c_int64)]),

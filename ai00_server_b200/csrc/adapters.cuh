@@ -124,13 +124,9 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
     const AdapterPart& q = p.part[blockIdx.y];
     pdl_wait();
     if (p.plan.base) {
-        if (want >= *p.plan.count()) return;
-        const int2 gr = p.plan.group()[want];
-        if (tid < ADP_TOK) {
-            // places of a group: up to the next group's first
-            const int last = want + 1 < *p.plan.count() ? p.plan.group()[want + 1].y : p.plan.count()[1];
-            g.tok[tid] = gr.y + tid < last ? p.plan.place()[gr.y + tid] : -1;
-        }
+        if (want >= p.plan.count()[0]) return;
+        const int4 gr = p.plan.group()[want];
+        if (tid < ADP_TOK) g.tok[tid] = tid < gr.z ? p.plan.place()[gr.y + tid] : -1;
         if (tid == 0) g.adapter = gr.x;
         __syncthreads();
     } else {
@@ -169,8 +165,8 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
 
     const int R8 = R * ADP_TOK, Rp = (R + 31) & ~31, pitch = Rp + 8;
     float* const part = reinterpret_cast<float*>(smem_raw);                      // [warp][R][8]: partial sums of the CTA's warps
-    float* const all = part + (size_t)ADP_WARPS * q.R * ADP_TOK;                 // [CTA][R][8]
-    E* const frag = reinterpret_cast<E*>(all + (size_t)ADP_CTAS * q.R * ADP_TOK);        // [part][token][pitch]
+    float* const all = part + (size_t)ADP_WARPS * p.rank * ADP_TOK;                 // [CTA][R][8]
+    E* const frag = reinterpret_cast<E*>(all + (size_t)ADP_CTAS * p.rank * ADP_TOK);        // [part][token][pitch]
 
     // ---- S: this CTA's k, a run of 32 of them to a warp at a time ----
     {
@@ -320,13 +316,13 @@ inline size_t adapter_few_smem(int R, int elem_parts) {
     return (size_t)(ADP_WARPS + ADP_CTAS) * R * ADP_TOK * 4 + (size_t)elem_parts * ADP_TOK * (((R + 31) & ~31) + 8) * 2;
 }
 
-// Tokens of a longer call ordered by adapter, and its groups: one CTA, a counting sort.  Where a token lands within its adapter depends on the order of the
-// atomics, its result does not: columns of a product do not see each other.
+// Tokens of a longer call ordered by adapter, its groups and its tiles: one CTA, a counting sort.  Where a token lands within its adapter depends on the order of
+// the atomics, its result does not: columns and rows of a product do not see each other.
 __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __grid_constant__ AdapterParams p) {
-    __shared__ int s_count[ADP_MAX_ADAPTERS + 1], s_first[ADP_MAX_ADAPTERS + 1], s_warp[2][ADP_PLAN_THREADS / 32], s_total[2];
+    __shared__ int s_count[ADP_MAX_ADAPTERS + 1], s_first[ADP_MAX_ADAPTERS + 1], s_warp[3][ADP_PLAN_THREADS / 32], s_total[3];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = p.adapters + (p.copy ? 1 : 0);
-    for (int i = tid; i <= ADP_MAX_ADAPTERS; i += ADP_PLAN_THREADS) s_count[i] = 0;
-    if (tid < 2) s_total[tid] = 0;
+    for (int i = tid; i < bins; i += ADP_PLAN_THREADS) s_count[i] = 0;
+    if (tid < 3) s_total[tid] = 0;
     pdl_wait();
     __syncthreads();
     auto bin_of = [&](int t) {
@@ -339,30 +335,45 @@ __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __
         if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&s_count[b], __popc(same));
     }
     __syncthreads();
-    // exclusive sums over the bins of tokens and of groups, ADP_PLAN_THREADS bins at a time
+    // exclusive sums over the bins of tokens, groups and tiles, ADP_PLAN_THREADS bins at a time
     for (int b0 = 0; b0 < bins; b0 += ADP_PLAN_THREADS) {
-        const int b = b0 + tid, c = b < bins ? s_count[b] : 0, gr = (c + ADP_TOK - 1) / ADP_TOK;
-        int st = c, sg = gr;
+        const int b = b0 + tid, c = b < bins ? s_count[b] : 0;
+        const bool tiled = c >= p.tile_least;
+        const int own[3] = {c, tiled ? 0 : (c + ADP_TOK - 1) / ADP_TOK, tiled ? (c + ADP_TILE - 1) / ADP_TILE : 0};
+        int at[3];
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int vt = __shfl_up_sync(0xffffffffu, st, o), vg = __shfl_up_sync(0xffffffffu, sg, o);
-            if (lane >= o) { st += vt; sg += vg; }
+        for (int i = 0; i < 3; ++i) {
+            at[i] = own[i];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, at[i], o);
+                if (lane >= o) at[i] += v;
+            }
+            if (lane == 31) s_warp[i][warp] = at[i];
         }
-        if (lane == 31) { s_warp[0][warp] = st; s_warp[1][warp] = sg; }
         __syncthreads();
-        int at = s_total[0] + st - c, ag = s_total[1] + sg - gr;
-        for (int w = 0; w < warp; ++w) { at += s_warp[0][w]; ag += s_warp[1][w]; }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            // (a warp's sum over the warps in front: one lane each)
+            int v = lane < warp ? s_warp[i][lane] : 0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            at[i] += s_total[i] + v - own[i];
+        }
         if (b < bins) {
-            s_first[b] = at;
-            for (int i = 0; i < gr; ++i) p.plan.group()[ag + i] = make_int2(b == p.adapters ? -1 : b, at + i * ADP_TOK);
+            const int id = b == p.adapters ? -1 : b, step = tiled ? ADP_TILE : ADP_TOK;
+            s_first[b] = at[0];
+            int4* const to = tiled ? p.plan.tile() + at[2] : p.plan.group() + at[1];
+            for (int i = 0; i * step < c; ++i) to[i] = make_int4(id, at[0] + i * step, min(step, c - i * step), 0);
         }
         __syncthreads();
-        if (tid == ADP_PLAN_THREADS - 1) { s_total[0] = at + c; s_total[1] = ag + gr; }
+        if (tid == ADP_PLAN_THREADS - 1)
+            for (int i = 0; i < 3; ++i) s_total[i] = at[i] + own[i];
         __syncthreads();
     }
     if (tid == 0) {
         p.plan.count()[0] = s_total[1];
-        p.plan.count()[1] = s_total[0];
+        p.plan.count()[1] = s_total[2];
     }
     for (int t0 = 0; t0 < p.tokens; t0 += ADP_PLAN_THREADS) {
         const int b = t0 + tid < p.tokens ? bin_of(t0 + tid) : -1;

@@ -7,12 +7,13 @@
 // softmax run.rs:1179; the samplers that need whole rows are sampler/mirostat.rs:44-90 and sampler/typical.rs:70-131.
 //
 // Bound: a row is read and written once, 8 bytes a token for f32 rows (row of 65536: 0.5 MB; 512 rows 41 us at the copy rate); one row is latency.
-// Shape: a cluster of eight CTAs a row, an eighth of the row each, which stays in shared memory between the only read and the only write.
-//   * lists touch few tokens: they are applied to the slice in shared memory, not looked up by every element.  A history entry adds decay^age to its
-//     token's sum in 32.32 fixed point (a word of fraction, whose carries go to a word of whole counts with the two flags), so that the order
-//     of the atomics changes nothing; whoever then takes a token's counts first (exchange with zero) applies them;
-//   * a CTA's maximum and its sum of exponentials go to the other seven in one exchange; a softmax entry is computed once, relative to the CTA's
-//     maximum, and scaled by the row's factor on its way out.
+// Shape: a cluster of eight or sixteen CTAs a row, the row in their registers (16 to 64 tokens a thread) between the only read and the only write.
+// Tokens go to the CTAs in stripes of 64, so that frequent tokens that are neighbours in a vocabulary spread over all of them.
+//   * a history is added up in shared memory, a pair of words for each token of the CTA: decay^age in units of 2^-28, its lower 14 bits to one word
+//     and the others to the other, so that neither overflows (2^17 - 1 entries; of a longer history the newest count), no atomic has to answer,
+//     and their order changes nothing.  An entry that counts adds one unit at least: the words say by themselves which tokens have been said;
+//   * one pass over the registers for the thread's maximum and its sum of exponentials, which are what the probabilities are made of; pairs are
+//     combined over the CTA, and over the cluster in one exchange.
 #pragma once
 #include <cuda_bf16.h>
 
@@ -37,220 +38,237 @@ __device__ __forceinline__ float4 logits4(const __nv_bfloat16* p) {
     return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
 }
 
-// NaN is kept: it reaches the sum, and through it the whole row
-__device__ __forceinline__ float logits_block(float v, float* red, const bool is_max) {
+constexpr unsigned LOGITS_SEEN = 1u << 31;        // flag in the upper word of a token that is in the history and does not count there
+
+// sum of exponentials relative to a maximum.  NaN never becomes the maximum: it stays in the sum, and through it reaches the whole row
+struct LogitsSum {
+    float m, s;
+    __device__ __forceinline__ void raise(float to) {
+        if (to > m) {
+            s *= expf(m - to);
+            m = to;
+        }
+    }
+};
+__device__ __forceinline__ LogitsSum logits_block(LogitsSum a, LogitsSum* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    v = is_max ? warp_max(v) : warp_sum(v);
+    auto whole = [](LogitsSum x) {
+        x.raise(warp_max(x.m));
+        x.s = warp_sum(x.s);
+        return x;
+    };
+    a = whole(a);
+    if (lane == 0) red[warp] = a;
     __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    float t = lane < LOGITS_THREADS / 32 ? red[lane] : (is_max ? -INFINITY : 0.f);
-    return is_max ? warp_max(t) : warp_sum(t);
+    return whole(lane < LOGITS_THREADS / 32 ? red[lane] : LogitsSum{-INFINITY, 0.f});
 }
 
-constexpr unsigned LOGITS_SEEN = 1u << 31, LOGITS_SAID = 1u << 30, LOGITS_COUNT = LOGITS_SAID - 1;
-
-template <typename E>
-__global__ void __cluster_dims__(LOGITS_CTAS, 1, 1) __launch_bounds__(LOGITS_THREADS) logits_kernel(const __grid_constant__ LogitsParams p) {
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    __shared__ float red[32];
-    __shared__ float2 stats[LOGITS_CTAS];
-    const int tid = threadIdx.x, cta = blockIdx.x % LOGITS_CTAS, row = blockIdx.x / LOGITS_CTAS;
+// NV: fours of tokens a thread holds.  VEC: a thread's fours are neighbours and rows allow accesses of four; else its tokens are LOGITS_THREADS apart
+template <typename E, int NV, bool VEC>
+__global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1)) logits_kernel(const __grid_constant__ LogitsParams p) {
+    extern __shared__ __align__(16) uint2 sums[];
+    __shared__ LogitsSum red[LOGITS_THREADS / 32];
+    __shared__ float2 stats[LOGITS_MOST_CTAS];
+    constexpr int TH = LOGITS_THREADS;
+    const int tid = threadIdx.x, lg_ctas = p.ctas_log, ctas = 1 << lg_ctas, cta = blockIdx.x & (ctas - 1), row = blockIdx.x >> lg_ctas;
     const bool softmax = p.kind != LOGITS_ROWS;
     // no CTA writes to another's memory before all have started
     if (softmax) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     pdl_wait();
-    const int t0 = min(cta * p.slice, p.V), n = min(p.slice, p.V - t0);
-    const E* const in = reinterpret_cast<const E*>(p.in) + (size_t)(p.in_row ? p.in_row[row] : row) * p.in_stride + t0;
-    float* const out = p.out + (size_t)row * p.out_stride + t0;
-    float* const buf = p.buffered ? reinterpret_cast<float*>(smem_raw) : out;
-    unsigned* const acc_lo = reinterpret_cast<unsigned*>(smem_raw + (p.buffered ? (size_t)p.slice * 4 : 0));
-    unsigned* const acc_hi = acc_lo + p.sub;
-
-    float rep = 1.f, presence = 0.f, frequency = 0.f, decay = 1.f, temperature = 1.f;
-    if (p.controls) {
-        const float* c = p.controls + (size_t)row * 5;
-        rep = c[0]; presence = c[1]; frequency = c[2]; decay = c[3]; temperature = c[4];
+    // the CTA's tokens by place: stripes cta, cta + ctas, ...; only the vocabulary's last stripe can be short
+    const int stripes = (p.V + LOGITS_STRIPE - 1) / LOGITS_STRIPE, own = (stripes - cta + ctas - 1) >> lg_ctas;
+    int n = max(own, 0) * LOGITS_STRIPE;
+    if (own > 0 && (((own - 1) << lg_ctas) | cta) == stripes - 1) n -= stripes * LOGITS_STRIPE - p.V;
+    auto token = [&](int i) { return (((i / LOGITS_STRIPE) << lg_ctas) | cta) * LOGITS_STRIPE + i % LOGITS_STRIPE; };
+    auto place = [&](int k, int c) { return VEC ? (k * TH + tid) * 4 + c : (k * 4 + c) * TH + tid; };       // of the thread's c-th token in its k-th four
+    const E* const in = reinterpret_cast<const E*>(p.in) + (size_t)(p.in_row ? p.in_row[row] : row) * p.in_stride;
+    float* const out = p.out + (size_t)row * p.out_stride;
+    float v[NV][4];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int i = place(k, 0);
+        if (VEC && i + 3 < n) {
+            const float4 x = logits4(in + token(i));
+            v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[k][c] = place(k, c) < n ? logit_of<E>(in[token(place(k, c))]) : -INFINITY;
+        }
     }
+    const float* const ctl = p.controls ? p.controls + (size_t)row * 5 : nullptr;
     const int h0 = p.hist_off ? p.hist_off[row] : 0, hn = p.hist_off ? p.hist_off[row + 1] - h0 : 0;
     const int b0 = p.bias_off ? p.bias_off[row] : 0, bn = p.bias_off ? p.bias_off[row + 1] - b0 : 0;
-    const int allow_row = p.allow ? (p.allow_row ? p.allow_row[row] : row) : -1;
-    const unsigned* const allow = allow_row >= 0 && allow_row < p.allow_rows ? p.allow + (size_t)allow_row * p.words : nullptr;
-    // a temperature that is not a positive number makes the row NaN
-    const float scale = temperature > 0.f && temperature < INFINITY ? 1.f / temperature : __int_as_float(0x7fc00000);
 
-    const bool lists = hn > 0 || bn > 0;
-    // one element of the row after its lists: mask and temperature
-    auto finish = [&](float l, int i) {
-        const int t = t0 + i;
-        if (allow && !((allow[t >> 5] >> (t & 31)) & 1u)) l = -INFINITY;
-        return l * scale;
-    };
-    float mx = -INFINITY;
-    if (p.vec) {
-        constexpr int U = 8;
-        for (int i0 = tid * 4; i0 < n; i0 += LOGITS_THREADS * 4 * U) {
-            float4 v[U];
+    // ---- lists, for as many of the CTA's tokens at a time as have their sums in shared memory ----
+    if (hn > 0 || bn > 0) {
+        // f(j, place of its token) for the entries of a list from `first` on that are among them
+        auto each = [&](const int* tok, int first, int count, int s0, auto&& f) {
+            constexpr int U = 4;
+            for (int j0 = first + tid; j0 < count; j0 += TH * U) {
+                unsigned t[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u * LOGITS_THREADS * 4;
-                if (i + 3 < n) v[u] = logits4(in + i);
+                for (int u = 0; u < U; ++u) t[u] = j0 + u * TH < count ? (unsigned)tok[j0 + u * TH] : 0xFFFFFFFFu;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const unsigned st = t[u] / LOGITS_STRIPE;
+                    const int i = (int)((st >> lg_ctas) * LOGITS_STRIPE + t[u] % LOGITS_STRIPE) - s0;
+                    if (t[u] < (unsigned)p.V && (int)(st & (ctas - 1)) == cta && i >= 0 && i < p.list_tokens) f(j0 + u * TH, i);
+                }
             }
+        };
+        // f(logit, sums) for those of the thread's tokens
+        auto apply = [&](int s0, auto&& f) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int i = i0 + u * LOGITS_THREADS * 4;
-                if (i >= n) break;
-                if (i + 3 < n) {
-                    if (!lists) {
-                        if (allow) {
-                            const unsigned w = allow[(t0 + i) >> 5] >> ((t0 + i) & 31);       // four tokens of a word: i and t0 are multiples of 4
-                            if (!(w & 1u)) v[u].x = -INFINITY;
-                            if (!(w & 2u)) v[u].y = -INFINITY;
-                            if (!(w & 4u)) v[u].z = -INFINITY;
-                            if (!(w & 8u)) v[u].w = -INFINITY;
-                        }
-                        v[u].x *= scale; v[u].y *= scale; v[u].z *= scale; v[u].w *= scale;
-                        mx = fmaxf(fmaxf(fmaxf(mx, v[u].x), fmaxf(v[u].y, v[u].z)), v[u].w);
-                    }
-                    *reinterpret_cast<float4*>(buf + i) = v[u];
+            for (int k = 0; k < NV; ++k) {
+                const int i = place(k, 0) - s0;
+                if (VEC) {
+                    if (i < 0 || i >= p.list_tokens) continue;
+                    const uint4 a = *reinterpret_cast<const uint4*>(sums + i), b = *reinterpret_cast<const uint4*>(sums + i + 2);
+                    if ((a.x | a.y | a.z | a.w | b.x | b.y | b.z | b.w) == 0u) continue;
+                    f(v[k][0], make_uint2(a.x, a.y)); f(v[k][1], make_uint2(a.z, a.w)); f(v[k][2], make_uint2(b.x, b.y)); f(v[k][3], make_uint2(b.z, b.w));
+                    *reinterpret_cast<uint4*>(sums + i) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(sums + i + 2) = make_uint4(0, 0, 0, 0);
                 } else {
-                    for (int k = i; k < n; ++k) {
-                        float l = logit_of<E>(in[k]);
-                        if (!lists) { l = finish(l, k); mx = fmaxf(mx, l); }
-                        buf[k] = l;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int e = place(k, c) - s0;
+                        if (e < 0 || e >= p.list_tokens) continue;
+                        const uint2 a = sums[e];
+                        if ((a.x | a.y) == 0u) continue;
+                        f(v[k][c], a);
+                        sums[e] = make_uint2(0, 0);
                     }
                 }
             }
-        }
-    } else {
-        for (int i = tid; i < n; i += LOGITS_THREADS) {
-            float l = logit_of<E>(in[i]);
-            if (!lists) { l = finish(l, i); mx = fmaxf(mx, l); }
-            buf[i] = l;
-        }
-    }
-    if (lists) {
-        const int from = p.hist_from ? p.hist_from[row] : 0;
-        const float lg = log2f(fminf(fmaxf(decay, 0.f), 1.f));
-        for (int s0 = 0; s0 < n; s0 += p.sub) {
-            const int sn = min(p.sub, n - s0);
-            const unsigned first = (unsigned)(t0 + s0);
+        };
+        // (what is not zero after `apply` is zeroed there: the sums start at zero every time)
+        for (int i = tid * 2; i < p.list_tokens; i += TH * 2) *reinterpret_cast<uint4*>(sums + i) = make_uint4(0, 0, 0, 0);
+        for (int s0 = 0; s0 < n; s0 += p.list_tokens) {
             if (hn > 0) {
+                const float rep = ctl ? ctl[0] : 1.f, presence = ctl ? ctl[1] : 0.f, frequency = ctl ? ctl[2] : 0.f;
+                const float lg = log2f(fminf(fmaxf(ctl ? ctl[3] : 1.f, 0.f), 1.f));
+                const int from = p.hist_from ? p.hist_from[row] : 0;
                 __syncthreads();
-                for (int j = tid; j < hn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.hist[h0 + j] - first;
-                    if (e < (unsigned)sn) acc_lo[e] = acc_hi[e] = 0u;
-                }
-                __syncthreads();
-                for (int j = tid; j < hn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.hist[h0 + j] - first;
-                    if (e >= (unsigned)sn) continue;
-                    unsigned hi = LOGITS_SEEN;
-                    if (j >= from) {
-                        hi |= LOGITS_SAID;
-                        const int age = hn - 1 - j;
-                        const float w = age == 0 ? 1.f : exp2f(lg * (float)age);        // (zero decay: 0 from the second newest on)
-                        if (w >= 1.f) {
-                            atomicAdd(&acc_hi[e], 1u);
-                        } else {
-                            const unsigned c = (unsigned)(w * 4294967296.f);
-                            if (atomicAdd(&acc_lo[e], c) + c < c) atomicAdd(&acc_hi[e], 1u);
-                        }
+                each(p.hist + h0, max(0, hn - LOGITS_MAX_HISTORY), hn, s0, [&](int j, int i) {
+                    if (j < from) {
+                        if (!(*reinterpret_cast<volatile unsigned*>(&sums[i].y) & LOGITS_SEEN)) atomicOr(&sums[i].y, LOGITS_SEEN);
+                        return;
                     }
-                    atomicOr(&acc_hi[e], hi);
-                }
+                    const int age = hn - 1 - j;
+                    const unsigned c = age == 0 ? 1u << 28 : max(1u, (unsigned)(exp2f(lg * (float)age) * 268435456.f + 0.5f));      // (zero decay: one unit from the second newest on)
+                    if (c & 0x3FFFu) atomicAdd(&sums[i].x, c & 0x3FFFu);
+                    if (c >> 14) atomicAdd(&sums[i].y, c >> 14);
+                });
                 __syncthreads();
-                for (int j = tid; j < hn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.hist[h0 + j] - first;
-                    if (e >= (unsigned)sn || acc_hi[e] == 0u) continue;
-                    const unsigned hi = atomicExch(&acc_hi[e], 0u);
-                    if (hi == 0u) continue;
-                    float l = buf[s0 + e];
+                apply(s0, [&](float& l, uint2 a) {
+                    if ((a.x | a.y) == 0u) return;
                     l = l > 0.f ? l / rep : l * rep;
-                    if (hi & LOGITS_SAID) l -= presence + frequency * ((float)(hi & LOGITS_COUNT) + (float)acc_lo[e] * 0x1p-32f);
-                    buf[s0 + e] = l;
-                }
+                    const unsigned up = a.y & ~LOGITS_SEEN;
+                    if (a.x | up) l -= presence + frequency * ((float)up * 0x1p-14f + (float)a.x * 0x1p-28f);
+                });
             }
             if (bn > 0) {
                 // a token listed twice has its last value: the highest place wins
                 __syncthreads();
-                for (int j = tid; j < bn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.bias_tok[b0 + j] - first;
-                    if (e < (unsigned)sn) acc_lo[e] = 0u;
-                }
+                each(p.bias_tok + b0, 0, bn, s0, [&](int j, int i) { atomicMax(&sums[i].x, (unsigned)j + 1u); });
                 __syncthreads();
-                for (int j = tid; j < bn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.bias_tok[b0 + j] - first;
-                    if (e < (unsigned)sn) atomicMax(&acc_lo[e], (unsigned)j + 1u);
-                }
-                __syncthreads();
-                for (int j = tid; j < bn; j += LOGITS_THREADS) {
-                    const unsigned e = (unsigned)p.bias_tok[b0 + j] - first;
-                    if (e < (unsigned)sn && acc_lo[e] == (unsigned)j + 1u) buf[s0 + e] += p.bias_val[b0 + j];
-                }
+                apply(s0, [&](float& l, uint2 a) {
+                    if (a.x) l += p.bias_val[b0 + a.x - 1u];
+                });
             }
-        }
-        __syncthreads();
-        for (int i = tid; i < n; i += LOGITS_THREADS) {
-            const float l = finish(buf[i], i);
-            buf[i] = l;
-            mx = fmaxf(mx, l);
         }
     }
-    if (!softmax) {
-        if (!p.buffered) return;
-        __syncthreads();
-        if (p.vec) {
-            for (int i = tid * 4; i < n; i += LOGITS_THREADS * 4) {
-                if (i + 3 < n) *reinterpret_cast<float4*>(out + i) = *reinterpret_cast<const float4*>(buf + i);
-                else for (int k = i; k < n; ++k) out[k] = buf[k];
+
+    // ---- mask and temperature ----
+    const float temperature = ctl ? ctl[4] : 1.f;
+    // a temperature that is not a positive number makes the row NaN
+    const float scale = temperature > 0.f && temperature < INFINITY ? 1.f / temperature : __int_as_float(0x7fc00000);
+    const int allow_row = p.allow ? (p.allow_row ? p.allow_row[row] : row) : -1;
+    if (allow_row >= 0 && allow_row < p.allow_rows) {
+        const unsigned* const allow = p.allow + (size_t)allow_row * p.words;
+        if (VEC) {
+            unsigned w[NV];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int t = token(place(k, 0));
+                w[k] = place(k, 0) < n ? allow[t / 32] >> (t % 32) : 0u;        // four tokens of a word: t is a multiple of 4
             }
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (!((w[k] >> c) & 1u)) v[k][c] = -INFINITY;
         } else {
-            for (int i = tid; i < n; i += LOGITS_THREADS) out[i] = buf[i];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                unsigned w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) w[c] = place(k, c) < n ? allow[token(place(k, c)) / 32] : 0u;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (!((w[c] >> (place(k, c) % 32)) & 1u)) v[k][c] = -INFINITY;       // (places and tokens agree modulo 32)
+            }
         }
+    }
+    auto put = [&](auto&& last) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int i = place(k, 0);
+            if (VEC && i + 3 < n) {
+                *reinterpret_cast<float4*>(out + token(i)) = make_float4(last(v[k][0]), last(v[k][1]), last(v[k][2]), last(v[k][3]));
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (place(k, c) < n) out[token(place(k, c))] = last(v[k][c]);
+            }
+        }
+    };
+    if (!softmax) {
+        put([&](float l) { return l * scale; });
         return;
     }
-    mx = logits_block(mx, red, true);          // (its barriers also stand between the writes to the slice and its readers)
-    const float shift = mx == -INFINITY ? 0.f : mx;
-    float sum = 0.f;
+
+    // ---- the thread's maximum and sum; from here on a probability is its exponential ----
     const bool probs = p.kind == LOGITS_PROBS;
-    for (int i = tid; i < n; i += LOGITS_THREADS) {
-        const float e = expf(buf[i] - shift);
-        sum += e;
-        if (probs) buf[i] = e;
-    }
-    sum = logits_block(sum, red, false);
+    LogitsSum sum{-INFINITY, 0.f};
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if (place(k, c) < n) v[k][c] *= scale;       // (what is behind the last token stays -inf under every scale)
+            sum.m = fmaxf(sum.m, v[k][c]);
+        }
+    const float mine = sum.m, shift = mine == -INFINITY ? 0.f : mine;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float e = expf(v[k][c] - shift);
+            sum.s += e;
+            if (probs) v[k][c] = e;
+        }
+
+    // ---- the CTAs' statistics, in their order ----
+    sum = logits_block(sum, red);
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (tid < LOGITS_CTAS) {
+    if (tid < ctas) {
         uint32_t remote;
         const uint32_t local = smem_u32(&stats[cta]);
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(tid));
-        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(mx), "f"(sum) : "memory");
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(sum.m), "f"(sum.s) : "memory");
     }
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    float top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < LOGITS_CTAS; ++c) top = fmaxf(top, stats[c].x);
-    float z = 0.f;
-#pragma unroll
-    for (int c = 0; c < LOGITS_CTAS; ++c) z += stats[c].y * (stats[c].x == -INFINITY ? 1.f : expf(stats[c].x - top));
+    float top = -INFINITY, z = 0.f;
+    for (int c = 0; c < ctas; ++c) top = fmaxf(top, stats[c].x);
+    for (int c = 0; c < ctas; ++c) z += stats[c].y * (stats[c].x == -INFINITY ? 1.f : expf(stats[c].x - top));
     // nothing left of the row (its sums are zero, not NaN): probabilities 0, logarithms -inf
     const bool none = top == -INFINITY && z == 0.f;
-    const float mul = probs ? (none ? 0.f : (mx == -INFINITY ? 1.f : expf(mx - top)) / z) : 1.f;
-    const float sub = probs || none ? 0.f : logf(z), base = probs || none ? 0.f : top;
-    auto last = [&](float v) { return probs ? v * mul : (v - base) - sub; };
-    if (p.vec) {
-        for (int i = tid * 4; i < n; i += LOGITS_THREADS * 4) {
-            if (i + 3 < n) {
-                float4 v = *reinterpret_cast<const float4*>(buf + i);
-                v.x = last(v.x); v.y = last(v.y); v.z = last(v.z); v.w = last(v.w);
-                *reinterpret_cast<float4*>(out + i) = v;
-            } else {
-                for (int k = i; k < n; ++k) out[k] = last(buf[k]);
-            }
-        }
+    if (probs) {
+        const float mul = none ? 0.f : (mine == -INFINITY ? 1.f : expf(mine - top)) / z;
+        put([&](float e) { return e * mul; });
     } else {
-        for (int i = tid; i < n; i += LOGITS_THREADS) out[i] = last(buf[i]);
+        const float base = top == -INFINITY ? 0.f : top, sub = none ? 0.f : logf(z);
+        put([&](float l) { return (l - base) - sub; });
     }
 }
 

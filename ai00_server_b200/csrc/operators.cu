@@ -2,28 +2,44 @@
 // the engine makes of them.
 #include "operators.cuh"
 #include "adapters.cuh"
+#include "adapter_tiles.cuh"
 #include "logits.cuh"
 
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <type_traits>
 
 namespace b200 {
 
 // a kernel's dynamic shared memory, once for every device that launches it
 template <auto KERN>
-static void prepare(size_t bytes) {
+static void prepare(size_t bytes, bool wide_clusters = false) {
     static std::atomic<unsigned long long> done{0};
     int dev = 0;
     CK(cudaGetDevice(&dev));
     const unsigned long long bit = 1ull << (dev & 63);
     if (done.load(std::memory_order_acquire) & bit) return;
     allow_smem(KERN, bytes);
+    if (wide_clusters) CK(cudaFuncSetAttribute(KERN, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     done.fetch_or(bit, std::memory_order_release);
 }
 
+static int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    CK(cudaGetDevice(&dev));
+    int n = known[dev & 63].load(std::memory_order_relaxed);
+    if (n == 0) {
+        CK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        known[dev & 63].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// cluster: CTAs of a cluster where the kernel does not say
 template <typename P>
-static void launch(void (*kern)(P), dim3 grid, int threads, size_t smem, cudaStream_t s, const P& p) {
+static void launch(void (*kern)(P), dim3 grid, int threads, size_t smem, cudaStream_t s, const P& p, int cluster = 0) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = grid;
@@ -31,33 +47,26 @@ static void launch(void (*kern)(P), dim3 grid, int threads, size_t smem, cudaStr
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     // starts while the kernel in front drains; every kernel here waits for that one's end before it reads anything
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster ? 2 : 1;
     CK(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
-size_t adapters_workspace(int tokens, int adapters) {
+// tiles that `tokens` tokens can need
+static int adapter_tiles(int tokens, int adapters) { return (int)std::min<long long>((long long)adapters + 1 + tokens / ADP_TILE, tokens); }
+static size_t adapter_plan_bytes(int tokens, int adapters) {
+    return (AdapterPlan::ints(tokens, adapter_groups(tokens, adapters), adapter_tiles(tokens, adapters)) * 4 + 255) & ~(size_t)255;
+}
+
+size_t adapters_workspace(int tokens, int adapters, int nparts, int rank) {
     if (tokens <= ADP_INLINE) return 0;
-    return AdapterPlan::ints(tokens, adapter_groups(tokens, adapters)) * 4;
-}
-
-void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan_kernel, dim3(1), ADP_PLAN_THREADS, 0, s, p); }
-
-template <typename E, typename O>
-static void ready() {
-    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
-}
-
-template <typename E, typename O>
-static void apply(cudaStream_t s, const AdapterParams& p, int nparts) {
-    int R = 0;
-    for (int i = 0; i < nparts; ++i) R = std::max(R, p.part[i].R);
-    const size_t smem = adapter_few_smem(R, AdpParts<E, O>::N);
-    ready<E, O>();
-    launch(adapter_few_kernel<E, O>, dim3(ADP_CTAS * adapter_groups(p.tokens, p.adapters), nparts), ADP_THREADS, smem, s, p);
+    return adapter_plan_bytes(tokens, adapters) + (size_t)nparts * adt_low_bytes(tokens, rank, 3);
 }
 
 // f(element, output) of the types of a call
@@ -68,31 +77,87 @@ static void with_types(int type, int out_type, F&& f) {
     else wide ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
 }
 
+void adapters_shape(AdapterParams& p, void* workspace, int type, int out_type) {
+    p.plan.base = nullptr;
+    if (p.tokens <= ADP_INLINE) return;
+    with_types(type, out_type, [&](auto e, auto o) { p.out_tokens = adt_out_tokens(p.rank, AdpParts<decltype(e), decltype(o)>::N); });
+    // tiles for adapters with ADT_LEAST tokens and more; for all of them where there are that many an adapter on average
+    p.tile_least = p.tokens >= (long long)ADT_LEAST * p.adapters ? 1 : ADT_LEAST;
+    p.plan.base = (int*)workspace;
+    p.plan.groups = adapter_groups(p.tokens, p.adapters);
+    p.plan.tiles = adapter_tiles(p.tokens, p.adapters);
+    p.low = (uint8_t*)workspace + adapter_plan_bytes(p.tokens, p.adapters);
+}
+
+void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan_kernel, dim3(1), ADP_PLAN_THREADS, 0, s, p); }
+
+template <typename E, typename O>
+static void ready() {
+    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
+    size_t low = 0, out = 0;
+    for (int r = 8; r <= ADP_MAX_RANK; r += 8) {
+        low = std::max<size_t>(low, adt_low_smem(r));
+        out = std::max<size_t>(out, adt_out_smem(r, AdpParts<E, O>::N));
+    }
+    prepare<adapter_low_kernel<E, AdpParts<E, O>::N>>(low);
+    prepare<adapter_out_kernel<E, O>>(out);
+}
+
+template <typename E, typename O>
+static void apply(cudaStream_t s, const AdapterParams& p) {
+    constexpr int NP = AdpParts<E, O>::N;
+    ready<E, O>();
+    int groups = adapter_groups(p.tokens, p.adapters);
+    if (p.plan.base) {
+        const int tiles = std::min(p.plan.tiles, p.tile_least > 1 ? p.tokens / p.tile_least + p.tokens / ADP_TILE : p.plan.tiles);
+        if (tiles > 0) {
+            launch(adapter_low_kernel<E, NP>, dim3(ADP_CTAS * tiles, p.nparts), ADT_LOW_THREADS, adt_low_smem(p.rank), s, p);
+            // as many CTAs as run at once, or a unit each
+            long long units = 0;
+            for (int i = 0; i < p.nparts; ++i) units += (long long)tiles * (ADP_TILE / p.out_tokens) * ((p.part[i].N + 127) / 128);
+            const size_t smem = adt_out_smem(p.rank, NP);
+            const int most = sm_count() * (smem <= ADT_HALF_SM ? 2 : 1);
+            launch(adapter_out_kernel<E, O>, dim3((unsigned)std::min<long long>(units, most)), ADT_THREADS, smem, s, p);
+        }
+        groups = p.tile_least > 1 ? std::min(groups, (p.adapters + (p.copy ? 1 : 0)) * ((p.tile_least - 1 + ADP_TOK - 1) / ADP_TOK)) : 0;
+    }
+    if (groups > 0) launch(adapter_few_kernel<E, O>, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
+}
+
 void adapters_prepare(int type, int out_type) {
     with_types(type, out_type, [](auto e, auto o) { ready<decltype(e), decltype(o)>(); });
 }
 
-void adapters_apply(cudaStream_t s, const AdapterParams& p, int nparts, int type, int out_type) {
-    with_types(type, out_type, [&](auto e, auto o) { apply<decltype(e), decltype(o)>(s, p, nparts); });
+void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type) {
+    with_types(type, out_type, [&](auto e, auto o) { apply<decltype(e), decltype(o)>(s, p); });
 }
 
-template <typename E>
-static void logits_launch(cudaStream_t s, const LogitsParams& p, int rows, size_t smem) {
-    prepare<logits_kernel<E>>(LOGITS_SMEM_MAX);
-    launch(logits_kernel<E>, dim3(rows * LOGITS_CTAS), LOGITS_THREADS, smem, s, p);
+template <typename E, int NV, bool VEC>
+static void logits_launch(cudaStream_t s, const LogitsParams& p, int rows) {
+    constexpr size_t most = (size_t)std::min(LOGITS_LIST_TOKENS, LOGITS_THREADS * NV * 4) * sizeof(uint2);
+    prepare<logits_kernel<E, NV, VEC>>(most, true);
+    launch(logits_kernel<E, NV, VEC>, dim3(rows << p.ctas_log), LOGITS_THREADS, (size_t)p.list_tokens * sizeof(uint2), s, p, 1 << p.ctas_log);
 }
 
 void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type) {
-    const int size = type == B200RWKV_TYPE_F32 ? 4 : 2;
-    p.slice = ((p.V + LOGITS_CTAS - 1) / LOGITS_CTAS + 3) & ~3;
-    p.sub = p.hist_off || p.bias_off ? std::min(p.slice, LOGITS_SUB) : 0;
-    const size_t lists = (size_t)p.sub * 8, slice = (size_t)p.slice * 4;
-    p.buffered = slice + lists <= LOGITS_SMEM_MAX;
+    const int size = type == B200RWKV_TYPE_F32 ? 4 : 2, stripes = (p.V + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
     p.vec = (uintptr_t)p.in % (4 * size) == 0 && p.in_stride % 4 == 0 && (uintptr_t)p.out % 16 == 0 && p.out_stride % 4 == 0;
-    const size_t smem = lists + (p.buffered ? slice : 0);
-    if (type == B200RWKV_TYPE_F32) logits_launch<float>(s, p, rows, smem);
-    else if (type == B200RWKV_TYPE_F16) logits_launch<__half>(s, p, rows, smem);
-    else logits_launch<__nv_bfloat16>(s, p, rows, smem);
+    // sixteen CTAs where eight would hold more than 16 tokens a thread, and for few rows, which are latency
+    p.ctas_log = p.V > 8 * LOGITS_THREADS * 16 || rows <= 9 ? 4 : 3;
+    const int tokens = ((stripes - 1) >> p.ctas_log) * LOGITS_STRIPE + LOGITS_STRIPE, each = LOGITS_THREADS * 4;
+    p.list_tokens = p.hist_off || p.bias_off ? std::min(tokens, LOGITS_LIST_TOKENS) : 0;
+    auto go = [&](auto nv) {
+        auto typed = [&](auto e) {
+            if (p.vec) logits_launch<decltype(e), decltype(nv)::value, true>(s, p, rows);
+            else logits_launch<decltype(e), decltype(nv)::value, false>(s, p, rows);
+        };
+        if (type == B200RWKV_TYPE_F32) typed(float{});
+        else if (type == B200RWKV_TYPE_F16) typed(__half{});
+        else typed(__nv_bfloat16{});
+    };
+    if (tokens <= 4 * each) go(std::integral_constant<int, 4>{});
+    else if (tokens <= 8 * each) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, 16>{});
 }
 
 // the calling thread's device for the length of a call
@@ -114,12 +179,12 @@ using namespace b200;
 
 extern "C" {
 
-int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters) {
-    if (tokens < 0 || adapters < 1 || adapters > B200RWKV_MAX_ADAPTERS) {
+int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters, int32_t num_parts, int32_t rank) {
+    if (tokens < 0 || tokens > (1 << 20) || adapters < 1 || adapters > B200RWKV_MAX_ADAPTERS || num_parts < 1 || num_parts > B200RWKV_MAX_PARTS || rank < 1 || rank > B200RWKV_MAX_RANK) {
         last_error_text() = "op_adapters_workspace: bad argument";
         return B200RWKV_ERR_INVALID;
     }
-    return (int64_t)adapters_workspace(tokens, adapters);
+    return (int64_t)adapters_workspace(tokens, adapters, num_parts, rank);
 }
 
 int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* q) {
@@ -158,20 +223,18 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
         d.out = s.out; d.out_stride = s.out_stride;
         d.K = s.in_features; d.N = s.out_features; d.R = s.rank;
         d.vec = ((uintptr_t)s.out | (uintptr_t)s.base) % (4 * osize) == 0 && s.out_stride % 4 == 0 && (!s.base || s.base_stride % 4 == 0);
+        p.rank = std::max(p.rank, s.rank);
         if (s.base != s.out || s.base_stride != s.out_stride) p.copy = 1;
     }
     if (q->tokens == 0) return B200RWKV_OK;
-    const size_t need = adapters_workspace(q->tokens, q->adapters);
+    const size_t need = adapters_workspace(q->tokens, q->adapters, q->num_parts, p.rank);
+    p.nparts = q->num_parts;
     REQUIRE(need == 0 || (q->workspace && (uintptr_t)q->workspace % 16 == 0 && q->workspace_bytes >= need), B200RWKV_ERR_INVALID,
             "op_adapters: workspace is missing, misaligned or smaller than b200rwkv_op_adapters_workspace");
     OnDevice on(device);
-    if (need) {
-        p.plan.base = (int*)q->workspace;
-        p.plan.tokens = q->tokens;
-        p.plan.most = adapter_groups(q->tokens, q->adapters);
-        adapters_plan((cudaStream_t)stream, p);
-    }
-    adapters_apply((cudaStream_t)stream, p, q->num_parts, q->type, q->out_type);
+    adapters_shape(p, q->workspace, q->type, q->out_type);
+    if (p.plan.base) adapters_plan((cudaStream_t)stream, p);
+    adapters_apply((cudaStream_t)stream, p, q->type, q->out_type);
     API_END
 }
 
@@ -180,7 +243,8 @@ int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* 
     REQUIRE(q && q->struct_bytes == sizeof(*q), B200RWKV_ERR_INVALID, "op_logits: struct_bytes must be sizeof(b200rwkv_logits)");
     REQUIRE(q->type >= B200RWKV_TYPE_F32 && q->type <= B200RWKV_TYPE_BF16, B200RWKV_ERR_UNSUPPORTED, "op_logits: logits are f32, f16 or bf16");
     REQUIRE(q->kind >= B200RWKV_LOGITS && q->kind <= B200RWKV_LOG_PROBS, B200RWKV_ERR_INVALID, "op_logits: kind must be logits, probabilities or log-probabilities");
-    REQUIRE(q->rows >= 0 && q->rows <= (1 << 24) && q->vocab >= 1 && q->vocab <= (1 << 28), B200RWKV_ERR_INVALID, "op_logits: rows or vocab out of range");
+    REQUIRE(q->rows >= 0 && q->rows <= (1 << 24) && q->vocab >= 1, B200RWKV_ERR_INVALID, "op_logits: rows or vocab out of range");
+    REQUIRE(q->vocab <= LOGITS_MAX_VOCAB, B200RWKV_ERR_UNSUPPORTED, "op_logits: vocabularies above 524288 are not supported");
     if (q->rows == 0) return B200RWKV_OK;
     const int size = q->type == B200RWKV_TYPE_F32 ? 4 : 2;
     REQUIRE(q->logits && q->out, B200RWKV_ERR_INVALID, "op_logits: null logits or out");

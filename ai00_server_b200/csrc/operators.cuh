@@ -12,6 +12,7 @@ constexpr int ADP_TOK = 8;                       // tokens of a group: the N of 
 constexpr int ADP_MAX_PARTS = 8, ADP_MAX_RANK = 256, ADP_MAX_ADAPTERS = 1024;
 constexpr int ADP_INLINE = ADP_THREADS;          // tokens of a call whose groups every CTA finds by itself; more take adapter_plan_kernel
 constexpr int ADP_PLAN_THREADS = 1024;
+constexpr int ADP_TILE = 128;                    // tokens of a tile (adapter_tiles.cuh)
 
 // one adapter of one projection, where adapters lie apart
 struct AdapterEntry {
@@ -37,14 +38,15 @@ struct AdapterPart {
     int vec;                     // rows of base and out take accesses of four elements
 };
 
-// groups of more tokens than ADP_INLINE: [0] = groups, then {adapter, first place} of each, then tokens by place
+// a call of more tokens than ADP_INLINE: counts of groups (adapters.cuh) and of tiles (adapter_tiles.cuh), {adapter, first place, tokens} of each, tokens by place
 struct AdapterPlan {
     int* base;
-    int tokens, most;            // most: groups there can be
+    int groups, tiles;           // room: as many as there can be
     __host__ __device__ int* count() const { return base; }
-    __host__ __device__ int2* group() const { return reinterpret_cast<int2*>(base + 4); }
-    __host__ __device__ int* place() const { return base + 4 + 2 * (size_t)most; }
-    __host__ __device__ static size_t ints(int tokens, int most) { return 4 + 2 * (size_t)most + tokens; }
+    __host__ __device__ int4* group() const { return reinterpret_cast<int4*>(base) + 1; }
+    __host__ __device__ int4* tile() const { return group() + groups; }
+    __host__ __device__ int* place() const { return reinterpret_cast<int*>(tile() + tiles); }
+    __host__ __device__ static size_t ints(int tokens, int groups, int tiles) { return 4 * (1 + (size_t)groups + tiles) + tokens; }
 };
 
 struct AdapterParams {
@@ -53,6 +55,11 @@ struct AdapterParams {
     const int* index;
     const float* scale;
     AdapterPlan plan;
+    int rank;                    // the largest of the parts
+    int nparts;
+    int tile_least;              // adapters with fewer tokens than this go by groups
+    int out_tokens;              // tokens of a unit of the second tile kernel
+    uint8_t* low;                // S between the tile kernels (adapter_tiles.cuh)
     AdapterPart part[ADP_MAX_PARTS];
 };
 
@@ -62,19 +69,24 @@ __host__ __device__ inline int adapter_groups(int tokens, int adapters) {
     return (int)(full < tokens ? full : tokens);
 }
 
-// bytes of the plan that a call of this many tokens needs (0: none)
-B200_HIDDEN size_t adapters_workspace(int tokens, int adapters);
+// bytes that a call of this many tokens needs (0: none), for parts of up to this rank
+B200_HIDDEN size_t adapters_workspace(int tokens, int adapters, int nparts, int rank);
+// p.plan, p.low and the forms its tokens take, from p.tokens, p.adapters, p.rank and the types
+B200_HIDDEN void adapters_shape(AdapterParams& p, void* workspace, int type, int out_type);
 // sets up the kernels of a type; a captured call needs it beforehand
 B200_HIDDEN void adapters_prepare(int type, int out_type);
 // orders the tokens of a longer call by adapter; its groups serve any number of adapters_apply calls with the same tokens
 B200_HIDDEN void adapters_plan(cudaStream_t s, const AdapterParams& p);
-// parts [0, nparts) of p; type: B200RWKV_TYPE_F16 / _BF16, out_type: that or _F32
-B200_HIDDEN void adapters_apply(cudaStream_t s, const AdapterParams& p, int nparts, int type, int out_type);
+// the p.nparts parts of p; type: B200RWKV_TYPE_F16 / _BF16, out_type: that or _F32
+B200_HIDDEN void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type);
 
 // ---- rows of logits ----
-constexpr int LOGITS_CTAS = 8, LOGITS_THREADS = 256;
-constexpr int LOGITS_SUB = 8192;                 // tokens of a slice that a pass over the lists covers
-constexpr size_t LOGITS_SMEM_MAX = 220 * 1024;
+constexpr int LOGITS_THREADS = 512;
+constexpr int LOGITS_STRIPE = 64;                // neighbouring tokens of a CTA; the next ones are the next CTA's
+constexpr int LOGITS_MOST_CTAS = 16;             // CTAs of a row
+constexpr int LOGITS_LIST_TOKENS = 16384;        // tokens of a CTA whose sums lie in shared memory at once
+constexpr int LOGITS_MAX_HISTORY = (1 << 17) - 1;
+constexpr int LOGITS_MAX_VOCAB = LOGITS_MOST_CTAS * LOGITS_THREADS * 64;
 enum LogitsKind : int { LOGITS_ROWS = 0, LOGITS_PROBS = 1, LOGITS_LOGPROBS = 2 };
 
 struct LogitsParams {
@@ -82,11 +94,11 @@ struct LogitsParams {
     long long in_stride;         // elements
     float* out;
     long long out_stride;
-    int V, slice;                // slice: tokens of a CTA, a multiple of 4
+    int V;
     int kind;
     int vec;                     // rows start on 16-byte boundaries (in and out)
-    int buffered;                // the slice fits shared memory; else it waits in `out`
-    int sub;                     // tokens of a pass over the lists (0: no lists)
+    int ctas_log;                // log2 of the CTAs of a row
+    int list_tokens;             // tokens of a CTA whose sums lie in shared memory at once (0: no lists)
     const int* in_row;           // row of `in` of each output row (null: the same)
     const float* controls;       // [rows][5]: repetition, presence, frequency, decay, temperature
     const int* hist_off;
@@ -100,7 +112,7 @@ struct LogitsParams {
     const float* bias_val;
 };
 
-// slice, sub, buffered and vec of p are filled in here
+// ctas_log, list_tokens and vec of p are filled in here; V is at most LOGITS_MAX_VOCAB
 B200_HIDDEN void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type);
 
 }  // namespace b200

@@ -35,7 +35,7 @@ void b200rwkv_engine::adapter_setup() {
     CK(cudaDeviceSynchronize());
 }
 
-size_t b200rwkv_engine::adapter_ws_bytes() const { return (adapters_workspace(std::max(maxT, ADP_INLINE + 1), ADAPTER_POOL) + 255) & ~(size_t)255; }
+size_t b200rwkv_engine::adapter_ws_bytes() const { return (adapters_workspace(std::max(maxT, ADP_INLINE + 1), ADAPTER_POOL, GEMM_MAX_SEG, ADP_MAX_RANK) + 255) & ~(size_t)255; }
 
 uint64_t b200rwkv_engine::adapter_load(const StFile& st, float alpha) {
     REQUIRE(!kx && world == 1, B200RWKV_ERR_UNSUPPORTED, "adapters of slots: RWKV models on one GPU");
@@ -131,11 +131,8 @@ AdapterParams b200rwkv_engine::adapter_params(int rows, bool out_rows) const {
     p.tokens = rows;
     p.adapters = ADAPTER_POOL;
     p.index = out_rows ? d_index_tok + maxT : d_index_tok;
-    if (adapters_workspace(rows, ADAPTER_POOL)) {
-        p.plan.base = (int*)(adapter_ws + (out_rows ? adapter_ws_bytes() : 0));
-        p.plan.tokens = rows;
-        p.plan.most = adapter_groups(rows, ADAPTER_POOL);
-    }
+    p.rank = adapter_rank;
+    adapters_shape(p, adapter_ws + (out_rows ? adapter_ws_bytes() : 0), B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
     return p;
 }
 
@@ -188,7 +185,8 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
         d.vec = sg.ldo % 4 == 0 && (uintptr_t)sg.out % 16 == 0;
     }
     if (n == 0) return;
-    adapters_apply(s, p, n, B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
+    p.nparts = n;
+    adapters_apply(s, p, B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
     ++launches_last_step;
     for (int i = 0; i < gp.nseg; ++i) {
         const GemmSeg &sg = gp.seg[i], &to = was.seg[i];
@@ -202,6 +200,7 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
 void b200rwkv_engine::sample_rows(int nrows, const b200rwkv_row_controls& q, float* out) {
     REQUIRE(rank == 0, B200RWKV_ERR_INVALID, "sample_rows: only rank 0 holds the gathered logits");
     REQUIRE(d_keep, B200RWKV_ERR_UNSUPPORTED, "sample_rows: the model keeps no logits rows");
+    REQUIRE(V <= LOGITS_MAX_VOCAB, B200RWKV_ERR_UNSUPPORTED, "sample_rows: vocabularies above 524288 are not supported");
     REQUIRE(nrows >= 0 && nrows <= 4096 && (nrows == 0 || (q.slots && out)), B200RWKV_ERR_INVALID, "sample_rows: bad argument");
     REQUIRE(q.kind >= B200RWKV_LOGITS && q.kind <= B200RWKV_LOG_PROBS, B200RWKV_ERR_INVALID, "sample_rows: kind must be logits, probabilities or log-probabilities");
     if (nrows == 0) return;

@@ -99,7 +99,7 @@ def low_rank(x, a, b, index, scale, base=None, out=None, out_dtype=None):
         p.in_features, p.out_features, p.rank = k, width, rank
     q.parts = parts
     lib = capi.lib()
-    need = lib.b200rwkv_op_adapters_workspace(tokens, adapters)
+    need = lib.b200rwkv_op_adapters_workspace(tokens, adapters, n, max(w.shape[1] for w in a))
     if need > 0:
         work = torch.empty(need, dtype=torch.uint8, device=device)
         q.workspace, q.workspace_bytes = work.data_ptr(), need

@@ -356,7 +356,8 @@ typedef struct {
     void* workspace;             /* b200rwkv_op_adapters_workspace bytes, 16-byte aligned; contents before and after do not matter */
     size_t workspace_bytes;
 } b200rwkv_adapters;
-int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters);      /* 0: none is needed; negative: a status */
+/* rank: the largest of the parts.  0: none is needed; negative: a status */
+int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters, int32_t num_parts, int32_t rank);
 int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* args);
 
 /* Rows of logits adjusted for their requests, as logits, probabilities or log-probabilities.  For row i, token t, with the row's
@@ -366,7 +367,7 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
  *     l += the last bias value listed for t;   l = -inf where bit t of the row's mask is 0;   l /= temperature
  * A row of which the mask leaves nothing has probabilities 0 and log-probabilities -inf; a NaN that the mask leaves makes a row of
  * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number makes any row NaN; decay is
- * taken into [0, 1].  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
+ * taken into [0, 1].  Vocabularies of up to 524288 tokens; of a history, the newest 131071 tokens.  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
  * sampler/bnf.rs:35-38, run.rs:679-681 and softmax (run.rs:1179) of the samplers that need whole rows. */
 typedef struct {
     uint32_t struct_bytes;

@@ -43,12 +43,12 @@ def test_op_adapters_null_struct_and_no_tokens():
 
 
 def test_op_adapters_workspace():
-    lib = capi.lib()
-    assert lib.b200rwkv_op_adapters_workspace(256, 4) == 0
-    assert lib.b200rwkv_op_adapters_workspace(257, 4) > 257 * 4
-    assert lib.b200rwkv_op_adapters_workspace(-1, 4) == capi.ERR_INVALID
-    assert lib.b200rwkv_op_adapters_workspace(8, 0) == capi.ERR_INVALID
-    assert lib.b200rwkv_op_adapters_workspace(8, 1025) == capi.ERR_INVALID
+    f = capi.lib().b200rwkv_op_adapters_workspace
+    assert f(256, 4, 1, 16) == 0
+    assert f(257, 4, 1, 16) > 257 * 4
+    assert f(1000, 4, 1, 16) < f(1000, 4, 2, 16) and f(1000, 4, 1, 64) < f(1000, 4, 1, 65)
+    for bad in [(-1, 4, 1, 16), ((1 << 20) + 1, 4, 1, 16), (8, 0, 1, 16), (8, 1025, 1, 16), (8, 4, 0, 16), (8, 4, 9, 16), (8, 4, 1, 0), (8, 4, 1, 257)]:
+        assert f(*bad) == capi.ERR_INVALID
 
 
 def _logits(**change):
