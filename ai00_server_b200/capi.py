@@ -74,6 +74,7 @@ class RowControls(C.Structure):
 TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
 LOGITS, PROBS, LOG_PROBS = 0, 1, 2
 MAX_PARTS, MAX_RANK, MAX_ADAPTERS = 8, 256, 1024
+ADAPTERS_WITHOUT_WORKSPACE = 256          # tokens of a b200rwkv_op_adapters call that needs none
 QUANT_NONE, QUANT_INT8, QUANT_NF4 = 0, 1, 2
 ARCH_KEMIRAX = 100          # Info.version of the config.json-described families
 ARCH_DEGAVIK = 101

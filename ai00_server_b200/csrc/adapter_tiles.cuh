@@ -70,20 +70,6 @@ __device__ __forceinline__ bool adt_bar_wait(uint32_t bar, uint32_t parity) {
     return true;
 }
 
-// four neighbours of a row of base as they lie in memory
-template <typename O> struct AdtRaw {
-    using Four = uint2;
-    static __device__ __forceinline__ void widen(const uint2& r, float (&v)[4]) {
-        const O* const e = reinterpret_cast<const O*>(&r);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = AdpType<O>::widen(e[i]);
-    }
-};
-template <> struct AdtRaw<float> {
-    using Four = float4;
-    static __device__ __forceinline__ void widen(const float4& r, float (&v)[4]) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
-};
-
 // the adapter of a tile in one projection
 template <typename E>
 struct AdtWeights {
@@ -391,7 +377,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
     };
     // base of four tokens of the 32, four outputs a lane, as they lie in memory: widened where they are used, or the loads would be waited for here
     constexpr int OWN = ADT_ROWS / (ADT_THREADS / 32);
-    using Raw = typename AdtRaw<O>::Four;
+    using Raw = typename AdpRaw<O>::Four;
     Raw y[OWN];
     auto load_base = [&](const Unit& x, int buf, int c) {
         const int t0 = c + warp * OWN;
@@ -475,7 +461,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
             float w[OWN][4];
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
-                AdtRaw<O>::widen(y[i], w[i]);
+                AdpRaw<O>::widen(y[i], w[i]);
                 if (!cur.R) continue;
                 const float back = fine ? s_back[buf][(c + t0 + i) & (ADT_TOK - 1)] : __int_as_float(0x7fc00000);
                 const float4 x = *reinterpret_cast<const float4*>(st + (t0 + i) * ADT_PITCH + lane * 4);

@@ -10,6 +10,8 @@
 // the second; between them the eight partial S (R x 8 floats) go to every CTA of the cluster in one exchange, so that nothing but x, A, B, base and out
 // touches memory.  Both products are m16n8k16 with the adapter's rows as M and the eight tokens as N: a lane reads 16 bytes of a row at a time, which
 // is two steps of k for it (the order of k within 32 is the same permutation on both sides of a product, so it is never undone).
+// A group of a single token (every request with its own adapter) goes without the tensor cores, of which it would use one column in eight: 448 units of 32
+// outputs at rank 32 for each of 64 tokens are 12400 cycles of m16n8k16 and 4100 of f32 multiply-adds.
 // S is f32; the second product takes it as two or three 16-bit parts, enough for the output's type, scaled per token by a power of two.
 #pragma once
 #include <cuda_bf16.h>
@@ -44,17 +46,19 @@ template <> struct AdpParts<__nv_bfloat16, float> { static constexpr int N = 3; 
 
 __device__ __forceinline__ uint4 adp_ld16(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 
-__device__ __forceinline__ void adp_load4(const float* p, float (&v)[4]) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-}
-template <typename O>
-__device__ __forceinline__ void adp_load4(const O* p, float (&v)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const O* e = reinterpret_cast<const O*>(&u);
+// four neighbours of a row as they lie in memory: widened where they are used, or a load would be waited for where it is made
+template <typename O> struct AdpRaw {
+    using Four = uint2;
+    static __device__ __forceinline__ void widen(const uint2& r, float (&v)[4]) {
+        const O* const e = reinterpret_cast<const O*>(&r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = AdpType<O>::widen(e[i]);
-}
+        for (int i = 0; i < 4; ++i) v[i] = AdpType<O>::widen(e[i]);
+    }
+};
+template <> struct AdpRaw<float> {
+    using Four = float4;
+    static __device__ __forceinline__ void widen(const float4& r, float (&v)[4]) { v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w; }
+};
 __device__ __forceinline__ void adp_store4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
 template <typename O>
 __device__ __forceinline__ void adp_store4(O* p, const float (&v)[4]) {
@@ -71,31 +75,78 @@ __device__ __forceinline__ void adp_put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void adp_put(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void adp_put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// eight 16-bit numbers, widened
+__device__ __forceinline__ void adp_widen8(const uint4& u, float (&f)[8], __half) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = v.x; f[2 * i + 1] = v.y;
+    }
+}
+__device__ __forceinline__ void adp_widen8(const uint4& u, float (&f)[8], __nv_bfloat16) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+template <typename E>
+__device__ __forceinline__ float adp_dot8(const uint4& a, const float (&x)[8], float s) {
+    float f[8];
+    adp_widen8(a, f, E{});
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fmaf(f[i], x[i], s);
+    return s;
+}
+
 struct AdpGroup {
     int tok[ADP_TOK];            // tokens, -1 behind the last
     int adapter;                 // -1: none
     int found;
+    int alone;                   // a single token
 };
 
-// group `want` of a call of up to ADP_INLINE tokens, found by all threads of a CTA: a group starts at a token whose number of earlier tokens with
-// the same adapter is a multiple of ADP_TOK, groups count in the order of their first tokens
+// group `want` of a call of up to ADP_INLINE tokens, found by every CTA for itself: a group starts at a token whose number of earlier tokens with
+// the same adapter is a multiple of ADP_TOK, groups count in the order of their first tokens.  Up to 32 tokens are one warp's work and one barrier
 __device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const int want, AdpGroup& g, int* s_idx, int* s_cnt) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const bool one = p.tokens <= 32;
+    const unsigned before = (1u << lane) - 1u;
     int id = -2;
     if (tid < p.tokens) {
         id = p.index[tid];
         if (id < 0 || id >= p.adapters) id = p.copy ? -1 : -2;
     }
+    if (one) {
+        if (warp == 0) {
+            const int rank = __popc(__match_any_sync(0xffffffffu, id) & before);
+            const bool start = id >= -1 && rank % ADP_TOK == 0;
+            const unsigned starts = __ballot_sync(0xffffffffu, start), mine = __ballot_sync(0xffffffffu, start && __popc(starts & before) == want);
+            const int from = mine ? __ffs(mine) - 1 : 0;
+            const int adapter = __shfl_sync(0xffffffffu, id, from), first = __shfl_sync(0xffffffffu, rank, from);
+            if (lane < ADP_TOK) g.tok[lane] = -1;
+            __syncwarp();
+            if (mine && id == adapter && rank >= first && rank < first + ADP_TOK) g.tok[rank - first] = lane;
+            if (lane == 0) {
+                g.adapter = adapter;
+                g.found = mine != 0;
+            }
+        }
+        __syncthreads();
+        return;
+    }
     s_idx[tid] = id;
     if (tid < ADP_TOK) g.tok[tid] = -1;
     if (tid == 0) g.found = 0;
     __syncthreads();
-    const unsigned before = (1u << lane) - 1u;
     int rank = __popc(__match_any_sync(0xffffffffu, id) & before);
-    for (int w = 0; w < warp * 32; w += 4) {
-        const int4 v = *reinterpret_cast<const int4*>(s_idx + w);
-        rank += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
-    }
+    if (warp * 32 < p.tokens)
+        for (int w = 0; w < warp * 32; w += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(s_idx + w);
+            rank += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
+        }
     const bool start = id >= -1 && rank % ADP_TOK == 0;
     const unsigned starts = __ballot_sync(0xffffffffu, start);
     if (lane == 0) s_cnt[warp] = __popc(starts);
@@ -111,8 +162,10 @@ __device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const
     __syncthreads();
 }
 
-template <typename E, typename O>
-__global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) adapter_few_kernel(const __grid_constant__ AdapterParams p) {
+// MANY: registers for four CTAs on an SM instead of three, where a call has more than three for each (64 tokens with adapters of rank 32 to 14336 outputs, 512
+// CTAs, 20 us; with three 25; 16 tokens of four projections, 320 CTAs, 8.5 and 7.7)
+template <typename E, typename O, bool MANY>
+__global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, MANY ? 4 : 3) adapter_few_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ AdpGroup g;
     __shared__ __align__(16) int s_idx[ADP_THREADS];
@@ -127,11 +180,16 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
         if (want >= p.plan.count()[0]) return;
         const int4 gr = p.plan.group()[want];
         if (tid < ADP_TOK) g.tok[tid] = tid < gr.z ? p.plan.place()[gr.y + tid] : -1;
-        if (tid == 0) g.adapter = gr.x;
+        if (tid == 0) {
+            g.adapter = gr.x;
+            g.alone = gr.w;
+        }
         __syncthreads();
     } else {
         adapter_find_group(p, want, g, s_idx, s_cnt);
         if (!g.found) return;
+        if (tid == 0) g.alone = g.tok[1] < 0;
+        __syncthreads();
     }
     const int adapter = g.adapter, K = q.K, N = q.N;
     O* const out = reinterpret_cast<O*>(q.out);
@@ -163,10 +221,120 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
     }
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
+    if (g.alone) {
+        // ---- one token ----
+        const int tok = g.tok[0];
+        float* const part = reinterpret_cast<float*>(smem_raw);                  // [warp][R]
+        float* const all = part + ADP_WARPS * p.rank;                            // [CTA][R]
+        float* const sum = all + ADP_CTAS * p.rank;                              // [R rounded to 32]
+        const E* const x = reinterpret_cast<const E*>(q.x);
+        auto xat = [&](int k, int lo) { return q.x_a16 ? x + a16_index(tok + lo, k, q.x_th) : x + (size_t)(tok + lo) * q.x_stride + k; };
+        const int nk = (K + 31) / 32, c0 = (int)((long long)nk * cta / ADP_CTAS), c1 = (int)((long long)nk * (cta + 1) / ADP_CTAS);
+        for (int m0 = 0; m0 < R; m0 += 64) {
+            float acc[8] = {};                       // ranks m0 + row + 8 i
+            for (int c = c0 + warp; c < c1; c += ADP_WARPS) {
+                const int k = c * 32 + quad * 8;
+                if (k >= K) continue;
+                uint4 a[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    a[i] = make_uint4(0, 0, 0, 0);
+                    if (m0 + i * 8 < R) a[i] = adp_ld16(A + (size_t)(m0 + i * 8 + row) * K + k);
+                }
+                float xf[8];
+                adp_widen8(adp_ld16(xat(k, 0)), xf, E{});
+                if (q.x_lo) {                        // (hi + lo is exact in f32)
+                    float xl[8];
+                    adp_widen8(adp_ld16(xat(k, q.x_lo)), xl, E{});
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) xf[i] += xl[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] = adp_dot8<E>(a[i], xf, acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 1);
+                acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 2);
+                if (quad == 0 && m0 + i * 8 < R) part[warp * R + m0 + i * 8 + row] = acc[i];
+            }
+        }
+        __syncthreads();
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");      // every CTA of the cluster has started
+        for (int r = tid; r < R; r += ADP_THREADS) {
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < ADP_WARPS; ++w) v += part[w * R + r];
+            const uint32_t local = smem_u32(all + cta * R + r);
+#pragma unroll
+            for (int c = 0; c < ADP_CTAS; ++c) {
+                uint32_t remote;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(c));
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+            }
+        }
+        uint4 w[4];
+        auto load_b = [&](int u, int r0) {           // four rows of B for a lane, 32 ranks at a time
+            const int n = u * 32 + row * 4, r = r0 + quad * 8;
+            const E* const from = B + (size_t)n * R + r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = make_uint4(0, 0, 0, 0);
+                if (u < u1 && n + i < N && r < R) w[i] = adp_ld16(from + (size_t)i * R);
+            }
+        };
+        load_b(u0 + warp, 0);
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        for (int r = tid; r < ((R + 31) & ~31); r += ADP_THREADS) {
+            float v = 0.f;
+            if (r < R)
+#pragma unroll
+                for (int c = 0; c < ADP_CTAS; ++c) v += all[c * R + r];
+            sum[r] = v * scale;
+        }
+        __syncthreads();
+        for (int u = u0 + warp; u < u1; u += ADP_WARPS) {
+            const int n = u * 32 + lane;             // the column that this lane ends up with
+            const bool ok = n < N;
+            const O y = ok && base ? base[(size_t)tok * q.base_stride + n] : O(0.f);
+            float acc[4] = {};
+            for (int r0 = 0; r0 < R; r0 += 32) {
+                float s[8];
+                *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sum + r0 + quad * 8);
+                *reinterpret_cast<float4*>(s + 4) = *reinterpret_cast<const float4*>(sum + r0 + quad * 8 + 4);
+                uint4 v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = w[i];
+                if (r0 + 32 < R) load_b(u, r0 + 32);
+                else load_b(u + ADP_WARPS, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = adp_dot8<E>(v[i], s, acc[i]);
+            }
+            // four columns over four lanes: each lane keeps its own
+            const bool up = quad & 2, odd = quad & 1;
+            const float k0 = (up ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, up ? acc[0] : acc[2], 2);
+            const float k1 = (up ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, up ? acc[1] : acc[3], 2);
+            const float d = (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 1);
+            if (ok) adp_put(out + (size_t)tok * q.out_stride + n, adp_widen(y) + d);
+        }
+        return;
+    }
+
     const int R8 = R * ADP_TOK, Rp = (R + 31) & ~31, pitch = Rp + 8;
     float* const part = reinterpret_cast<float*>(smem_raw);                      // [warp][R][8]: partial sums of the CTA's warps
     float* const all = part + (size_t)ADP_WARPS * p.rank * ADP_TOK;                 // [CTA][R][8]
     E* const frag = reinterpret_cast<E*>(all + (size_t)ADP_CTAS * p.rank * ADP_TOK);        // [part][token][pitch]
+
+    // four rows of B for a lane, 32 ranks at a time
+    auto load_b = [&](int u, int r0, uint4 (&w)[4]) {
+        const int n = u * 32 + row * 4, r = r0 + quad * 8;
+        const E* const from = B + (size_t)n * R + r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = make_uint4(0, 0, 0, 0);
+            if (u < u1 && n + i < N && r < R) w[i] = adp_ld16(from + (size_t)i * R);
+        }
+    };
 
     // ---- S: this CTA's k, a run of 32 of them to a warp at a time ----
     {
@@ -229,6 +397,8 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
             asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(s.x), "f"(s.y), "f"(s.z), "f"(s.w) : "memory");
         }
     }
+    uint4 w[4];
+    load_b(u0 + warp, 0, w);
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 
     // ---- S of a token (one to a warp): sum over the CTAs in their order, scale, 16-bit parts relative to the token's largest ----
@@ -272,15 +442,18 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
     const float backa = s_back[quad * 2], backb = s_back[quad * 2 + 1];
     for (int u = u0 + warp; u < u1; u += ADP_WARPS) {
         const int n = u * 32 + row * 4;
+        const bool four = q.vec && n + 3 < N;
+        typename AdpRaw<O>::Four ya{}, yb{};             // base of the lane's two tokens
+        if (base && four) {
+            if (ta >= 0) ya = *reinterpret_cast<const typename AdpRaw<O>::Four*>(base + (size_t)ta * q.base_stride + n);
+            if (tb >= 0) yb = *reinterpret_cast<const typename AdpRaw<O>::Four*>(base + (size_t)tb * q.base_stride + n);
+        }
         float acc[2][4] = {};
         for (int r0 = 0; r0 < R; r0 += 32) {
+            uint4 v[4];
+            if (r0 + 32 < R) load_b(u, r0 + 32, v);
+            else load_b(u + ADP_WARPS, 0, v);
             const int r = r0 + quad * 8;
-            uint4 w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = make_uint4(0, 0, 0, 0);
-                if (n + i < N && r < R) w[i] = adp_ld16(B + (size_t)(n + i) * R + r);
-            }
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
                 const uint4 s = adp_ld16(frag + ((size_t)k * ADP_TOK + row) * pitch + r);
@@ -290,6 +463,8 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
                     AdpType<E>::mma(acc[i], w[2 * i].z, w[2 * i + 1].z, w[2 * i].w, w[2 * i + 1].w, s.z, s.w);
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = v[i];
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -299,9 +474,9 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS) 
             const float d[4] = {acc[0][h] * back, acc[0][2 + h] * back, acc[1][h] * back, acc[1][2 + h] * back};
             O* const o = out + (size_t)t * q.out_stride + n;
             const O* const y = base ? base + (size_t)t * q.base_stride + n : nullptr;
-            if (q.vec && n + 3 < N) {
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (y) adp_load4(y, v);
+            if (four) {
+                float v[4];
+                AdpRaw<O>::widen(h ? yb : ya, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += d[i];
                 adp_store4(o, v);
@@ -317,7 +492,8 @@ inline size_t adapter_few_smem(int R, int elem_parts) {
 }
 
 // Tokens of a longer call ordered by adapter, its groups and its tiles: one CTA, a counting sort.  Where a token lands within its adapter depends on the order of
-// the atomics, its result does not: columns and rows of a product do not see each other.
+// the atomics, its result does not: columns and rows of a product do not see each other, and a token goes alone only where its adapter has no other
+// (the one left over from groups of eight could be any).
 __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __grid_constant__ AdapterParams p) {
     __shared__ int s_count[ADP_MAX_ADAPTERS + 1], s_first[ADP_MAX_ADAPTERS + 1], s_warp[3][ADP_PLAN_THREADS / 32], s_total[3];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = p.adapters + (p.copy ? 1 : 0);
@@ -364,7 +540,7 @@ __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __
             const int id = b == p.adapters ? -1 : b, step = tiled ? ADP_TILE : ADP_TOK;
             s_first[b] = at[0];
             int4* const to = tiled ? p.plan.tile() + at[2] : p.plan.group() + at[1];
-            for (int i = 0; i * step < c; ++i) to[i] = make_int4(id, at[0] + i * step, min(step, c - i * step), 0);
+            for (int i = 0; i * step < c; ++i) to[i] = make_int4(id, at[0] + i * step, min(step, c - i * step), c == 1);
         }
         __syncthreads();
         if (tid == ADP_PLAN_THREADS - 1)

@@ -93,14 +93,20 @@ void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan
 
 template <typename E, typename O>
 static void ready() {
-    prepare<adapter_few_kernel<E, O>>(adapter_few_smem(ADP_MAX_RANK, AdpParts<E, O>::N));
-    size_t low = 0, out = 0;
-    for (int r = 8; r <= ADP_MAX_RANK; r += 8) {
-        low = std::max<size_t>(low, adt_low_smem(r));
-        out = std::max<size_t>(out, adt_out_smem(r, AdpParts<E, O>::N));
-    }
-    prepare<adapter_low_kernel<E, AdpParts<E, O>::N>>(low);
-    prepare<adapter_out_kernel<E, O>>(out);
+    constexpr int NP = AdpParts<E, O>::N;
+    struct Most { size_t low = 0, out = 0; };
+    static const Most most = [] {
+        Most m;
+        for (int r = 8; r <= ADP_MAX_RANK; r += 8) {
+            m.low = std::max<size_t>(m.low, adt_low_smem(r));
+            m.out = std::max<size_t>(m.out, adt_out_smem(r, NP));
+        }
+        return m;
+    }();
+    prepare<adapter_few_kernel<E, O, false>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    prepare<adapter_few_kernel<E, O, true>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    prepare<adapter_low_kernel<E, NP>>(most.low);
+    prepare<adapter_out_kernel<E, O>>(most.out);
 }
 
 template <typename E, typename O>
@@ -121,7 +127,10 @@ static void apply(cudaStream_t s, const AdapterParams& p) {
         }
         groups = p.tile_least > 1 ? std::min(groups, (p.adapters + (p.copy ? 1 : 0)) * ((p.tile_least - 1 + ADP_TOK - 1) / ADP_TOK)) : 0;
     }
-    if (groups > 0) launch(adapter_few_kernel<E, O>, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
+    if (groups > 0) {
+        const bool many = (long long)ADP_CTAS * groups * p.nparts > 3 * sm_count();
+        launch(many ? adapter_few_kernel<E, O, true> : adapter_few_kernel<E, O, false>, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
+    }
 }
 
 void adapters_prepare(int type, int out_type) {
@@ -189,7 +198,8 @@ int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters, int32_t
 
 int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* q) {
     API_BEGIN((b200rwkv_engine*)nullptr)
-    static_assert(B200RWKV_MAX_PARTS == ADP_MAX_PARTS && B200RWKV_MAX_RANK == ADP_MAX_RANK && B200RWKV_MAX_ADAPTERS == ADP_MAX_ADAPTERS, "limits");
+    static_assert(B200RWKV_MAX_PARTS == ADP_MAX_PARTS && B200RWKV_MAX_RANK == ADP_MAX_RANK && B200RWKV_MAX_ADAPTERS == ADP_MAX_ADAPTERS &&
+                      B200RWKV_ADAPTERS_WITHOUT_WORKSPACE == ADP_INLINE, "limits");
     REQUIRE(q && q->struct_bytes == sizeof(*q), B200RWKV_ERR_INVALID, "op_adapters: struct_bytes must be sizeof(b200rwkv_adapters)");
     REQUIRE(q->type == B200RWKV_TYPE_F16 || q->type == B200RWKV_TYPE_BF16, B200RWKV_ERR_UNSUPPORTED, "op_adapters: x, a and b are f16 or bf16");
     REQUIRE(q->out_type == q->type || q->out_type == B200RWKV_TYPE_F32, B200RWKV_ERR_UNSUPPORTED, "op_adapters: out is f32 or of the type of x");

@@ -18,16 +18,18 @@ from . import capi
 _TYPE = {torch.float32: capi.TYPE_F32, torch.float16: capi.TYPE_F16, torch.bfloat16: capi.TYPE_BF16}
 _KIND = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
 _PARTS = [None] + [capi.AdapterPart * n for n in range(1, capi.MAX_PARTS + 1)]
+_ADAPTERS_BYTES, _LOGITS_BYTES = C.sizeof(capi.Adapters), C.sizeof(capi.Logits)
+_I32, _F32 = torch.int32, torch.float32
+# the current stream of a device as a number: a call for a few microseconds of work has no time for a stream object
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _bad(what: str):
     raise capi.B200Error(capi.ERR_INVALID, what)
 
 
-def _check_list(t, name, dtype, device, size=None):
-    """A contiguous vector or table of `dtype` on `device`; its address (None for None)."""
-    if t is None:
-        return None
+def _list(t, name, dtype, device, size):
+    """Address of a contiguous vector or table of `dtype` on `device` with `size` elements (None: any number)."""
     if t.dtype is not dtype or t.device != device or not t.is_contiguous():
         _bad(f"{name} must be a contiguous {dtype} tensor on {device}")
     if size is not None and t.numel() != size:
@@ -35,14 +37,14 @@ def _check_list(t, name, dtype, device, size=None):
     return t.data_ptr()
 
 
-def _rows(t, name, rows, cols, dtype, device):
-    """[rows, cols] with neighbouring columns; (address, elements between rows)."""
-    if t.dtype is not dtype or t.device != device or t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+def _row_stride(t, name, rows, cols, dtype, device):
+    """Elements between the rows of a [rows, cols] tensor with neighbouring columns."""
+    if t.dtype is not dtype or t.device != device or tuple(t.shape) != (rows, cols):
         _bad(f"{name} must be a [{rows}, {cols}] {dtype} tensor on {device}")
     s0, s1 = t.stride()
     if s1 != 1 and cols > 1:
         _bad(f"{name}: columns of a row must be neighbours")
-    return t.data_ptr(), (s0 if rows > 1 else max(s0, cols))
+    return s0 if rows > 1 else cols
 
 
 def low_rank(x, a, b, index, scale, base=None, out=None, out_dtype=None):
@@ -65,47 +67,38 @@ def low_rank(x, a, b, index, scale, base=None, out=None, out_dtype=None):
     dtype, device = x0.dtype, x0.device
     if device.type != "cuda":
         _bad("low_rank: tensors must be in GPU memory")
-    if x0.dim() != 2 or a[0].dim() != 3:
-        _bad("low_rank: x is [tokens, in], a is [adapters, rank, in]")
+    if x0.dim() != 2 or a[0].dim() != 3 or b[0].dim() != 3:
+        _bad("low_rank: x is [tokens, in], a is [adapters, rank, in], b is [adapters, out, rank]")
     tokens, adapters = x0.shape[0], a[0].shape[0]
     if out is None:
         if out_dtype is None:
             out_dtype = dtype if base is None else base[0].dtype
-        out = [torch.empty(tokens, w.shape[1] if w.dim() == 3 else 0, dtype=out_dtype, device=device) for w in b]
+        out = [torch.empty(tokens, w.shape[1], dtype=out_dtype, device=device) for w in b]
     o_dtype = out[0].dtype
-    q = capi.Adapters()
-    q.struct_bytes = C.sizeof(capi.Adapters)
-    q.type, q.out_type = _TYPE.get(dtype, -1), _TYPE.get(o_dtype, -1)
-    q.tokens, q.adapters, q.num_parts = tokens, adapters, n
-    q.index = _check_list(index, "index", torch.int32, device, tokens)
-    q.scale = _check_list(scale, "scale", torch.float32, device, adapters)
-    parts = _PARTS[n]()
+    parts, top = _PARTS[n](), 1
     for i in range(n):
-        p, ai, bi = parts[i], a[i], b[i]
+        ai, bi, xi, oi = a[i], b[i], x[i], out[i]
         if ai.dim() != 3 or bi.dim() != 3:
             _bad("low_rank: a is [adapters, rank, in], b is [adapters, out, rank]")
-        _, rank, k = ai.shape
-        width = bi.shape[1]
-        if ai.shape[0] != adapters or bi.shape[0] != adapters or bi.shape[2] != rank:
+        m, rank, k = ai.shape
+        mb, width, rb = bi.shape
+        if m != adapters or mb != adapters or rb != rank:
             _bad("low_rank: shapes of a and b do not match")
-        p.x, p.x_stride = _rows(x[i], "x", tokens, k, dtype, device)
-        if tokens == 1:
-            p.x_stride = k
-        p.a = _check_list(ai, "a", dtype, device)
-        p.b = _check_list(bi, "b", dtype, device)
-        if base is not None:
-            p.base, p.base_stride = _rows(base[i], "base", tokens, width, o_dtype, device)
-        p.out, p.out_stride = _rows(out[i], "out", tokens, width, o_dtype, device)
-        p.in_features, p.out_features, p.rank = k, width, rank
-    q.parts = parts
-    lib = capi.lib()
-    need = lib.b200rwkv_op_adapters_workspace(tokens, adapters, n, max(w.shape[1] for w in a))
-    if need > 0:
+        if rank > top:
+            top = rank
+        yi = base[i] if base is not None else None
+        parts[i] = (xi.data_ptr(), _row_stride(xi, "x", tokens, k, dtype, device), _list(ai, "a", dtype, device, None), _list(bi, "b", dtype, device, None),
+                    None if yi is None else yi.data_ptr(), 0 if yi is None else _row_stride(yi, "base", tokens, width, o_dtype, device),
+                    oi.data_ptr(), _row_stride(oi, "out", tokens, width, o_dtype, device), k, width, rank, 0)
+    lib, where = capi.lib(), device.index
+    work, need = None, 0
+    if tokens > capi.ADAPTERS_WITHOUT_WORKSPACE:
+        need = lib.b200rwkv_op_adapters_workspace(tokens, adapters, n, min(top, capi.MAX_RANK))
+        capi.check(min(need, 0))
         work = torch.empty(need, dtype=torch.uint8, device=device)
-        q.workspace, q.workspace_bytes = work.data_ptr(), need
-    elif need < 0:
-        capi.check(need)
-    capi.check(lib.b200rwkv_op_adapters(device.index, torch.cuda.current_stream(device).cuda_stream, C.byref(q)))
+    q = capi.Adapters(_ADAPTERS_BYTES, _TYPE.get(dtype, -1), _TYPE.get(o_dtype, -1), tokens, adapters, n, _list(index, "index", _I32, device, tokens),
+                      _list(scale, "scale", _F32, device, adapters), parts, None if work is None else work.data_ptr(), need)
+    capi.check(lib.b200rwkv_op_adapters(where, _stream(where), C.byref(q)))
     return out if many else out[0]
 
 
@@ -119,38 +112,39 @@ def logits(rows, kind="probs", controls=None, history=None, history_offset=None,
     over those places.  bias_offset, bias_token, bias_value: ragged lists of additions, of which a token's last counts.  allow [masks, (vocab + 31) // 32]
     int32 words: bit t % 32 of word t // 32 of mask allow_row[i] (None: i; no such mask: everything) says whether row i may hold token t.
     `out` may be `rows` itself where they are f32."""
-    if rows.dim() != 2 or rows.device.type != "cuda":
+    device, dtype = rows.device, rows.dtype
+    if rows.dim() != 2 or device.type != "cuda":
         _bad("logits: rows must be a [rows, vocab] tensor in GPU memory")
-    device = rows.device
     n, vocab = rows.shape
     if out is None:
-        out = torch.empty(n, vocab, dtype=torch.float32, device=device)
-    q = capi.Logits()
-    q.struct_bytes = C.sizeof(capi.Logits)
-    q.type, q.kind = _TYPE.get(rows.dtype, -1), _KIND.get(kind, -1)
-    q.rows, q.vocab = n, vocab
-    q.logits, q.logits_stride = _rows(rows, "rows", n, vocab, rows.dtype, device)
-    q.out, q.out_stride = _rows(out, "out", n, vocab, torch.float32, device)
+        out = torch.empty(n, vocab, dtype=_F32, device=device)
+    c = ho = h = hf = al = ar = bo = bt = bv = None
+    masks = 0
     if controls is not None:
-        q.controls = _check_list(controls, "controls", torch.float32, device, n * 5)
+        c = _list(controls, "controls", _F32, device, n * 5)
     if history_offset is not None or history is not None:
         if history is None or history_offset is None:
             _bad("logits: history and history_offset come together")
-        q.history_offset = _check_list(history_offset, "history_offset", torch.int32, device, n + 1)
-        # (a tensor without elements has no address: no history at all)
-        q.history = _check_list(history, "history", torch.int32, device) or q.history_offset
-        q.history_from = _check_list(history_from, "history_from", torch.int32, device, n)
+        ho = _list(history_offset, "history_offset", _I32, device, n + 1)
+        h = _list(history, "history", _I32, device, None) or ho            # (a tensor without elements has no address)
+        if history_from is not None:
+            hf = _list(history_from, "history_from", _I32, device, n)
     if allow is not None:
         words = (vocab + 31) // 32
         if allow.dim() != 2 or allow.shape[1] != words:
             _bad(f"allow must be [masks, {words}]")
-        q.allow, q.allow_rows = _check_list(allow, "allow", torch.int32, device), allow.shape[0]
-        q.allow_row = _check_list(allow_row, "allow_row", torch.int32, device, n)
+        masks = allow.shape[0]
+        al = _list(allow, "allow", _I32, device, None)
+        if allow_row is not None:
+            ar = _list(allow_row, "allow_row", _I32, device, n)
     if bias_offset is not None or bias_token is not None:
         if bias_offset is None or bias_token is None or bias_value is None or bias_token.numel() != bias_value.numel():
             _bad("logits: bias_offset, bias_token and bias_value come together, a value for each token")
-        q.bias_offset = _check_list(bias_offset, "bias_offset", torch.int32, device, n + 1)
-        q.bias_token = _check_list(bias_token, "bias_token", torch.int32, device) or q.bias_offset
-        q.bias_value = _check_list(bias_value, "bias_value", torch.float32, device) or q.bias_offset
-    capi.check(capi.lib().b200rwkv_op_logits(device.index, torch.cuda.current_stream(device).cuda_stream, C.byref(q)))
+        bo = _list(bias_offset, "bias_offset", _I32, device, n + 1)
+        bt = _list(bias_token, "bias_token", _I32, device, None) or bo
+        bv = _list(bias_value, "bias_value", _F32, device, None) or bo
+    where = device.index
+    q = capi.Logits(_LOGITS_BYTES, _TYPE.get(dtype, -1), _KIND.get(kind, -1), n, vocab, masks, rows.data_ptr(), _row_stride(rows, "rows", n, vocab, dtype, device),
+                    out.data_ptr(), _row_stride(out, "out", n, vocab, _F32, device), c, ho, h, hf, al, ar, bo, bt, bv)
+    capi.check(capi.lib().b200rwkv_op_logits(where, _stream(where), C.byref(q)))
     return out

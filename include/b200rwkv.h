@@ -329,6 +329,7 @@ int32_t b200rwkv_op_wkv(int32_t device, int32_t version, int32_t T, int32_t H, c
 #define B200RWKV_MAX_PARTS 8
 #define B200RWKV_MAX_RANK 256
 #define B200RWKV_MAX_ADAPTERS 1024
+#define B200RWKV_ADAPTERS_WITHOUT_WORKSPACE 256     /* tokens of a call that needs none */
 typedef struct {
     const void* x;               /* [tokens, in] of `type`; rows x_stride elements apart (a multiple of 8) */
     int64_t x_stride;

@@ -114,6 +114,7 @@ def test_structs_match_the_header(tmp_path):
     for name, value in [("MAX_PARTS", capi.MAX_PARTS), ("MAX_RANK", capi.MAX_RANK), ("MAX_ADAPTERS", capi.MAX_ADAPTERS), ("TYPE_F32", capi.TYPE_F32), ("TYPE_F16", capi.TYPE_F16),
                         ("TYPE_BF16", capi.TYPE_BF16), ("LOGITS", capi.LOGITS), ("PROBS", capi.PROBS), ("LOG_PROBS", capi.LOG_PROBS)]:
         assert f"#define B200RWKV_{name} {value}\n" in header, name
+    assert f"#define B200RWKV_ADAPTERS_WITHOUT_WORKSPACE {capi.ADAPTERS_WITHOUT_WORKSPACE} " in header
 
 
 def test_engine_calls_refuse_null():
