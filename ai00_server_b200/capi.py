@@ -51,8 +51,7 @@ class AdapterPart(C.Structure):
 class Adapters(C.Structure):
     """b200rwkv_adapters."""
     _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("out_type", C.c_int32), ("tokens", C.c_int32), ("adapters", C.c_int32),
-                ("num_parts", C.c_int32), ("index", C.c_void_p), ("scale", C.c_void_p), ("parts", C.POINTER(AdapterPart)), ("workspace", C.c_void_p),
-                ("workspace_bytes", C.c_size_t)]
+                ("num_parts", C.c_int32), ("index", C.c_void_p), ("scale", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class Logits(C.Structure):
@@ -129,8 +128,8 @@ SYMBOLS = [
     ("b200rwkv_op_quantize", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P, _P]),
     ("b200rwkv_op_wkv", C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32] + [_P] * 14),
     ("b200rwkv_op_adapters_workspace", C.c_int64, [C.c_int32] * 4),
-    ("b200rwkv_op_adapters", C.c_int32, [C.c_int32, _P, C.POINTER(Adapters)]),
-    ("b200rwkv_op_logits", C.c_int32, [C.c_int32, _P, C.POINTER(Logits)]),
+    ("b200rwkv_op_adapters", C.c_int32, [C.c_int32, _P, _P, _P]),
+    ("b200rwkv_op_logits", C.c_int32, [C.c_int32, _P, _P]),
     ("b200rwkv_launch_count", C.c_int32, [_P, C.POINTER(C.c_int64)]),
     ("b200rwkv_keep_hidden", C.c_int32, [_P, C.c_int32]),
     ("b200rwkv_last_hidden", C.c_int32, [_P, _P, C.c_size_t]),

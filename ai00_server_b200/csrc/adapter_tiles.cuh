@@ -124,6 +124,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
     bool fine = true;

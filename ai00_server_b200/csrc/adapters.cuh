@@ -495,7 +495,10 @@ inline size_t adapter_few_smem(int R, int elem_parts) {
 // the atomics, its result does not: columns and rows of a product do not see each other, and a token goes alone only where its adapter has no other
 // (the one left over from groups of eight could be any).
 __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __grid_constant__ AdapterParams p) {
+    constexpr int KEPT = 8192;                   // tokens whose bins are kept between the two passes
     __shared__ int s_count[ADP_MAX_ADAPTERS + 1], s_first[ADP_MAX_ADAPTERS + 1], s_warp[3][ADP_PLAN_THREADS / 32], s_total[3];
+    __shared__ short s_bin[KEPT];
+    pdl_launch_dependents();                     // (they wait for this kernel's end before they read anything)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = p.adapters + (p.copy ? 1 : 0);
     for (int i = tid; i < bins; i += ADP_PLAN_THREADS) s_count[i] = 0;
     if (tid < 3) s_total[tid] = 0;
@@ -509,6 +512,7 @@ __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __
         const int b = t0 + tid < p.tokens ? bin_of(t0 + tid) : -1;
         const unsigned same = __match_any_sync(0xffffffffu, b);
         if (b >= 0 && lane == __ffs(same) - 1) atomicAdd(&s_count[b], __popc(same));
+        if (t0 + tid < KEPT) s_bin[t0 + tid] = (short)b;
     }
     __syncthreads();
     // exclusive sums over the bins of tokens, groups and tiles, ADP_PLAN_THREADS bins at a time
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(ADP_PLAN_THREADS) adapter_plan_kernel(const __
         p.plan.count()[1] = s_total[2];
     }
     for (int t0 = 0; t0 < p.tokens; t0 += ADP_PLAN_THREADS) {
-        const int b = t0 + tid < p.tokens ? bin_of(t0 + tid) : -1;
+        const int b = t0 + tid >= p.tokens ? -1 : (t0 + tid < KEPT ? s_bin[t0 + tid] : bin_of(t0 + tid));
         const unsigned same = __match_any_sync(0xffffffffu, b);
         int at = 0;
         const int leader = __ffs(same) - 1;

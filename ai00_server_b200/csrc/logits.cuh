@@ -7,7 +7,8 @@
 // softmax run.rs:1179; the samplers that need whole rows are sampler/mirostat.rs:44-90 and sampler/typical.rs:70-131.
 //
 // Bound: a row is read and written once, 8 bytes a token for f32 rows (row of 65536: 0.5 MB; 512 rows 41 us at the copy rate); one row is latency.
-// Shape: a cluster of eight or sixteen CTAs a row, the row in their registers (16 to 64 tokens a thread) between the only read and the only write.
+// Shape: a cluster of eight or sixteen CTAs a row, the row in their registers (16 to 64 tokens a thread) between the only read and the only write; 32 tokens a
+// thread and CTAs of 256 where there are many rows (512 rows of 65536: 57 us, with 16 tokens and CTAs of 512 70), which settle their sums more quickly.
 // Tokens go to the CTAs in stripes of 64, so that frequent tokens that are neighbours in a vocabulary spread over all of them.
 //   * a history is added up in shared memory, a pair of words for each token of the CTA: decay^age in units of 2^-28, its lower 14 bits to one word
 //     and the others to the other, so that neither overflows (2^17 - 1 entries; of a longer history the newest count), no atomic has to answer,
@@ -40,6 +41,13 @@ __device__ __forceinline__ float4 logits4(const __nv_bfloat16* p) {
 
 constexpr unsigned LOGITS_SEEN = 1u << 31;        // flag in the upper word of a token that is in the history and does not count there
 
+// e^x as a power of two: a multiplication and the unit's instruction, good to 2^-22 and to the rounding of its argument.  (expf is eight instructions)
+__device__ __forceinline__ float logits_exp(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 // sum of exponentials relative to a maximum.  NaN never becomes the maximum: it stays in the sum, and through it reaches the whole row
 struct LogitsSum {
     float m, s;
@@ -50,6 +58,7 @@ struct LogitsSum {
         }
     }
 };
+template <int TH>
 __device__ __forceinline__ LogitsSum logits_block(LogitsSum a, LogitsSum* red) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto whole = [](LogitsSum x) {
@@ -60,41 +69,52 @@ __device__ __forceinline__ LogitsSum logits_block(LogitsSum a, LogitsSum* red) {
     a = whole(a);
     if (lane == 0) red[warp] = a;
     __syncthreads();
-    return whole(lane < LOGITS_THREADS / 32 ? red[lane] : LogitsSum{-INFINITY, 0.f});
+    return whole(lane < TH / 32 ? red[lane] : LogitsSum{-INFINITY, 0.f});
 }
 
-// NV: fours of tokens a thread holds.  VEC: a thread's fours are neighbours and rows allow accesses of four; else its tokens are LOGITS_THREADS apart
-template <typename E, int NV, bool VEC>
-__global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1)) logits_kernel(const __grid_constant__ LogitsParams p) {
+// TH: threads of a CTA, each with NV fours of tokens.  VEC: fours are neighbours, moved in one access; a row may start anywhere if it does so in both buffers
+// alike: its fours then start up to three tokens in front of it.  Else a thread's tokens are TH apart
+template <typename E, int TH, int NV, bool VEC>
+__global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) / TH) logits_kernel(const __grid_constant__ LogitsParams p) {
     extern __shared__ __align__(16) uint2 sums[];
-    __shared__ LogitsSum red[LOGITS_THREADS / 32];
+    __shared__ LogitsSum red[TH / 32];
     __shared__ float2 stats[LOGITS_MOST_CTAS];
-    constexpr int TH = LOGITS_THREADS;
     const int tid = threadIdx.x, lg_ctas = p.ctas_log, ctas = 1 << lg_ctas, cta = blockIdx.x & (ctas - 1), row = blockIdx.x >> lg_ctas;
     const bool softmax = p.kind != LOGITS_ROWS;
     // no CTA writes to another's memory before all have started
     if (softmax) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     pdl_wait();
-    // the CTA's tokens by place: stripes cta, cta + ctas, ...; only the vocabulary's last stripe can be short
-    const int stripes = (p.V + LOGITS_STRIPE - 1) / LOGITS_STRIPE, own = (stripes - cta + ctas - 1) >> lg_ctas;
-    int n = max(own, 0) * LOGITS_STRIPE;
-    if (own > 0 && (((own - 1) << lg_ctas) | cta) == stripes - 1) n -= stripes * LOGITS_STRIPE - p.V;
-    auto token = [&](int i) { return (((i / LOGITS_STRIPE) << lg_ctas) | cta) * LOGITS_STRIPE + i % LOGITS_STRIPE; };
-    auto place = [&](int k, int c) { return VEC ? (k * TH + tid) * 4 + c : (k * 4 + c) * TH + tid; };       // of the thread's c-th token in its k-th four
     const E* const in = reinterpret_cast<const E*>(p.in) + (size_t)(p.in_row ? p.in_row[row] : row) * p.in_stride;
     float* const out = p.out + (size_t)row * p.out_stride;
+    // The CTA's tokens by place: stripes cta, cta + ctas, ... of the row with `ahead` places in front, so that fours lie on boundaries
+    const int V = p.V, ahead = VEC ? (int)((uintptr_t)out / 4 & 3) : 0;
+    const int stripes = (V + ahead + LOGITS_STRIPE - 1) / LOGITS_STRIPE, places = max((stripes - cta + ctas - 1) >> lg_ctas, 0) * LOGITS_STRIPE;
+    // of the thread's c-th token in its k-th four: place, and the token itself (places are a whole number of stripes apart, so tokens are an even step apart)
+    auto place = [&](int k, int c) { return VEC ? (k * TH + tid) * 4 + c : (k * 4 + c) * TH + tid; };
+    constexpr int PER = VEC ? 4 : 1;
+    int t_first = (((tid * PER / LOGITS_STRIPE) << lg_ctas) | cta) * LOGITS_STRIPE + tid * PER % LOGITS_STRIPE - ahead;
+    const int t_step = ((TH * PER / LOGITS_STRIPE) << lg_ctas) * LOGITS_STRIPE;
+    auto token = [&](int k, int c) { return VEC ? t_first + k * t_step + c : t_first + (k * 4 + c) * t_step; };
+    // (worked out again in every part below: kept over all of them, tokens and what is known of them take more registers than the row)
+    auto again = [&] { asm volatile("" : "+r"(t_first)); };
+    auto there = [&](int t) { return t >= 0 && t < V; };
+    auto whole = [&](int t) { return VEC && t >= 0 && t + 3 < V; };
     float v[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int i = place(k, 0);
-        if (VEC && i + 3 < n) {
-            const float4 x = logits4(in + token(i));
+        const int t = token(k, 0);
+        if (whole(t)) {
+            const float4 x = logits4(in + t);
             v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
         } else {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[k][c] = place(k, c) < n ? logit_of<E>(in[token(place(k, c))]) : -INFINITY;
+            for (int c = 0; c < 4; ++c) {
+                const int u = token(k, c);
+                v[k][c] = there(u) ? logit_of<E>(in[u]) : -INFINITY;
+            }
         }
     }
+    again();
     const float* const ctl = p.controls ? p.controls + (size_t)row * 5 : nullptr;
     const int h0 = p.hist_off ? p.hist_off[row] : 0, hn = p.hist_off ? p.hist_off[row + 1] - h0 : 0;
     const int b0 = p.bias_off ? p.bias_off[row] : 0, bn = p.bias_off ? p.bias_off[row + 1] - b0 : 0;
@@ -110,9 +130,9 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
                 for (int u = 0; u < U; ++u) t[u] = j0 + u * TH < count ? (unsigned)tok[j0 + u * TH] : 0xFFFFFFFFu;
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const unsigned st = t[u] / LOGITS_STRIPE;
-                    const int i = (int)((st >> lg_ctas) * LOGITS_STRIPE + t[u] % LOGITS_STRIPE) - s0;
-                    if (t[u] < (unsigned)p.V && (int)(st & (ctas - 1)) == cta && i >= 0 && i < p.list_tokens) f(j0 + u * TH, i);
+                    const unsigned at = t[u] + (unsigned)ahead, st = at / LOGITS_STRIPE;
+                    const int i = (int)((st >> lg_ctas) * LOGITS_STRIPE + at % LOGITS_STRIPE) - s0;
+                    if (t[u] < (unsigned)V && (int)(st & (ctas - 1)) == cta && i >= 0 && i < p.list_tokens) f(j0 + u * TH, i);
                 }
             }
         };
@@ -143,7 +163,7 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
         };
         // (what is not zero after `apply` is zeroed there: the sums start at zero every time)
         for (int i = tid * 2; i < p.list_tokens; i += TH * 2) *reinterpret_cast<uint4*>(sums + i) = make_uint4(0, 0, 0, 0);
-        for (int s0 = 0; s0 < n; s0 += p.list_tokens) {
+        for (int s0 = 0; s0 < places; s0 += p.list_tokens) {
             if (hn > 0) {
                 const float rep = ctl ? ctl[0] : 1.f, presence = ctl ? ctl[1] : 0.f, frequency = ctl ? ctl[2] : 0.f;
                 const float lg = log2f(fminf(fmaxf(ctl ? ctl[3] : 1.f, 0.f), 1.f));
@@ -180,6 +200,7 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
     }
 
     // ---- mask and temperature ----
+    again();
     const float temperature = ctl ? ctl[4] : 1.f;
     // a temperature that is not a positive number makes the row NaN
     const float scale = temperature > 0.f && temperature < INFINITY ? 1.f / temperature : __int_as_float(0x7fc00000);
@@ -190,8 +211,13 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
             unsigned w[NV];
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                const int t = token(place(k, 0));
-                w[k] = place(k, 0) < n ? allow[t / 32] >> (t % 32) : 0u;        // four tokens of a word: t is a multiple of 4
+                const int t = token(k, 0);
+                w[k] = 0u;
+                if (t <= -4 || t >= V) continue;
+                // four tokens from t on: of one word, or of two
+                const int q = t >> 5;
+                const unsigned lo = q >= 0 ? allow[q] : 0u, hi = (t & 31) > 28 && q + 1 < p.words ? allow[q + 1] : 0u;
+                w[k] = __funnelshift_r(lo, hi, t & 31);
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k)
@@ -203,23 +229,29 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
             for (int k = 0; k < NV; ++k) {
                 unsigned w[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) w[c] = place(k, c) < n ? allow[token(place(k, c)) / 32] : 0u;
+                for (int c = 0; c < 4; ++c) {
+                    const int t = token(k, c);
+                    w[c] = there(t) ? allow[t / 32] >> (t % 32) : 0u;
+                }
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    if (!((w[c] >> (place(k, c) % 32)) & 1u)) v[k][c] = -INFINITY;       // (places and tokens agree modulo 32)
+                    if (!(w[c] & 1u)) v[k][c] = -INFINITY;
             }
         }
     }
     auto put = [&](auto&& last) {
+        again();
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int i = place(k, 0);
-            if (VEC && i + 3 < n) {
-                *reinterpret_cast<float4*>(out + token(i)) = make_float4(last(v[k][0]), last(v[k][1]), last(v[k][2]), last(v[k][3]));
+            const int t = token(k, 0);
+            if (whole(t)) {
+                *reinterpret_cast<float4*>(out + t) = make_float4(last(v[k][0]), last(v[k][1]), last(v[k][2]), last(v[k][3]));
             } else {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (place(k, c) < n) out[token(place(k, c))] = last(v[k][c]);
+                for (int c = 0; c < 4; ++c) {
+                    const int u = token(k, c);
+                    if (there(u)) out[u] = last(v[k][c]);
+                }
             }
         }
     };
@@ -229,13 +261,14 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
     }
 
     // ---- the thread's maximum and sum; from here on a probability is its exponential ----
+    again();
     const bool probs = p.kind == LOGITS_PROBS;
     LogitsSum sum{-INFINITY, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            if (place(k, c) < n) v[k][c] *= scale;       // (what is behind the last token stays -inf under every scale)
+            if (there(token(k, c))) v[k][c] *= scale;       // (what is not of the row stays -inf under every scale)
             sum.m = fmaxf(sum.m, v[k][c]);
         }
     const float mine = sum.m, shift = mine == -INFINITY ? 0.f : mine;
@@ -243,13 +276,13 @@ __global__ void __launch_bounds__(LOGITS_THREADS, NV <= 4 ? 3 : (NV <= 8 ? 2 : 1
     for (int k = 0; k < NV; ++k)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            const float e = expf(v[k][c] - shift);
+            const float e = logits_exp(v[k][c] - shift);
             sum.s += e;
             if (probs) v[k][c] = e;
         }
 
     // ---- the CTAs' statistics, in their order ----
-    sum = logits_block(sum, red);
+    sum = logits_block<TH>(sum, red);
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (tid < ctas) {
         uint32_t remote;

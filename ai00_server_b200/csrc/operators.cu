@@ -141,32 +141,47 @@ void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_ty
     with_types(type, out_type, [&](auto e, auto o) { apply<decltype(e), decltype(o)>(s, p); });
 }
 
-template <typename E, int NV, bool VEC>
+template <typename E, int TH, int NV, bool VEC>
 static void logits_launch(cudaStream_t s, const LogitsParams& p, int rows) {
-    constexpr size_t most = (size_t)std::min(LOGITS_LIST_TOKENS, LOGITS_THREADS * NV * 4) * sizeof(uint2);
-    prepare<logits_kernel<E, NV, VEC>>(most, true);
-    launch(logits_kernel<E, NV, VEC>, dim3(rows << p.ctas_log), LOGITS_THREADS, (size_t)p.list_tokens * sizeof(uint2), s, p, 1 << p.ctas_log);
+    constexpr size_t most = (size_t)std::min(LOGITS_LIST_TOKENS, TH * NV * 4) * sizeof(uint2);
+    prepare<logits_kernel<E, TH, NV, VEC>>(most, true);
+    launch(logits_kernel<E, TH, NV, VEC>, dim3(rows << p.ctas_log), TH, (size_t)p.list_tokens * sizeof(uint2), s, p, 1 << p.ctas_log);
 }
 
 void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type) {
-    const int size = type == B200RWKV_TYPE_F32 ? 4 : 2, stripes = (p.V + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
-    p.vec = (uintptr_t)p.in % (4 * size) == 0 && p.in_stride % 4 == 0 && (uintptr_t)p.out % 16 == 0 && p.out_stride % 4 == 0;
-    // sixteen CTAs where eight would hold more than 16 tokens a thread, and for few rows, which are latency
-    p.ctas_log = p.V > 8 * LOGITS_THREADS * 16 || rows <= 9 ? 4 : 3;
-    const int tokens = ((stripes - 1) >> p.ctas_log) * LOGITS_STRIPE + LOGITS_STRIPE, each = LOGITS_THREADS * 4;
-    p.list_tokens = p.hist_off || p.bias_off ? std::min(tokens, LOGITS_LIST_TOKENS) : 0;
-    auto go = [&](auto nv) {
-        auto typed = [&](auto e) {
-            if (p.vec) logits_launch<decltype(e), decltype(nv)::value, true>(s, p, rows);
-            else logits_launch<decltype(e), decltype(nv)::value, false>(s, p, rows);
+    const int size = type == B200RWKV_TYPE_F32 ? 4 : 2;
+    // fours that lie on boundaries in both buffers: rows start alike, modulo four (rows that are picked: on boundaries)
+    const bool whole = p.in_stride % 4 == 0 && p.out_stride % 4 == 0;
+    p.vec = (uintptr_t)p.in % (4 * size) == 0 && (uintptr_t)p.out % 16 == 0 && (whole || (!p.in_row && p.in_stride % 4 == p.out_stride % 4));
+    const int stripes = (p.V + (whole ? 0 : 3) + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
+    auto tokens_of = [&](int lg) { return ((stripes - 1) >> lg) * LOGITS_STRIPE + LOGITS_STRIPE; };
+    // up to 16 tokens a thread and CTAs of 512 while all rows find room at once; 32 tokens a thread beyond, sixteen CTAs and 64 tokens for the widest rows
+    const int sms = sm_count();
+    int threads = 512, nv = 4;
+    p.ctas_log = rows * 16 <= sms ? 4 : 3;
+    if (rows * 8 > sms && tokens_of(3) <= 256 * 32) threads = 256, nv = tokens_of(3) <= 256 * 16 ? 4 : 8;
+    else if (tokens_of(p.ctas_log) > 512 * 16) {
+        nv = 8;
+        if (tokens_of(3) > 512 * 32) p.ctas_log = 4;
+        if (tokens_of(4) > 512 * 32) nv = 16;
+    }
+    p.list_tokens = p.hist_off || p.bias_off ? std::min(tokens_of(p.ctas_log), LOGITS_LIST_TOKENS) : 0;
+    auto typed = [&](auto e) {
+        using E = decltype(e);
+        auto form = [&](auto th, auto n) {
+            constexpr int TH = decltype(th)::value, NV = decltype(n)::value;
+            p.vec ? logits_launch<E, TH, NV, true>(s, p, rows) : logits_launch<E, TH, NV, false>(s, p, rows);
         };
-        if (type == B200RWKV_TYPE_F32) typed(float{});
-        else if (type == B200RWKV_TYPE_F16) typed(__half{});
-        else typed(__nv_bfloat16{});
+        using std::integral_constant;
+        if (threads == 256 && nv == 4) form(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+        else if (threads == 256) form(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+        else if (nv == 4) form(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+        else if (nv == 8) form(integral_constant<int, 512>{}, integral_constant<int, 8>{});
+        else form(integral_constant<int, 512>{}, integral_constant<int, 16>{});
     };
-    if (tokens <= 4 * each) go(std::integral_constant<int, 4>{});
-    else if (tokens <= 8 * each) go(std::integral_constant<int, 8>{});
-    else go(std::integral_constant<int, 16>{});
+    if (type == B200RWKV_TYPE_F32) typed(float{});
+    else if (type == B200RWKV_TYPE_F16) typed(__half{});
+    else typed(__nv_bfloat16{});
 }
 
 // the calling thread's device for the length of a call
@@ -196,7 +211,7 @@ int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters, int32_t
     return (int64_t)adapters_workspace(tokens, adapters, num_parts, rank);
 }
 
-int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* q) {
+int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* q, const b200rwkv_adapter_part* parts) {
     API_BEGIN((b200rwkv_engine*)nullptr)
     static_assert(B200RWKV_MAX_PARTS == ADP_MAX_PARTS && B200RWKV_MAX_RANK == ADP_MAX_RANK && B200RWKV_MAX_ADAPTERS == ADP_MAX_ADAPTERS &&
                       B200RWKV_ADAPTERS_WITHOUT_WORKSPACE == ADP_INLINE, "limits");
@@ -205,7 +220,7 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
     REQUIRE(q->out_type == q->type || q->out_type == B200RWKV_TYPE_F32, B200RWKV_ERR_UNSUPPORTED, "op_adapters: out is f32 or of the type of x");
     REQUIRE(q->tokens >= 0 && q->tokens <= (1 << 20), B200RWKV_ERR_INVALID, "op_adapters: tokens must be in [0, 2^20]");
     REQUIRE(q->adapters >= 1 && q->adapters <= B200RWKV_MAX_ADAPTERS, B200RWKV_ERR_INVALID, "op_adapters: adapters must be in [1, 1024]");
-    REQUIRE(q->num_parts >= 1 && q->num_parts <= B200RWKV_MAX_PARTS && q->parts, B200RWKV_ERR_INVALID, "op_adapters: num_parts must be in [1, 8]");
+    REQUIRE(q->num_parts >= 1 && q->num_parts <= B200RWKV_MAX_PARTS && parts, B200RWKV_ERR_INVALID, "op_adapters: num_parts must be in [1, 8]");
     REQUIRE(q->tokens == 0 || (q->index && q->scale), B200RWKV_ERR_INVALID, "op_adapters: null index or scale");
     AdapterParams p;
     memset(&p, 0, sizeof(p));
@@ -215,7 +230,7 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
     p.scale = q->scale;
     const int osize = q->out_type == B200RWKV_TYPE_F32 ? 4 : 2;
     for (int i = 0; i < q->num_parts; ++i) {
-        const b200rwkv_adapter_part& s = q->parts[i];
+        const b200rwkv_adapter_part& s = parts[i];
         AdapterPart& d = p.part[i];
         REQUIRE(s.in_features >= 8 && s.in_features % 8 == 0 && s.in_features <= (1 << 24), B200RWKV_ERR_UNSUPPORTED, "op_adapters: in_features must be a multiple of 8");
         REQUIRE(s.out_features >= 1 && s.out_features <= (1 << 24), B200RWKV_ERR_INVALID, "op_adapters: out_features must be positive");

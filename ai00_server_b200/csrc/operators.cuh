@@ -81,12 +81,11 @@ B200_HIDDEN void adapters_plan(cudaStream_t s, const AdapterParams& p);
 B200_HIDDEN void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type);
 
 // ---- rows of logits ----
-constexpr int LOGITS_THREADS = 512;
 constexpr int LOGITS_STRIPE = 64;                // neighbouring tokens of a CTA; the next ones are the next CTA's
 constexpr int LOGITS_MOST_CTAS = 16;             // CTAs of a row
 constexpr int LOGITS_LIST_TOKENS = 16384;        // tokens of a CTA whose sums lie in shared memory at once
 constexpr int LOGITS_MAX_HISTORY = (1 << 17) - 1;
-constexpr int LOGITS_MAX_VOCAB = LOGITS_MOST_CTAS * LOGITS_THREADS * 64;
+constexpr int LOGITS_MAX_VOCAB = 1 << 19;
 enum LogitsKind : int { LOGITS_ROWS = 0, LOGITS_PROBS = 1, LOGITS_LOGPROBS = 2 };
 
 struct LogitsParams {
@@ -96,7 +95,7 @@ struct LogitsParams {
     long long out_stride;
     int V;
     int kind;
-    int vec;                     // rows start on 16-byte boundaries (in and out)
+    int vec;                     // fours of a row of `out` on a boundary lie on one in `in`
     int ctas_log;                // log2 of the CTAs of a row
     int list_tokens;             // tokens of a CTA whose sums lie in shared memory at once (0: no lists)
     const int* in_row;           // row of `in` of each output row (null: the same)

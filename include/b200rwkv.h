@@ -353,13 +353,13 @@ typedef struct {
     int32_t num_parts;           /* 1 .. B200RWKV_MAX_PARTS */
     const int32_t* index;        /* [tokens] */
     const float* scale;          /* [adapters] */
-    const b200rwkv_adapter_part* parts;      /* host array */
     void* workspace;             /* b200rwkv_op_adapters_workspace bytes, 16-byte aligned; contents before and after do not matter */
     size_t workspace_bytes;
 } b200rwkv_adapters;
 /* rank: the largest of the parts.  0: none is needed; negative: a status */
 int64_t b200rwkv_op_adapters_workspace(int32_t tokens, int32_t adapters, int32_t num_parts, int32_t rank);
-int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* args);
+/* parts: host array of args->num_parts */
+int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapters* args, const b200rwkv_adapter_part* parts);
 
 /* Rows of logits adjusted for their requests, as logits, probabilities or log-probabilities.  For row i, token t, with the row's
  * controls (repetition, presence, frequency, decay, temperature; 1, 0, 0, 1, 1 without them) and its history h_0 .. h_{n-1}, oldest first:

@@ -10,10 +10,9 @@ def _adapters(**change):
     part = capi.AdapterPart(x=4096, x_stride=64, a=4096, b=4096, base=4096, base_stride=32, out=8192, out_stride=32, in_features=64, out_features=32, rank=16)
     q = capi.Adapters(struct_bytes=C.sizeof(capi.Adapters), type=capi.TYPE_F16, out_type=capi.TYPE_F32, tokens=4, adapters=2, num_parts=1, index=4096, scale=4096)
     for k, v in change.items():
-        setattr(part if hasattr(part, k) else q, k, v)
-    q.parts = (capi.AdapterPart * 1)(part) if change.get("parts", 1) else None
-    q._keep = q.parts
-    return q
+        if k != "parts":
+            setattr(part if hasattr(part, k) else q, k, v)
+    return C.byref(q), (C.byref(part) if change.get("parts", 1) else None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -30,16 +29,15 @@ def _adapters(**change):
     ({"tokens": 300, "workspace": 4096, "workspace_bytes": 64}, capi.ERR_INVALID),
     ({"tokens": 300, "workspace": 4100, "workspace_bytes": 1 << 20}, capi.ERR_INVALID)])
 def test_op_adapters_refuses(change, code):
-    q = _adapters(**change)
     with pytest.raises(capi.B200Error) as ei:
-        capi.check(capi.lib().b200rwkv_op_adapters(0, None, C.byref(q)))
+        capi.check(capi.lib().b200rwkv_op_adapters(0, None, *_adapters(**change)))
     assert ei.value.code == code
     assert "op_adapters" in str(ei.value)
 
 
 def test_op_adapters_null_struct_and_no_tokens():
-    assert capi.lib().b200rwkv_op_adapters(0, None, None) == capi.ERR_INVALID
-    assert capi.lib().b200rwkv_op_adapters(0, None, C.byref(_adapters(tokens=0, index=None, scale=None, x=None, out=None))) == 0
+    assert capi.lib().b200rwkv_op_adapters(0, None, None, None) == capi.ERR_INVALID
+    assert capi.lib().b200rwkv_op_adapters(0, None, *_adapters(tokens=0, index=None, scale=None, x=None, out=None)) == 0
 
 
 def test_op_adapters_workspace():
@@ -114,6 +112,8 @@ def test_structs_match_the_header(tmp_path):
     for name, value in [("MAX_PARTS", capi.MAX_PARTS), ("MAX_RANK", capi.MAX_RANK), ("MAX_ADAPTERS", capi.MAX_ADAPTERS), ("TYPE_F32", capi.TYPE_F32), ("TYPE_F16", capi.TYPE_F16),
                         ("TYPE_BF16", capi.TYPE_BF16), ("LOGITS", capi.LOGITS), ("PROBS", capi.PROBS), ("LOG_PROBS", capi.LOG_PROBS)]:
         assert f"#define B200RWKV_{name} {value}\n" in header, name
+    from ai00_server_b200 import device_ops
+    assert (device_ops._PART.size, device_ops._ADAPTERS.size, device_ops._LOGITS.size) == tuple(C.sizeof(c) for c in (capi.AdapterPart, capi.Adapters, capi.Logits))
     assert f"#define B200RWKV_ADAPTERS_WITHOUT_WORKSPACE {capi.ADAPTERS_WITHOUT_WORKSPACE} " in header
 
 
