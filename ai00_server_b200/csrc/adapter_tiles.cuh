@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
     __shared__ __align__(8) uint64_t s_bar[2];
     __shared__ uint32_t s_tmem;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int L = p.rank, TT = p.out_tokens, subs = ADT_TOK / TT;
+    const int L = p.rank, TT = p.out_tokens;
     const uint32_t oper = (smem_u32(smem_any) + 1023u) & ~1023u, wts = oper + adt_operand(L, NP);
     float* const rows = reinterpret_cast<float*>(smem_any + (wts + adt_weights(L) - smem_u32(smem_any)));
     const uint32_t bar = smem_u32(s_bar);
@@ -277,30 +277,33 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
     tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&s_tmem);
     const int tiles = p.plan.count()[1];
+    const size_t low_bytes = adt_low_bytes(p.tokens, L, NP);
     for (int i = tid; i < min(tiles, ADT_TABLE); i += ADT_THREADS) s_tiles[i] = p.plan.tile()[i];
     __syncthreads();
 
     struct Unit {
-        const E* B;
-        const O* base;
+        const E* w;                                  // the unit's rows of B
+        const O* base;                               // its first output of token 0
         O* out;
-        const uint8_t* low;
+        const uint8_t* low;                          // S of its first token
         long long base_stride, out_stride;
-        int cnt, first, N, n0, R;
+        int cnt, first, left, R;                     // left: outputs from its first on
         bool vec;
     };
     // where the CTA is: projection, tile (in pieces of TT tokens), block of outputs
+    const int sub_log = TT == 128 ? 0 : (TT == 64 ? 1 : 2);
     int part = 0, ts = 0, block = blockIdx.x, nb = (p.part[0].N + 127) / 128;
     // the unit there, or the next one of the CTA that has something to do; and on to the one behind it
     auto fetch = [&](Unit& x) {
         while (part < p.nparts) {
-            if (block >= nb) {
-                ts += block / nb;
-                block %= nb;
+            while (block >= nb) {
+                block -= nb;
+                ++ts;
             }
-            if (ts >= tiles * subs) {
+            const int tile = ts >> sub_log;
+            if (tile >= tiles) {
                 // the rest of the way in blocks of the next projection
-                const long long over = (long long)(ts - tiles * subs) * nb + block;
+                const long long over = (long long)(ts - (tiles << sub_log)) * nb + block;
                 if (++part == p.nparts) break;
                 nb = (p.part[part].N + 127) / 128;
                 ts = (int)(over / nb);
@@ -308,43 +311,51 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
                 continue;
             }
             const AdapterPart& q = p.part[part];
-            const int tile = ts / subs, sub = ts % subs, n0 = block * 128;
+            const int n0 = block * 128, skip = (ts - (tile << sub_log)) * TT;
             block += gridDim.x;
             const int4 gr = tile < ADT_TABLE ? s_tiles[tile] : p.plan.tile()[tile];
-            x.cnt = min(TT, gr.z - sub * TT);
+            x.cnt = min(TT, gr.z - skip);
             if (x.cnt <= 0) continue;
             const AdtWeights<E> ad(p, q, gr.x);
             if (ad.R == 0 && (!p.copy || (q.base == q.out && q.base_stride == q.out_stride))) continue;
-            x.B = ad.B; x.R = ad.R;
-            x.base = reinterpret_cast<const O*>(q.base); x.out = reinterpret_cast<O*>(q.out);
+            x.R = ad.R;
+            x.w = ad.B + (size_t)n0 * ad.R;
+            x.base = q.base ? reinterpret_cast<const O*>(q.base) + n0 : nullptr;
+            x.out = reinterpret_cast<O*>(q.out) + n0;
             x.base_stride = q.base_stride; x.out_stride = q.out_stride;
-            x.low = p.low + (size_t)part * adt_low_bytes(p.tokens, L, NP);
-            x.first = gr.y + sub * TT;
-            x.N = q.N; x.n0 = n0;
-            x.vec = q.vec && n0 + 128 <= q.N;
+            x.first = gr.y + skip;
+            x.low = p.low + (size_t)part * low_bytes + (size_t)x.first * 128;
+            x.left = q.N - n0;
+            x.vec = q.vec && x.left >= 128;
             return true;
         }
         return false;
     };
+    const size_t tile_bytes = (size_t)p.tokens * 128;        // of 64 ranks of S
+    // a thread: 16 bytes at one place of every 32nd row
+    const int c16 = tid & 7, r8 = tid >> 3;
+    const uint32_t swz = adt_swizzled(r8, c16);              // (rows 32 apart: 4096 bytes further)
     auto load_operands = [&](const Unit& x) {
-        // a thread: 16 bytes at one place of every 32nd row
-        const int have = min(128, x.N - x.n0), c = tid & 7, r16 = adt_r16(x.R);
+        const int have = min(128, x.left), r16 = adt_r16(x.R);
         for (int r0 = 0; r0 < r16; r0 += 64) {
-            const int rank = r0 + c * 8;
+            const int rank = r0 + c16 * 8;
             if (rank >= r16) continue;
             const bool real = rank < x.R;
-            const E* const w = x.B + (size_t)(x.n0 + (tid >> 3)) * x.R + (real ? rank : 0);
-            const uint32_t to = wts + (r0 >> 6) * (128 * 128);
+            const E* w = x.w + r8 * x.R + (real ? rank : 0);
+            const uint32_t to = wts + (r0 >> 6) * (128 * 128) + swz;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if ((tid >> 3) + i * 32 < have) adt_cp16(to + adt_swizzled((tid >> 3) + i * 32, c), w + (size_t)i * 32 * x.R, real);
+            for (int i = 0; i < 4; ++i) {
+                if (r8 + i * 32 < have) adt_cp16(to + i * 4096, w, real);
+                w += 32 * x.R;
+            }
 #pragma unroll
             for (int k = 0; k < NP; ++k) {
                 const int tile = k * adt_chunks(L) + (r0 >> 6);
-                const uint8_t* const s = x.low + ((size_t)tile * p.tokens + x.first + (tid >> 3)) * 128 + c * 16;
+                const uint8_t* const s = x.low + tile * tile_bytes + r8 * 128 + c16 * 16;
+                const uint32_t at = oper + (uint32_t)tile * (TT * 128) + swz;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if ((tid >> 3) + i * 32 < x.cnt) adt_cp16(oper + (uint32_t)tile * (TT * 128) + adt_swizzled((tid >> 3) + i * 32, c), s + i * 32 * 128, true);
+                    if (r8 + i * 32 < x.cnt) adt_cp16(at + i * 4096, s + i * 4096, true);
             }
         }
     };
@@ -362,7 +373,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
     };
     auto token_of = [&](const Unit& x) { return tid < x.cnt ? p.plan.place()[x.first + tid] : 0; };
     auto back_of = [&](const Unit& x) {
-        return x.R && tid < x.cnt ? *reinterpret_cast<const float*>(x.low + (size_t)NP * adt_chunks(L) * p.tokens * 128 + (size_t)(x.first + tid) * 4) : 0.f;
+        return x.R && tid < x.cnt ? *reinterpret_cast<const float*>(x.low + NP * adt_chunks(L) * tile_bytes - (size_t)x.first * 124 + tid * 4) : 0.f;
     };
     // a thread's token: where its rows are; its base is asked of L2
     auto place_token = [&](const Unit& x, int buf, int t, float back) {
@@ -370,10 +381,10 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
         s_at[buf][tid] = make_longlong2((long long)t * x.base_stride, (long long)t * x.out_stride);
         s_back[buf][tid] = back;
         if (x.base) {
-            const O* const row = x.base + (long long)t * x.base_stride + x.n0;
+            const O* const row = x.base + (long long)t * x.base_stride;
 #pragma unroll
             for (int i = 0; i < (int)sizeof(O); ++i)
-                if (x.n0 + i * (128 / (int)sizeof(O)) < x.N) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i * (128 / (int)sizeof(O))));
+                if (i * (128 / (int)sizeof(O)) < x.left) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + i * (128 / (int)sizeof(O))));
         }
     };
     // base of four tokens of the 32, four outputs a lane, as they lie in memory: widened where they are used, or the loads would be waited for here
@@ -382,7 +393,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
     Raw y[OWN];
     auto load_base = [&](const Unit& x, int buf, int c) {
         const int t0 = c + warp * OWN;
-        const O* const from = x.base + x.n0 + lane * 4;
+        const O* const from = x.base + lane * 4;
         if (!x.base) {
 #pragma unroll
             for (int i = 0; i < OWN; ++i) y[i] = Raw{};
@@ -391,13 +402,23 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
             for (int i = 0; i < OWN; ++i)
                 if (t0 + i < x.cnt) y[i] = *reinterpret_cast<const Raw*>(from + s_at[buf][t0 + i].x);
         } else {
+            // (loops, not predicated code beside the accesses above)
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
                 Raw r{};
                 O* const e = reinterpret_cast<O*>(&r);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (t0 + i < x.cnt && x.n0 + lane * 4 + k < x.N) e[k] = from[s_at[buf][t0 + i].x + k];
+                if (t0 + i < x.cnt) {
+                    const O* const at = from + s_at[buf][t0 + i].x;
+                    const int n = min(4, x.left - lane * 4);
+#pragma unroll 1
+                    for (int k = 0; k < n; ++k) {
+                        const O o = at[k];
+                        if (k == 0) e[0] = o;
+                        else if (k == 1) e[1] = o;
+                        else if (k == 2) e[2] = o;
+                        else e[3] = o;
+                    }
+                }
                 y[i] = r;
             }
         }
@@ -473,17 +494,18 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
             }
             if (!last) load_base(cur, buf, c + ADT_ROWS);
             else if (more) load_base(next, buf_next, 0);
-            O* const to = cur.out + cur.n0 + lane * 4;
+            O* const to = cur.out + lane * 4;
             if (cur.vec) {
 #pragma unroll
                 for (int i = 0; i < OWN; ++i)
                     if (c + t0 + i < cur.cnt) adp_store4(to + s_at[buf][c + t0 + i].y, w[i]);
             } else {
 #pragma unroll
-                for (int i = 0; i < OWN; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c + t0 + i < cur.cnt && cur.n0 + lane * 4 + e < cur.N) adp_put(to + s_at[buf][c + t0 + i].y + e, w[i][e]);
+                for (int i = 0; i < OWN; ++i) {
+                    const int n = c + t0 + i < cur.cnt ? min(4, cur.left - lane * 4) : 0;
+#pragma unroll 1
+                    for (int e = 0; e < n; ++e) adp_put(to + s_at[buf][c + t0 + i].y + e, e == 0 ? w[i][0] : (e == 1 ? w[i][1] : (e == 2 ? w[i][2] : w[i][3])));
+                }
             }
             if (c == 0 && !last && more && next.R) load_operands(next);
         }
