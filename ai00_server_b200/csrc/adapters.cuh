@@ -163,7 +163,7 @@ __device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const
 }
 
 // MANY: registers for four CTAs on an SM instead of three, where a call has more than three for each (64 tokens with adapters of rank 32 to 14336 outputs, 512
-// CTAs, 20 us; with three 25; 16 tokens of four projections, 320 CTAs, 8.5 and 7.7)
+// CTAs: 20 us, with three 30; 16 tokens of four projections, 320 CTAs, stay at three: 7.7 us, with four 8.5)
 template <typename E, typename O, bool MANY>
 __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, MANY ? 4 : 3) adapter_few_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];

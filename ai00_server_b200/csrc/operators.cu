@@ -249,7 +249,12 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
         d.K = s.in_features; d.N = s.out_features; d.R = s.rank;
         d.vec = ((uintptr_t)s.out | (uintptr_t)s.base) % (4 * osize) == 0 && s.out_stride % 4 == 0 && (!s.base || s.base_stride % 4 == 0);
         p.rank = std::max(p.rank, s.rank);
-        if (s.base != s.out || s.base_stride != s.out_stride) p.copy = 1;
+        // (the projections of a call run side by side)
+        for (int j = 0; j < q->num_parts; ++j)
+            REQUIRE(parts[j].x != s.out && (j == i || (parts[j].out != s.out && parts[j].base != s.out)), B200RWKV_ERR_INVALID,
+                    "op_adapters: the out of a part is the x, base or out of another (or its own x)");
+        REQUIRE(s.base != s.out || s.base_stride == s.out_stride || q->tokens == 1, B200RWKV_ERR_INVALID, "op_adapters: base is out, but with another stride");
+        if (s.base != s.out) p.copy = 1;
     }
     if (q->tokens == 0) return B200RWKV_OK;
     const size_t need = adapters_workspace(q->tokens, q->adapters, q->num_parts, p.rank);
@@ -275,6 +280,8 @@ int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* 
     REQUIRE(q->logits && q->out, B200RWKV_ERR_INVALID, "op_logits: null logits or out");
     REQUIRE(q->logits_stride >= q->vocab && q->out_stride >= q->vocab, B200RWKV_ERR_INVALID, "op_logits: rows overlap (a stride is smaller than the vocabulary)");
     REQUIRE((uintptr_t)q->logits % size == 0 && (uintptr_t)q->out % 4 == 0, B200RWKV_ERR_INVALID, "op_logits: misaligned logits or out");
+    REQUIRE((const void*)q->out != q->logits || (q->type == B200RWKV_TYPE_F32 && (q->rows == 1 || q->logits_stride == q->out_stride)), B200RWKV_ERR_INVALID,
+            "op_logits: out is logits, but their rows do not lie alike");
     REQUIRE(!q->history_offset || q->history, B200RWKV_ERR_INVALID, "op_logits: history offsets without tokens");
     REQUIRE(!q->bias_offset || (q->bias_token && q->bias_value), B200RWKV_ERR_INVALID, "op_logits: bias offsets without tokens or values");
     REQUIRE(!q->allow || q->allow_rows >= (q->allow_row ? 0 : q->rows), B200RWKV_ERR_INVALID, "op_logits: fewer masks than rows");

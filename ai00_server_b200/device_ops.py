@@ -5,7 +5,7 @@ requests of a batch, for programs that hold theirs as torch tensors.
   logits     rows of logits adjusted by penalties, biases and grammar masks, as logits, probabilities or log-probabilities
 
 A call enqueues kernels on the current stream of its tensors' device and returns; it can be captured into a graph.  Arguments that
-do not fit raise capi.B200Error before anything is enqueued.  Nothing here has a gradient: the operators serve.
+do not fit raise capi.B200Error before anything is enqueued, and so do tensors that ask for a gradient: the operators serve, they have none.
 """
 from __future__ import annotations
 
@@ -31,6 +31,8 @@ def _list(t, name, dtype, where, size):
     """Address of a contiguous vector or table of `dtype` on device `where` with `size` elements (None: any number)."""
     if t.dtype is not dtype or t.get_device() != where or not t.is_contiguous():
         _bad(f"{name} must be a contiguous {dtype} tensor on cuda:{where}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(f"{name} requires a gradient: these operators have none (call them under torch.no_grad())")
     if size is not None and t.numel() != size:
         _bad(f"{name} has {t.numel()} elements, {size} are wanted")
     return t.data_ptr()
@@ -40,6 +42,8 @@ def _row_stride(t, name, shape, dtype, where):
     """Elements between the rows of a [rows, cols] tensor with neighbouring columns."""
     if t.dtype is not dtype or t.shape != shape or t.get_device() != where:
         _bad(f"{name} must be a {list(shape)} {dtype} tensor on cuda:{where}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(f"{name} requires a gradient: these operators have none (call them under torch.no_grad())")
     s0, s1 = t.stride()
     if s1 != 1 and shape[1] > 1:
         _bad(f"{name}: columns of a row must be neighbours")

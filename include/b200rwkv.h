@@ -258,7 +258,8 @@ int32_t b200rwkv_sample_rows(b200rwkv_engine*, int32_t nrows, const b200rwkv_row
  * W x + alpha * lora.1 (lora.0^T x).  A model holds up to 64 of them.  RWKV models on one GPU (also with quantised layers and at
  * precision 1); others answer B200RWKV_ERR_UNSUPPORTED.  b200rwkv_slot_adapter: tokens of the slot use the adapter from the next
  * b200rwkv_infer call on (id 0: none), until the next call for that slot -- resetting or writing the slot's state does not change it.
- * b200rwkv_adapter_free refuses (B200RWKV_ERR_STATE) while a slot has the adapter.  The image is borrowed during the call only. */
+ * b200rwkv_adapter_free refuses (B200RWKV_ERR_STATE) while a slot has the adapter.  The image is borrowed during the call only.  The
+ * measurement hooks (b200rwkv_bench_decode, b200rwkv_profile_*) run without adapters. */
 int32_t b200rwkv_adapter_load(b200rwkv_engine*, const uint8_t* st, size_t len, float alpha, uint64_t* adapter_id);
 int32_t b200rwkv_adapter_free(b200rwkv_engine*, uint64_t adapter_id);
 int32_t b200rwkv_slot_adapter(b200rwkv_engine*, int32_t slot, uint64_t adapter_id);
@@ -337,7 +338,7 @@ typedef struct {
     const void* b;               /* [adapters, out_features, rank] of `type` */
     const void* base;            /* [tokens, out_features] of `out_type`, or NULL; may be `out` itself, else apart from it */
     int64_t base_stride;
-    void* out;                   /* [tokens, out_features] of `out_type`; nothing else is written */
+    void* out;                   /* [tokens, out_features] of `out_type`; nothing else is written.  Apart from every x and from the other parts' base and out */
     int64_t out_stride;
     int32_t in_features;         /* a multiple of 8 */
     int32_t out_features;

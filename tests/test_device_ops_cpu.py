@@ -25,6 +25,7 @@ def _adapters(**change):
     ({"a": None}, capi.ERR_INVALID), ({"b": None}, capi.ERR_INVALID), ({"out": None}, capi.ERR_INVALID), ({"x": 4098}, capi.ERR_INVALID),
     ({"a": 4104}, capi.ERR_INVALID), ({"b": 4104}, capi.ERR_INVALID), ({"x_stride": 68}, capi.ERR_INVALID), ({"x_stride": 56}, capi.ERR_INVALID),
     ({"out_stride": 31}, capi.ERR_INVALID), ({"base_stride": 31}, capi.ERR_INVALID), ({"out": 8194}, capi.ERR_INVALID),
+    ({"out": 4096}, capi.ERR_INVALID), ({"base": 8192, "base_stride": 64}, capi.ERR_INVALID),       # its own x; the same rows with another stride
     ({"tokens": 300}, capi.ERR_INVALID),                                             # no workspace
     ({"tokens": 300, "workspace": 4096, "workspace_bytes": 64}, capi.ERR_INVALID),
     ({"tokens": 300, "workspace": 4100, "workspace_bytes": 1 << 20}, capi.ERR_INVALID)])
@@ -33,6 +34,17 @@ def test_op_adapters_refuses(change, code):
         capi.check(capi.lib().b200rwkv_op_adapters(0, None, *_adapters(**change)))
     assert ei.value.code == code
     assert "op_adapters" in str(ei.value)
+
+
+@pytest.mark.parametrize("change", [{"out": 8192}, {"base": 8192}, {"x": 8192}, {"x": 12288 + 4096, "out": 4096}])
+def test_op_adapters_refuses_parts_that_write_what_another_reads(change):
+    def part(**c):
+        return capi.AdapterPart(**{**dict(x=4096, x_stride=64, a=4096, b=4096, base=12288, base_stride=32, out=12288, out_stride=32, in_features=64, out_features=32, rank=16), **c})
+    parts = (capi.AdapterPart * 2)(part(base=8192, out=8192), part(**change))
+    q = capi.Adapters(struct_bytes=C.sizeof(capi.Adapters), type=capi.TYPE_F16, out_type=capi.TYPE_F32, tokens=4, adapters=2, num_parts=2, index=4096, scale=4096)
+    with pytest.raises(capi.B200Error, match="of another") as ei:
+        capi.check(capi.lib().b200rwkv_op_adapters(0, None, C.byref(q), parts))
+    assert ei.value.code == capi.ERR_INVALID
 
 
 def test_op_adapters_null_struct_and_no_tokens():
@@ -62,7 +74,8 @@ def _logits(**change):
     ({"out": None}, capi.ERR_INVALID), ({"logits_stride": 99}, capi.ERR_INVALID), ({"out_stride": 99}, capi.ERR_INVALID), ({"logits": 4098}, capi.ERR_INVALID),
     ({"out": 8194}, capi.ERR_INVALID), ({"history_offset": 4096}, capi.ERR_INVALID), ({"bias_offset": 4096}, capi.ERR_INVALID),
     ({"bias_offset": 4096, "bias_token": 4096}, capi.ERR_INVALID), ({"allow": 4096, "allow_rows": 1}, capi.ERR_INVALID),
-    ({"allow": 4096, "allow_rows": -1, "allow_row": 4096}, capi.ERR_INVALID)])
+    ({"allow": 4096, "allow_rows": -1, "allow_row": 4096}, capi.ERR_INVALID), ({"vocab": 524289, "logits_stride": 1 << 20, "out_stride": 1 << 20}, capi.ERR_UNSUPPORTED),
+    ({"rows": (1 << 24) + 1}, capi.ERR_INVALID), ({"out": 4096, "type": capi.TYPE_F16}, capi.ERR_INVALID), ({"out": 4096, "out_stride": 128}, capi.ERR_INVALID)])
 def test_op_logits_refuses(change, code):
     with pytest.raises(capi.B200Error) as ei:
         capi.check(capi.lib().b200rwkv_op_logits(0, None, C.byref(_logits(**change))))

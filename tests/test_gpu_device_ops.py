@@ -490,6 +490,67 @@ def test_logits_graph_stream_and_no_rows(ops):
     assert torch.equal(o2, res)
 
 
+def test_logits_history_longer_than_is_counted(ops):
+    """Of a history the newest 2^17 - 1 tokens count: a token that is older than those alone is as if it had not been said."""
+    V, m = 300, 140000
+    most = (1 << 17) - 1
+    rows = rnd(1, V, seed=13)
+    history = [7] * 10 + [5] * (m - 10)
+    off, flat = ragged([history])
+    controls = torch.tensor([[2.0, 1.0, 0.5, 1.0, 1.0]]).cuda()
+    out = ops.logits(rows, kind="logits", controls=controls, history=flat, history_offset=off)
+    r = float(rows[0, 5])
+    want = (r / 2 if r > 0 else r * 2) - (1.0 + 0.5 * most)
+    assert abs(float(out[0, 5]) - want) <= abs(want) * 2.0 ** -22
+    keep = torch.ones(V, dtype=torch.bool, device="cuda")
+    keep[5] = False
+    assert torch.equal(out[0, keep], rows[0, keep])
+
+
+def test_tensors_that_ask_for_a_gradient_are_refused(ops):
+    x, a, b, scale, y = make(3, 64, 32, 8, 2, F16, F16)
+    index = indices(3, 2, "distinct")
+    for t in (x, a, b, y):
+        t.requires_grad_()
+        with pytest.raises(capi.B200Error):
+            ops.low_rank(x, a, b, index, scale, base=y)
+        with torch.no_grad():
+            ops.low_rank(x, a, b, index, scale, base=y)
+        t.requires_grad_(False)
+    rows = rnd(2, 50).requires_grad_()
+    with pytest.raises(capi.B200Error):
+        ops.logits(rows)
+
+
+def test_the_first_call_of_a_process_can_be_captured():
+    """Kernels are set up by the call that needs them first, also while a stream is captured."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch
+from ai00_server_b200 import device_ops as d
+r = lambda *s: torch.randn(*s, device="cuda")
+sets = [(T, r(T, 64).half(), r(3, 16, 64).half(), r(3, 40, 16).half(), (torch.arange(T, device="cuda") % 3).int(), torch.ones(3, device="cuda")) for T in (1, 40, 300)]
+rows = r(4, 500)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    outs = [d.low_rank(x, a, b, i, s) for _, x, a, b, i, s in sets]
+    probs = d.logits(rows)
+g.replay()
+torch.cuda.synchronize()
+for (T, x, a, b, i, s), o in zip(sets, outs):
+    w = torch.stack([(x[t].float() @ a[t % 3].float().T) @ b[t % 3].float().T for t in range(T)])
+    assert ((o.float() - w).abs() <= 2e-2 * w.abs().max()).all()
+assert ((probs - rows.softmax(1)).abs() <= 1e-6).all()
+print("captured")
+"""
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
+
+
 def test_head_adapter_then_probabilities(ops):
     """A decode batch's last steps as a server runs them, captured as one graph: adapters of the vocabulary head on the head's own output, then the
     requests' penalties, masks and biases."""
