@@ -101,6 +101,17 @@ __device__ __forceinline__ float adp_dot8(const uint4& a, const float (&x)[8], f
     return s;
 }
 
+// the activations that projections with adapters end in (gate, channel-mix key and receptance), as the projection's own epilogue computes them: tokens without
+// an adapter have the same bits beside those with one
+__device__ __forceinline__ float adp_act(float v, int act) {
+    if (act == ACT_RELU2) {
+        const float r = fmaxf(v, 0.f);
+        return r * r;
+    }
+    const float s = sigmoidf_(v);
+    return act == ACT_SILU ? v * s : s;
+}
+
 struct AdpGroup {
     int tok[ADP_TOK];            // tokens, -1 behind the last
     int adapter;                 // -1: none
@@ -117,7 +128,7 @@ __device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const
     int id = -2;
     if (tid < p.tokens) {
         id = p.index[tid];
-        if (id < 0 || id >= p.adapters) id = p.copy ? -1 : -2;
+        if (id < 0 || id >= p.adapters) id = p.copy && !(p.finish && id == -2) ? -1 : -2;
     }
     if (one) {
         if (warp == 0) {
@@ -164,7 +175,8 @@ __device__ __forceinline__ void adapter_find_group(const AdapterParams& p, const
 
 // MANY: registers for four CTAs on an SM instead of three, where a call has more than three for each (64 tokens with adapters of rank 32 to 14336 outputs, 512
 // CTAs: 20 us, with three 30; 16 tokens of four projections, 320 CTAs, stay at three: 7.7 us, with four 8.5)
-template <typename E, typename O, bool MANY>
+// FIN: parts may end in an activation, as f32 rows or as the operand of the next projection
+template <typename E, typename O, bool MANY, bool FIN>
 __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, MANY ? 4 : 3) adapter_few_kernel(const __grid_constant__ AdapterParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ AdpGroup g;
@@ -176,6 +188,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, 
     const int cta = blockIdx.x % ADP_CTAS, want = blockIdx.x / ADP_CTAS;
     const AdapterPart& q = p.part[blockIdx.y];
     pdl_wait();
+    pdl_launch_dependents();                     // (a projection behind this one then has its first weights when its turn comes)
     if (p.plan.base) {
         if (want >= p.plan.count()[0]) return;
         const int4 gr = p.plan.group()[want];
@@ -194,6 +207,45 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, 
     const int adapter = g.adapter, K = q.K, N = q.N;
     O* const out = reinterpret_cast<O*>(q.out);
     const O* const base = reinterpret_cast<const O*>(q.base);
+    // outputs n (.. n + 3) of token t
+    auto put = [&](int t, int n, float v) {
+        if constexpr (FIN) {
+            if (q.fin) v = adp_act(v, q.act);
+            if (q.fin >= ADP_A16) {
+                __half hi = __float2half_rn(v), lo;
+                if (q.fin == ADP_A16_SPLIT) {
+                    split_h(v, hi, lo);
+                    reinterpret_cast<__half*>(q.out)[a16_index(t + 16, n, q.out_th)] = lo;
+                } else {
+                    hi = f2h_sat(v);
+                }
+                reinterpret_cast<__half*>(q.out)[a16_index(t, n, q.out_th)] = hi;
+                return;
+            }
+        }
+        adp_put(out + (size_t)t * q.out_stride + n, v);
+    };
+    auto put4 = [&](int t, int n, float (&v)[4]) {
+        if constexpr (FIN) {
+            if (q.fin) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = adp_act(v[i], q.act);
+            }
+            if (q.fin >= ADP_A16) {
+                uint2 hi, lo;
+                if (q.fin == ADP_A16_SPLIT) {
+                    split_pack_h2(v[0], v[1], hi.x, lo.x);
+                    split_pack_h2(v[2], v[3], hi.y, lo.y);
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(q.out) + a16_index(t + 16, n, q.out_th)) = lo;
+                } else {
+                    hi = make_uint2(pack_h2(v[0], v[1]), pack_h2(v[2], v[3]));
+                }
+                *reinterpret_cast<uint2*>(reinterpret_cast<__half*>(q.out) + a16_index(t, n, q.out_th)) = hi;
+                return;
+            }
+        }
+        adp_store4(out + (size_t)t * q.out_stride + n, v);
+    };
     const E *A = nullptr, *B = nullptr;
     int R = 0;
     float scale = 0.f;
@@ -215,7 +267,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, 
             const int t = g.tok[j];
             if (t < 0) continue;
             for (int n = u0 * 32 + lane; n < min(u1 * 32, N); n += 32)
-                adp_put(out + (size_t)t * q.out_stride + n, base ? adp_widen(base[(size_t)t * q.base_stride + n]) : 0.f);
+                put(t, n, base ? adp_widen(base[(size_t)t * q.base_stride + n]) : 0.f);
         }
         return;
     }
@@ -315,7 +367,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, 
             const float k0 = (up ? acc[2] : acc[0]) + __shfl_xor_sync(0xffffffffu, up ? acc[0] : acc[2], 2);
             const float k1 = (up ? acc[3] : acc[1]) + __shfl_xor_sync(0xffffffffu, up ? acc[1] : acc[3], 2);
             const float d = (odd ? k1 : k0) + __shfl_xor_sync(0xffffffffu, odd ? k0 : k1, 1);
-            if (ok) adp_put(out + (size_t)tok * q.out_stride + n, adp_widen(y) + d);
+            if (ok) put(tok, n, adp_widen(y) + d);
         }
         return;
     }
@@ -472,16 +524,15 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADP_THREADS, 
             if (t < 0) continue;
             const float back = h ? backb : backa;
             const float d[4] = {acc[0][h] * back, acc[0][2 + h] * back, acc[1][h] * back, acc[1][2 + h] * back};
-            O* const o = out + (size_t)t * q.out_stride + n;
             const O* const y = base ? base + (size_t)t * q.base_stride + n : nullptr;
             if (four) {
                 float v[4];
                 AdpRaw<O>::widen(h ? yb : ya, v);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += d[i];
-                adp_store4(o, v);
+                put4(t, n, v);
             } else {
-                for (int i = 0; i < 4 && n + i < N; ++i) adp_put(o + i, (y ? adp_widen(y[i]) : 0.f) + d[i]);
+                for (int i = 0; i < 4 && n + i < N; ++i) put(t, n + i, (y ? adp_widen(y[i]) : 0.f) + d[i]);
             }
         }
     }

@@ -91,6 +91,9 @@ void adapters_shape(AdapterParams& p, void* workspace, int type, int out_type) {
 
 void adapters_plan(cudaStream_t s, const AdapterParams& p) { launch(adapter_plan_kernel, dim3(1), ADP_PLAN_THREADS, 0, s, p); }
 
+// types of the engine's own calls
+template <typename E, typename O> constexpr bool adapter_finishes = std::is_same_v<E, __half> && std::is_same_v<O, float>;
+
 template <typename E, typename O>
 static void ready() {
     constexpr int NP = AdpParts<E, O>::N;
@@ -103,8 +106,11 @@ static void ready() {
         }
         return m;
     }();
-    prepare<adapter_few_kernel<E, O, false>>(adapter_few_smem(ADP_MAX_RANK, NP));
-    prepare<adapter_few_kernel<E, O, true>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    prepare<adapter_few_kernel<E, O, false, false>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    prepare<adapter_few_kernel<E, O, true, false>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    if constexpr (adapter_finishes<E, O>) {
+        prepare<adapter_few_kernel<E, O, false, true>>(adapter_few_smem(ADP_MAX_RANK, NP));
+    }
     prepare<adapter_low_kernel<E, NP>>(most.low);
     prepare<adapter_out_kernel<E, O>>(most.out);
 }
@@ -129,7 +135,11 @@ static void apply(cudaStream_t s, const AdapterParams& p) {
     }
     if (groups > 0) {
         const bool many = (long long)ADP_CTAS * groups * p.nparts > 3 * sm_count();
-        launch(many ? adapter_few_kernel<E, O, true> : adapter_few_kernel<E, O, false>, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
+        auto kern = many ? adapter_few_kernel<E, O, true, false> : adapter_few_kernel<E, O, false, false>;
+        if constexpr (adapter_finishes<E, O>) {
+            if (p.finish) kern = adapter_few_kernel<E, O, false, true>;
+        }
+        launch(kern, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
     }
 }
 

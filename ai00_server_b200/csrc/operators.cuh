@@ -36,7 +36,10 @@ struct AdapterPart {
     long long out_stride;
     int K, N, R;                 // R: the largest rank
     int vec;                     // rows of base and out take accesses of four elements
+    int fin;                     // (AdapterParams::finish) `out` has the activation `act` of the sums: AdapterFin
+    int act, out_th;             // out_th: height of an A16 output
 };
+enum AdapterFin : int { ADP_SUMS = 0, ADP_F32 = 1, ADP_A16 = 2, ADP_A16_SPLIT = 3 };
 
 // a call of more tokens than ADP_INLINE: counts of groups (adapters.cuh) and of tiles (adapter_tiles.cuh), {adapter, first place, tokens} of each, tokens by place
 struct AdapterPlan {
@@ -52,6 +55,7 @@ struct AdapterPlan {
 struct AdapterParams {
     int tokens, adapters;
     int copy;                    // tokens without an adapter have their base copied (base and out differ)
+    int finish;                  // some parts end in their activation (up to ADP_INLINE tokens, f16 to f32); index -2 is then a row behind the last token
     const int* index;
     const float* scale;
     AdapterPlan plan;

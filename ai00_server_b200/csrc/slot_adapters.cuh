@@ -1,6 +1,6 @@
 // Adapters of slots in the steps of the RWKV models: what surrounds adapters.cuh's products.  A step with such slots runs its projections as ever; behind
 // each launch the adapters are added to the outputs in place.  Projections that end in an activation (gate, channel-mix key and receptance) leave
-// their sums in a scratch row instead, and the activation follows here.
+// their sums in a scratch row instead, and the activation follows: in the adapters' kernel itself in steps of up to ADP_INLINE tokens, here in longer ones.
 // Measured beside the projections of a step: see the table of steps with adapters.
 #pragma once
 #include "operators.cuh"
@@ -9,7 +9,7 @@ namespace b200 {
 
 constexpr int ADAPTER_POOL = 64;               // adapters a model holds at once
 
-// adapter (place in the pool, -1: none) of every token and of every logits row of the step; rows behind the last have none
+// adapter (place in the pool, -1: none) of every token and of every logits row of the step; rows behind the last: -2
 struct AdapterIndexParams {
     MetaView meta;
     const int* slot_adapter;
@@ -18,10 +18,11 @@ struct AdapterIndexParams {
 };
 __global__ void adapter_index_kernel(const __grid_constant__ AdapterIndexParams p) {
     pdl_wait();
+    pdl_launch_dependents();
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     const int T = p.meta.T(), R = p.meta.R();
-    if (i < p.rows) p.tok[i] = i < T ? p.slot_adapter[p.meta.tok_slot()[i]] : -1;
-    if (i < p.out_rows) p.row[i] = i < R ? p.slot_adapter[p.meta.tok_slot()[p.meta.out_tok()[i]]] : -1;
+    if (i < p.rows) p.tok[i] = i < T ? p.slot_adapter[p.meta.tok_slot()[i]] : -2;
+    if (i < p.out_rows) p.row[i] = i < R ? p.slot_adapter[p.meta.tok_slot()[p.meta.out_tok()[i]]] : -2;
 }
 
 // dst[r][i] = src[i][r], zero for r in [ranks, padded): `<name>.lora.0` as the converter writes it -> rows of k
@@ -52,6 +53,7 @@ struct AdapterFinishParams {
 };
 __global__ void __launch_bounds__(256) adapter_finish_kernel(const __grid_constant__ AdapterFinishParams p) {
     pdl_wait();
+    pdl_launch_dependents();
     const int per = p.N / 8, total = per * *p.nrows;
     for (int i = blockIdx.x * 256 + threadIdx.x; i < total; i += gridDim.x * 256) {
         const int m = i / per, n = (i - m * per) * 8;

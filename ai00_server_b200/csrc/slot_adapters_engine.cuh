@@ -183,12 +183,25 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
         d.base_stride = d.out_stride = sg.ldo;
         d.K = site.K; d.N = site.N; d.R = adapter_rank;
         d.vec = sg.ldo % 4 == 0 && (uintptr_t)sg.out % 16 == 0;
+        const GemmSeg& to = was.seg[i];
+        if (p.plan.base || sg.out == to.out) continue;
+        const bool a16 = to.out_mode == OUT_A16;
+        REQUIRE(to.act == ACT_SIGMOID || to.act == ACT_SILU || to.act == ACT_RELU2, B200RWKV_ERR_INVALID, "internal: activation behind an adapter");
+        p.copy = p.finish = 1;
+        d.out = to.out;
+        d.act = to.act;
+        d.fin = a16 ? (split ? ADP_A16_SPLIT : ADP_A16) : ADP_F32;
+        if (a16) d.out_th = to.ldo;
+        else {
+            d.out_stride = to.ldo;
+            d.vec = d.vec && to.ldo % 4 == 0 && (uintptr_t)to.out % 16 == 0;
+        }
     }
     if (n == 0) return;
     p.nparts = n;
     adapters_apply(s, p, B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
     ++launches_last_step;
-    for (int i = 0; i < gp.nseg; ++i) {
+    for (int i = 0; i < gp.nseg && !p.finish; ++i) {
         const GemmSeg &sg = gp.seg[i], &to = was.seg[i];
         if (g.site[i] < 0 || sg.out == to.out) continue;
         AdapterFinishParams q{(const float*)sg.out, gp.nrows, to.out, to.N, to.act, to.out_mode == OUT_A16, split, to.ldo};
