@@ -1,7 +1,8 @@
 // Adapters of slots in the steps of the RWKV models: what surrounds adapters.cuh's products.  A step with such slots runs its projections as ever; behind
 // each launch the adapters are added to the outputs in place.  Projections that end in an activation (gate, channel-mix key and receptance) leave
 // their sums in a scratch row instead, and the activation follows: in the adapters' kernel itself in steps of up to ADP_INLINE tokens, here in longer ones.
-// Measured beside the projections of a step: see the table of steps with adapters.
+// Bound: four dependent launches a layer, 6 to 8 us each (8 layers of 7B widths, rank 16: a step of 16 slots 1061 us without adapters, 1549 with sixteen of them; with
+// the activations in launches of their own 1592).
 #pragma once
 #include "operators.cuh"
 
