@@ -8,7 +8,7 @@
 //
 // Bound: a row is read and written once, 8 bytes a token for f32 rows (row of 65536: 0.5 MB; 512 rows 41 us at the copy rate); one row is latency.
 // Shape: a cluster of eight or sixteen CTAs a row, the row in their registers (16 to 64 tokens a thread) between the only read and the only write; 32 tokens a
-// thread and CTAs of 256 where there are many rows (512 rows of 65536: 57 us, with 16 tokens and CTAs of 512 70), which settle their sums more quickly.
+// thread and CTAs of 256 where there are many rows (512 rows of 65536: 56 us, with 16 tokens and CTAs of 512 70, with 32 and sixteen CTAs of 128 63), which settle their sums more quickly.
 // Tokens go to the CTAs in stripes of 64, so that frequent tokens that are neighbours in a vocabulary spread over all of them.
 //   * a history is added up in shared memory, a pair of words for each token of the CTA: decay^age in units of 2^-28, its lower 14 bits to one word
 //     and the others to the other, so that neither overflows (2^17 - 1 entries; of a longer history the newest count), no atomic has to answer,
@@ -41,12 +41,13 @@ __device__ __forceinline__ float4 logits4(const __nv_bfloat16* p) {
 
 constexpr unsigned LOGITS_SEEN = 1u << 31;        // flag in the upper word of a token that is in the history and does not count there
 
-// e^x as a power of two: a multiplication and the unit's instruction, good to 2^-22 and to the rounding of its argument.  (expf is eight instructions)
-__device__ __forceinline__ float logits_exp(float x) {
+// 2^x by the unit's instruction, good to 2^-22; what is below 2^-126 is zero.  (expf is eight instructions)
+__device__ __forceinline__ float logits_exp2(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float logits_exp(float x) { return logits_exp2(x * 1.4426950408889634f); }
 
 // sum of exponentials relative to a maximum.  NaN never becomes the maximum: it stays in the sum, and through it reaches the whole row
 struct LogitsSum {
@@ -99,6 +100,9 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
     auto again = [&] { asm volatile("" : "+r"(t_first)); };
     auto there = [&](int t) { return t >= 0 && t < V; };
     auto whole = [&](int t) { return VEC && t >= 0 && t + 3 < V; };
+    const float* const ctl = p.controls ? p.controls + (size_t)row * 5 : nullptr;
+    const int h0 = p.hist_off ? p.hist_off[row] : 0, hn = p.hist_off ? p.hist_off[row + 1] - h0 : 0;
+    const int b0 = p.bias_off ? p.bias_off[row] : 0, bn = p.bias_off ? p.bias_off[row + 1] - b0 : 0;
     float v[NV][4];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -115,15 +119,12 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
         }
     }
     again();
-    const float* const ctl = p.controls ? p.controls + (size_t)row * 5 : nullptr;
-    const int h0 = p.hist_off ? p.hist_off[row] : 0, hn = p.hist_off ? p.hist_off[row + 1] - h0 : 0;
-    const int b0 = p.bias_off ? p.bias_off[row] : 0, bn = p.bias_off ? p.bias_off[row + 1] - b0 : 0;
 
     // ---- lists, for as many of the CTA's tokens at a time as have their sums in shared memory ----
     if (hn > 0 || bn > 0) {
         // f(j, place of its token) for the entries of a list from `first` on that are among them
         auto each = [&](const int* tok, int first, int count, int s0, auto&& f) {
-            constexpr int U = 4;
+            constexpr int U = 4;                     // entries in flight (96 rows of 100003 with histories of 8000: 66 us, with one 75; with eight single rows take 15 % longer)
             for (int j0 = first + tid; j0 < count; j0 += TH * U) {
                 unsigned t[U];
 #pragma unroll
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
                         return;
                     }
                     const int age = hn - 1 - j;
-                    const unsigned c = age == 0 ? 1u << 28 : max(1u, (unsigned)(exp2f(lg * (float)age) * 268435456.f + 0.5f));      // (zero decay: one unit from the second newest on)
+                    const unsigned c = age == 0 ? 1u << 28 : max(1u, (unsigned)(logits_exp2(lg * (float)age) * 268435456.f + 0.5f));      // (zero decay: one unit from the second newest on)
                     if (c & 0x3FFFu) atomicAdd(&sums[i].x, c & 0x3FFFu);
                     if (c >> 14) atomicAdd(&sums[i].y, c >> 14);
                 });
