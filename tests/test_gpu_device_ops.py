@@ -100,6 +100,29 @@ def test_adapters_against_64_bits(ops, dtype, out_dtype, T, K, N, R, n, how):
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("T,n,how", [(8193, 1024, "mixed"), (20000, 3, "mixed"), (33000, 1000, "runs"), (1 << 20, 5, "mixed")])
+def test_adapters_of_very_long_calls(ops, T, n, how):
+    """More tokens than the order keeps bins for, more tiles than a CTA keeps places of; the largest call."""
+    x, a, b, scale, y = make(T, 8, 4, 8, n, F16, F32)
+    index = indices(T, n, how)
+    out = ops.low_rank(x, a, b, index, scale, base=y)
+    check_adapters(out, *adapter_want(x, a, b, index, scale, y, F32))
+
+
+@pytest.mark.parametrize("T", [4, 260])
+def test_adapters_rows_far_apart(ops, T):
+    """Rows of x, base and out further from each other than 32 bits count elements."""
+    K, N, n = 64, 40, 3
+    step = ((1 << 32) // (T - 1) + 4096) & ~7
+    x, a, b, scale, y = make(T, K, N, 16, n, F16, F16)
+    far = [torch.empty((T - 1) * step + 64, dtype=F16, device="cuda").as_strided((T, w), (step, 1)) for w in (K, N, N)]
+    far[0].copy_(x)
+    far[1].copy_(y)
+    index = indices(T, n, "mixed")
+    ops.low_rank(far[0], a, b, index, scale, base=far[1], out=far[2])
+    check_adapters(far[2].contiguous(), *adapter_want(x, a, b, index, scale, y, F16))
+
+
 @pytest.mark.parametrize("T,n", [(5, 3), (300, 9), (700, 2)])
 def test_adapters_without_a_base_and_in_place(ops, T, n):
     x, a, b, scale, y = make(T, 200, 76, 24, n, F16, F32)
@@ -488,6 +511,46 @@ def test_logits_graph_stream_and_no_rows(ops):
         o2 = ops.logits(rows, kind="log_probs", controls=controls, history=flat, history_offset=off)
     s.synchronize()
     assert torch.equal(o2, res)
+
+
+@pytest.mark.parametrize("kind", ["logits", "probs"])
+def test_logits_rows_far_apart(ops, kind):
+    n, V, step = 4, 1000, (1 << 32) // 3 + 4096
+    rows = rnd(n, V, seed=21)
+    far = torch.empty((n - 1) * step + V, device="cuda").as_strided((n, V), (step, 1))
+    out = torch.empty((n - 1) * step + V, device="cuda").as_strided((n, V), (step, 1))
+    far.copy_(rows)
+    ops.logits(far, kind=kind, out=out)
+    assert torch.equal(out.contiguous(), ops.logits(rows, kind=kind)) if kind == "logits" else bool(((out - ops.logits(rows)).abs() <= 2.0 ** -20 * out).all())
+
+
+def test_calls_from_two_threads(ops):
+    """Two host threads, each on a stream of its own, at the same time: what each gets is what it gets alone."""
+    import threading
+    sets = []
+    for i, T in enumerate((40, 700)):
+        x, a, b, scale, y = make(T, 256, 96, 16, 5, F16, F32, seed=10 * i)
+        index = indices(T, 5, "mixed", seed=i)
+        rows = rnd(9 + i, 3000 + i, seed=30 + i)
+        sets.append((x, a, b, index, scale, y, rows, ops.low_rank(x, a, b, index, scale, base=y), ops.logits(rows)))
+    torch.cuda.synchronize()
+    wrong, gate = [], threading.Barrier(2, timeout=60)
+
+    def work(s):
+        x, a, b, index, scale, y, rows, want, probs = s
+        stream = torch.cuda.Stream()
+        gate.wait()
+        with torch.cuda.stream(stream):
+            got = [(ops.low_rank(x, a, b, index, scale, base=y), ops.logits(rows)) for _ in range(50)]
+        stream.synchronize()
+        wrong.extend(1 for o, q in got if not (torch.equal(o, want) and torch.equal(q, probs)))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in sets]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 def test_logits_history_longer_than_is_counted(ops):
