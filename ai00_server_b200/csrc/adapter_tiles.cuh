@@ -44,8 +44,10 @@ __host__ __device__ constexpr int adt_out_tokens(int R, int parts) {
 __host__ __device__ constexpr int adt_operand(int R, int parts) { return parts * adt_chunks(R) * adt_out_tokens(R, parts) * 128; }
 __host__ __device__ constexpr int adt_out_smem(int R, int parts) { return adt_out_bytes(R, parts, adt_out_tokens(R, parts)); }
 
-// S of a projection between the two kernels: [part][64 ranks][place] rows of 128 bytes, then the powers of two by place
-__host__ __device__ inline size_t adt_low_bytes(int tokens, int R, int parts) { return (size_t)tokens * ((size_t)parts * adt_chunks(R) * 128 + 4); }
+// S of a projection between the two kernels: [part][64 ranks][place] rows of 128 bytes, then the powers of two by place.  Whole rows, or the next projection's
+// would not start where 16-byte accesses may (the powers of two alone take 4 bytes a token)
+__host__ __device__ constexpr size_t adt_low_bytes(int tokens, int R, int parts) { return ((size_t)tokens * ((size_t)parts * adt_chunks(R) * 128 + 4) + 127) & ~(size_t)127; }
+static_assert(adt_low_bytes(257, 8, 2) % 128 == 0 && adt_low_bytes(1021, 256, 2) % 128 == 0 && adt_low_bytes(1022, 64, 3) % 128 == 0, "rows of S on boundaries");
 
 __device__ __forceinline__ uint64_t adt_desc(uint32_t saddr) {        // K-major operand in the 128-byte swizzle: 8-row atoms of 1024 bytes
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);

@@ -61,6 +61,16 @@ def test_op_adapters_workspace():
         assert f(*bad) == capi.ERR_INVALID
 
 
+def test_op_adapters_workspace_keeps_projections_on_boundaries():
+    """What a further projection adds to the workspace is a multiple of sixteen bytes, whatever the tokens and the rank: every projection's S starts where
+    sixteen-byte accesses may."""
+    f = capi.lib().b200rwkv_op_adapters_workspace
+    for tokens in [*range(257, 1025), 1021, 4099, 65537, 1 << 20]:
+        for rank in range(1, capi.MAX_RANK + 1):
+            assert (f(tokens, 4, 2, rank) - f(tokens, 4, 1, rank)) % 16 == 0, (tokens, rank)
+        assert (f(tokens, 4, 8, 256) - f(tokens, 4, 1, 256)) % 16 == 0, tokens
+
+
 def _logits(**change):
     q = capi.Logits(struct_bytes=C.sizeof(capi.Logits), type=capi.TYPE_F32, kind=capi.PROBS, rows=2, vocab=100, logits=4096, logits_stride=100, out=8192, out_stride=100)
     for k, v in change.items():

@@ -169,6 +169,27 @@ def test_adapters_several_projections_at_once(ops, T):
         assert torch.equal(o, ops.low_rank(x, a, b, index, scale, base=y))
 
 
+@pytest.mark.parametrize("dtype,out_dtype", [(F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("T,n,how", [(257, 5, "mixed"), (258, 3, "runs"), (259, 40, "tail"), (333, 4, "runs"), (1021, 70, "tail"), (1022, 6, "mixed"), (1023, 2, "one")])
+def test_adapters_several_projections_of_ragged_prompts(ops, dtype, out_dtype, T, n, how):
+    """Token counts that are no multiples of four or sixteen, through projections of other widths and ranks in one call: the values of calls of their own, to the
+    bit.  "tail": more adapters than tokens allow tiles for all of, most tokens with one of them, the others few each."""
+    sizes = [(136, 300, 16), (256, 64, 72), (72, 8, 8), (200, 131, 40)]
+    if how == "tail":
+        index = indices(T, n, "mixed")
+        index[torch.arange(T, device="cuda") % 5 != 0] = 1
+    else:
+        index = indices(T, n, how)
+    for base in (True, False):
+        made = [make(T, K, N, R, n, dtype, out_dtype, base=base, seed=10 * i) for i, (K, N, R) in enumerate(sizes)]
+        scale = made[0][3]
+        outs = ops.low_rank([m[0] for m in made], [m[1] for m in made], [m[2] for m in made], index, scale, base=[m[4] for m in made] if base else None, out_dtype=out_dtype)
+        for o, (x, a, b, _, y) in zip(outs, made):
+            want, err = adapter_want(x, a, b, index, scale, y, out_dtype)
+            check_adapters(o, want, err)
+            assert torch.equal(o, ops.low_rank(x, a, b, index, scale, base=y, out_dtype=out_dtype))
+
+
 def test_adapters_bad_values_stay_with_their_token(ops):
     T, n = 300, 3
     for count in (20, T):
