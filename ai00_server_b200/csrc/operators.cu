@@ -163,8 +163,15 @@ void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type) {
     // fours that lie on boundaries in both buffers: rows start alike, modulo four (rows that are picked: on boundaries)
     const bool whole = p.in_stride % 4 == 0 && p.out_stride % 4 == 0;
     p.vec = (uintptr_t)p.in % (4 * size) == 0 && (uintptr_t)p.out % 16 == 0 && (whole || (!p.in_row && p.in_stride % 4 == p.out_stride % 4));
-    const int stripes = (p.V + (whole ? 0 : 3) + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
+    // places of a row's tokens: up to three more in front of rows that start off a boundary
+    int stripes = (p.V + (whole ? 0 : 3) + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
     auto tokens_of = [&](int lg) { return ((stripes - 1) >> lg) * LOGITS_STRIPE + LOGITS_STRIPE; };
+    constexpr int MOST = 512 * 64;               // places that a CTA of the widest form has
+    static_assert(LOGITS_MAX_VOCAB == MOST * LOGITS_MOST_CTAS && LOGITS_MAX_VOCAB % LOGITS_STRIPE == 0, "the widest rows fit");
+    if (tokens_of(4) > MOST) {                   // not with those in front: one token at a time
+        p.vec = 0;
+        stripes = (p.V + LOGITS_STRIPE - 1) / LOGITS_STRIPE;
+    }
     // up to 16 tokens a thread and CTAs of 512 while all rows find room at once; 32 tokens a thread beyond, sixteen CTAs and 64 tokens for the widest rows
     const int sms = sm_count();
     int threads = 512, nv = 4;

@@ -411,6 +411,25 @@ def test_logits_wider_than_shared_memory(ops):
 
 
 @pytest.mark.parametrize("kind", ["logits", "probs", "log_probs"])
+@pytest.mark.parametrize("V,stride", [(524287, 524287), (524286, 524289), (524288, 524291), (524288, 524288), (524285, 524285)])
+def test_logits_widest_rows_off_boundaries(ops, kind, V, stride):
+    """The widest vocabularies, rows that start up to three tokens behind a boundary: their last tokens are written, count in the sums and take their lists."""
+    n = 4
+    rows = torch.empty(n * stride, device="cuda").as_strided((n, V), (stride, 1))
+    rows.copy_(rnd(n, V, seed=V % 97))
+    rows[:, V - 3:] += 12.0                              # the last tokens are most of a row
+    out = torch.full((n * stride,), float("nan"), device="cuda").as_strided((n, V), (stride, 1))
+    _, controls, _, _, _, _, _ = logits_case(n, 8, F32, 0, None, 0, seed=3)
+    histories = [[V - 1, 5, V - 1], [], [V - 2, V - 1], [V - 3] * 4]
+    biases = [[(V - 1, 1.5)], [(V - 2, -2.0), (0, 3.0)], [], [(V - 1, 0.25), (V - 3, 4.0)]]
+    call(ops, rows, kind, controls, histories, None, biases, None, None, out=out)
+    want, err = logits_want(rows, kind, controls, histories, None, biases)
+    check_logits(out, want, err)
+    if stride > V:
+        assert bool(torch.as_strided(out, (n - 1, stride - V), (stride, 1), V).isnan().all())
+
+
+@pytest.mark.parametrize("kind", ["logits", "probs", "log_probs"])
 def test_logits_parts_alone(ops, kind):
     """Histories, biases and masks each without the others; no controls at all."""
     rows, controls, histories, froms, biases, masks, mask_of = logits_case(4, 5000, F32, 200, 0.4, 50, seed=5)
