@@ -11,8 +11,9 @@
 // thread and CTAs of 256 where there are many rows (512 rows of 65536: 56 us, with 16 tokens and CTAs of 512 70, with 32 and sixteen CTAs of 128 63), which settle their sums more quickly.
 // Tokens go to the CTAs in stripes of 64, so that frequent tokens that are neighbours in a vocabulary spread over all of them.
 //   * a history is added up in shared memory, a pair of words for each token of the CTA: decay^age in units of 2^-28, its lower 14 bits to one word
-//     and the others to the other, so that neither overflows (2^17 - 1 entries; of a longer history the newest count), no atomic has to answer,
-//     and their order changes nothing.  An entry that counts adds one unit at least: the words say by themselves which tokens have been said;
+//     and the others to the other, so that neither overflows 31 bits (2^17 - 1 entries; of a longer history the newest count), no atomic has to answer,
+//     and their order changes nothing.  An entry is off by half a unit at most, and one of less than that adds nothing: bit 31 of the first word then says
+//     that its token counts, as that of the second does for a token that is in the history alone;
 //   * one pass over the registers for the thread's maximum and its sum of exponentials, which are what the probabilities are made of; pairs are
 //     combined over the CTA, and over the cluster in one exchange.
 #pragma once
@@ -40,6 +41,7 @@ __device__ __forceinline__ float4 logits4(const __nv_bfloat16* p) {
 }
 
 constexpr unsigned LOGITS_SEEN = 1u << 31;        // flag in the upper word of a token that is in the history and does not count there
+constexpr unsigned LOGITS_SAID = 1u << 31;        // flag in the lower word of one that counts with less than half a unit
 
 // 2^x by the unit's instruction, good to 2^-22; what is below 2^-126 is zero.  (expf is eight instructions)
 __device__ __forceinline__ float logits_exp2(float x) {
@@ -124,7 +126,7 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
     if (hn > 0 || bn > 0) {
         // f(j, place of its token) for the entries of a list from `first` on that are among them
         auto each = [&](const int* tok, int first, int count, int s0, auto&& f) {
-            constexpr int U = 4;                     // entries in flight (96 rows of 100003 with histories of 8000: 66 us, with one 75; with eight single rows take 15 % longer)
+            constexpr int U = 4;                     // entries in flight (96 rows of 100003 with histories of 8000: 67 us, with one 75; with eight single rows take 15 % longer)
             for (int j0 = first + tid; j0 < count; j0 += TH * U) {
                 unsigned t[U];
 #pragma unroll
@@ -170,13 +172,14 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
                 const float lg = log2f(fminf(fmaxf(ctl ? ctl[3] : 1.f, 0.f), 1.f));
                 const int from = p.hist_from ? p.hist_from[row] : 0;
                 __syncthreads();
+                auto flag = [](unsigned* word, unsigned bit) {
+                    if (!(*reinterpret_cast<volatile unsigned*>(word) & bit)) atomicOr(word, bit);
+                };
                 each(p.hist + h0, max(0, hn - LOGITS_MAX_HISTORY), hn, s0, [&](int j, int i) {
-                    if (j < from) {
-                        if (!(*reinterpret_cast<volatile unsigned*>(&sums[i].y) & LOGITS_SEEN)) atomicOr(&sums[i].y, LOGITS_SEEN);
-                        return;
-                    }
+                    if (j < from) return flag(&sums[i].y, LOGITS_SEEN);
                     const int age = hn - 1 - j;
-                    const unsigned c = age == 0 ? 1u << 28 : max(1u, (unsigned)(logits_exp2(lg * (float)age) * 268435456.f + 0.5f));      // (zero decay: one unit from the second newest on)
+                    const unsigned c = age == 0 ? 1u << 28 : (unsigned)(logits_exp2(lg * (float)age) * 268435456.f + 0.5f);      // (zero decay: nothing from the second newest on)
+                    if (c == 0u) return flag(&sums[i].x, LOGITS_SAID);
                     if (c & 0x3FFFu) atomicAdd(&sums[i].x, c & 0x3FFFu);
                     if (c >> 14) atomicAdd(&sums[i].y, c >> 14);
                 });
@@ -184,8 +187,8 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
                 apply(s0, [&](float& l, uint2 a) {
                     if ((a.x | a.y) == 0u) return;
                     l = l > 0.f ? l / rep : l * rep;
-                    const unsigned up = a.y & ~LOGITS_SEEN;
-                    if (a.x | up) l -= presence + frequency * ((float)up * 0x1p-14f + (float)a.x * 0x1p-28f);
+                    const unsigned up = a.y & ~LOGITS_SEEN, low = a.x & ~LOGITS_SAID;
+                    if (a.x | up) l -= presence + frequency * ((float)up * 0x1p-14f + (float)low * 0x1p-28f);
                 });
             }
             if (bn > 0) {

@@ -514,6 +514,30 @@ def test_logits_repeats_and_the_edges_of_decay(ops):
     assert torch.equal(out[[1, 3, 4]], rows[[1, 3, 4]])
 
 
+@pytest.mark.parametrize("m", [3000, 100000])
+def test_logits_weights_that_decay_away(ops, m):
+    """One token said over and over: what has decayed away adds nothing to its weight, and counts for presence all the same.
+
+    An entry is kept in units of 2^-28: it is off by half a unit, or by itself where it is less.  Then as in logits_want."""
+    V, decays, frequency = 50, [0.0, 0.5, 0.9, 0.99, 0.999, 0.9999], 0.5
+    rows = rnd(len(decays), V, seed=31)
+    controls = torch.tensor([[1.0, 0.25, frequency, d, 1.0] for d in decays]).cuda()
+    history = [4] * 3 + [9] * m                          # (token 4 is the oldest)
+    off, flat = ragged([history] * len(decays))
+    out = ops.logits(rows, kind="logits", controls=controls, history=flat, history_offset=off).double().cpu().numpy()
+    l = rows.double().cpu().numpy()
+    for i, d in enumerate(controls[:, 3].double().tolist()):
+        age = np.arange(m + 3)
+        w = np.where(age == 0, 1.0, d ** age)
+        with np.errstate(divide="ignore"):
+            w_off = np.where(w > 0, w * 2.0 ** -22 * (2 + age * np.abs(np.log2(d))), 0) if d > 0 else 0 * w
+        w_off = w_off + np.minimum(w, 2.0 ** -29) * (age > 0)
+        for t, part in ((9, slice(0, m)), (4, slice(m, m + 3))):
+            down = 0.25 + frequency * w[part].sum()
+            bound = frequency * w_off[part].sum() + 2.0 ** -22 * down + 2.0 ** -23 * abs(l[i, t] - down)
+            assert abs(out[i, t] - (l[i, t] - down)) <= bound, (d, t, out[i, t], l[i, t] - down, bound)
+
+
 @pytest.mark.parametrize("V", [4096, 4097, 65536, 460001])
 def test_logits_strides_in_place_and_rows_behind(ops, V):
     for shift in (0, 1, 4):
