@@ -63,7 +63,7 @@ __device__ __forceinline__ void adt_fence() { asm volatile("fence.proxy.async.sh
 __device__ __forceinline__ void adt_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void adt_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t adt_swizzled(int row, int chunk) { return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4)); }
-// waits of these kernels end: a barrier that does not come within about a second makes the CTA go on without it, and what it writes NaN
+// waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and makes NaN of what hangs on it
 __device__ __forceinline__ bool adt_bar_wait(uint32_t bar, uint32_t parity) {
     if (mbar_try(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
@@ -139,7 +139,8 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
         const uint32_t st = ring + (uint32_t)slot * stage_bytes;
         unsigned pass = 0;
         for (int i = slot; i < slabs; i += ADT_STAGES, ++pass) {
-            if (pass > 0) fine = fine && adt_bar_wait(free_bar + slot * 8, (pass - 1) & 1u);
+            // (a slab that is still read is not loaded over: its barrier then does not come either, nor S)
+            if (pass > 0 && !(fine = adt_bar_wait(free_bar + slot * 8, (pass - 1) & 1u))) break;
             const int k = (i * ADP_CTAS + cta) * 64 + (me & 7) * 8;
             const bool in = k < K;
             const int kk = in ? k : 0;
@@ -158,16 +159,17 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
         const uint32_t idesc = adt_idesc<E>(128, Rn);
         for (int i = 0; i < slabs; ++i) {
             const int slot = i % ADT_STAGES;
-            fine = fine && adt_bar_wait(full + slot * 8, (uint32_t)(i / ADT_STAGES) & 1u);
+            if (!(fine = adt_bar_wait(full + slot * 8, (uint32_t)(i / ADT_STAGES) & 1u))) break;
             tc_fence_after();
             const uint32_t st = ring + (uint32_t)slot * stage_bytes;
 #pragma unroll
             for (int k = 0; k < 4; ++k) tc_mma_f16(tmem, adt_desc(st + k * 32), adt_desc(st + ADT_TOK * 128 + k * 32), idesc, i > 0 || k > 0);
             tc_commit(free_bar + slot * 8);
         }
-        tc_commit(bar_s);
+        if (fine) tc_commit(bar_s);
     }
     fine = fine && adt_bar_wait(bar_s, 0);
+    if (!fine) adt_bar_wait(bar_s, 0);               // (the slabs are not written over while another thread may still see the products end)
     __syncwarp();
     tc_fence_after();
 
@@ -185,6 +187,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = 0.f;
             }
+            if (!fine) v[0] = __int_as_float(0x7fc00000);        // (one rank of the thread's token is enough)
 #pragma unroll
             for (int j = 0; j < 16; j += 4)
                 *reinterpret_cast<float4*>(exch + row * pitch + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
@@ -245,7 +248,7 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
                     *reinterpret_cast<uint2*>(low + ((size_t)(k * adt_chunks(L) + r / 64) * p.tokens + at) * 128 + (r % 64) * 2) = h;
                 }
             }
-            if (sub == 0) *reinterpret_cast<float*>(low + (size_t)NP * adt_chunks(L) * p.tokens * 128 + (size_t)at * 4) = fine ? back : __int_as_float(0x7fc00000);
+            if (sub == 0) *reinterpret_cast<float*>(low + (size_t)NP * adt_chunks(L) * p.tokens * 128 + (size_t)at * 4) = back;
         }
     }
     // no CTA leaves while another may read its sums
@@ -452,6 +455,8 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
         float back_next = 0.f;
         if (cur.R) {
             fine = fine && adt_bar_wait(bar + (uses & 1u) * 8, (uses >> 1) & 1u);
+            if (!fine)                               // (no one reads them before all have come through the barrier below)
+                for (int i = 0; i < cur.cnt; ++i) s_back[buf][i] = __int_as_float(0x7fc00000);
             __syncwarp();
             tc_fence_after();
         }
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
             for (int i = 0; i < OWN; ++i) {
                 AdpRaw<O>::widen(y[i], w[i]);
                 if (!cur.R) continue;
-                const float back = fine ? s_back[buf][(c + t0 + i) & (ADT_TOK - 1)] : __int_as_float(0x7fc00000);
+                const float back = s_back[buf][(c + t0 + i) & (ADT_TOK - 1)];
                 const float4 x = *reinterpret_cast<const float4*>(st + (t0 + i) * ADT_PITCH + lane * 4);
                 w[i][0] = fmaf(x.x, back, w[i][0]);
                 w[i][1] = fmaf(x.y, back, w[i][1]);
