@@ -116,9 +116,10 @@ static void ready() {
 }
 
 template <typename E, typename O>
-static void apply(cudaStream_t s, const AdapterParams& p) {
+static int apply(cudaStream_t s, const AdapterParams& p) {
     constexpr int NP = AdpParts<E, O>::N;
     ready<E, O>();
+    int launched = 0;
     int groups = adapter_groups(p.tokens, p.adapters);
     if (p.plan.base) {
         const int tiles = std::min(p.plan.tiles, p.tile_least > 1 ? p.tokens / p.tile_least + p.tokens / ADP_TILE : p.plan.tiles);
@@ -130,6 +131,7 @@ static void apply(cudaStream_t s, const AdapterParams& p) {
             const size_t smem = adt_out_smem(p.rank, NP);
             const int most = sm_count() * (smem <= ADT_HALF_SM ? 2 : 1);
             launch(adapter_out_kernel<E, O>, dim3((unsigned)std::min<long long>(units, most)), ADT_THREADS, smem, s, p);
+            launched += 2;
         }
         groups = p.tile_least > 1 ? std::min(groups, (p.adapters + (p.copy ? 1 : 0)) * ((p.tile_least - 1 + ADP_TOK - 1) / ADP_TOK)) : 0;
     }
@@ -140,15 +142,19 @@ static void apply(cudaStream_t s, const AdapterParams& p) {
             if (p.finish) kern = adapter_few_kernel<E, O, false, true>;
         }
         launch(kern, dim3(ADP_CTAS * groups, p.nparts), ADP_THREADS, adapter_few_smem(p.rank, NP), s, p);
+        ++launched;
     }
+    return launched;
 }
 
 void adapters_prepare(int type, int out_type) {
     with_types(type, out_type, [](auto e, auto o) { ready<decltype(e), decltype(o)>(); });
 }
 
-void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type) {
-    with_types(type, out_type, [&](auto e, auto o) { apply<decltype(e), decltype(o)>(s, p); });
+int adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type) {
+    int launched = 0;
+    with_types(type, out_type, [&](auto e, auto o) { launched = apply<decltype(e), decltype(o)>(s, p); });
+    return launched;
 }
 
 template <typename E, int TH, int NV, bool VEC>

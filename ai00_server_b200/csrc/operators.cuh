@@ -81,8 +81,8 @@ B200_HIDDEN void adapters_shape(AdapterParams& p, void* workspace, int type, int
 B200_HIDDEN void adapters_prepare(int type, int out_type);
 // orders the tokens of a longer call by adapter; its groups serve any number of adapters_apply calls with the same tokens
 B200_HIDDEN void adapters_plan(cudaStream_t s, const AdapterParams& p);
-// the p.nparts parts of p; type: B200RWKV_TYPE_F16 / _BF16, out_type: that or _F32
-B200_HIDDEN void adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type);
+// the p.nparts parts of p; type: B200RWKV_TYPE_F16 / _BF16, out_type: that or _F32.  Kernels launched
+B200_HIDDEN int adapters_apply(cudaStream_t s, const AdapterParams& p, int type, int out_type);
 
 // ---- rows of logits ----
 constexpr int LOGITS_STRIPE = 64;                // neighbouring tokens of a CTA; the next ones are the next CTA's

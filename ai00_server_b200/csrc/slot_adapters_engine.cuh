@@ -199,8 +199,7 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
     }
     if (n == 0) return;
     p.nparts = n;
-    adapters_apply(s, p, B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
-    ++launches_last_step;
+    launches_last_step += adapters_apply(s, p, B200RWKV_TYPE_F16, B200RWKV_TYPE_F32);
     for (int i = 0; i < gp.nseg && !p.finish; ++i) {
         const GemmSeg &sg = gp.seg[i], &to = was.seg[i];
         if (g.site[i] < 0 || sg.out == to.out) continue;

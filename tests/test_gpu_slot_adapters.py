@@ -170,6 +170,36 @@ def test_binding_changes_between_calls():
         m.close()
 
 
+def test_launches_of_steps_with_adapters_are_counted():
+    """b200rwkv_launch_count of steps with adapters: one kernel for the slots' adapters, and behind each projection launch one in steps of up to 256 tokens.  Longer
+    steps order their tokens once, take three kernels behind each (sums, outputs, adapters of few tokens; 1536 tokens and more two), and one for each activation
+    (gate, channel-mix key and receptance); the head's rows are few."""
+    st = synth.make_st("tiny6", 0)
+    counts = {}
+    for adapter in (False, True):
+        m = runtime.Model(st, max_batch=8, token_chunk_size=256)
+        try:
+            for s in range(8):
+                m.state.load(m.state.init(), s)
+            if adapter:
+                m.set_adapter(1, m.load_adapter(*files("tiny6")[0]))
+
+            def launched(n, slots):
+                before = m.launch_count()
+                m.infer_raw(list(range(slots)), [n] * slots, [5] * (n * slots), [capi.OPTION_LAST] * slots)
+                return m.launch_count() - before
+
+            counts[adapter] = [launched(1, 3), launched(1, 3), launched(20, 3), launched(100, 3), launched(220, 7)]
+        finally:
+            m.close()
+    extra = [b - a for a, b in zip(counts[False], counts[True])]
+    layers, behind = m.info["num_layer"], extra[0] - 1           # projection launches with adapters, the head's among them
+    assert behind >= 4 * layers + 1
+    assert extra[1] == extra[0] and extra[2] == extra[0]
+    assert extra[3] == 2 + 3 * (behind - 1) + 3 * layers + 1
+    assert extra[4] == 2 + 2 * (behind - 1) + 3 * layers + 1
+
+
 def test_adapter_refusals():
     st = synth.make_st("tiny6", 0)
     m = runtime.Model(st, max_batch=2, token_chunk_size=32)
