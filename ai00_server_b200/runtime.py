@@ -359,6 +359,10 @@ class Model:
 
     def set_adapter(self, slot: int, adapter: Adapter | None) -> None:
         """Tokens of the slot use the adapter (None: the weights alone) from the next infer call on."""
+        if adapter is not None and adapter._model is not self:
+            raise capi.B200Error(capi.ERR_STATE, "set_adapter: the adapter belongs to another model")
+        if adapter is not None and not adapter.id:
+            raise capi.B200Error(capi.ERR_STATE, "set_adapter: the adapter was freed")
         capi.check(capi.lib().b200rwkv_slot_adapter(self._h, slot, adapter.id if adapter is not None else 0), self._h)
 
     def sample_rows(self, slots, kind: str = "probs", controls=None, history=None, history_from=None, allow=None, bias=None, out: np.ndarray | None = None):

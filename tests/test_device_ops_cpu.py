@@ -147,3 +147,19 @@ def test_engine_calls_refuse_null():
     assert lib.b200rwkv_adapter_free(None, 1) == capi.ERR_INVALID
     assert lib.b200rwkv_slot_adapter(None, 0, 1) == capi.ERR_INVALID
     assert lib.b200rwkv_sample_rows(None, 1, C.byref(capi.RowControls()), None) == capi.ERR_INVALID
+
+
+def test_a_freed_or_foreign_adapter_is_not_bound():
+    """A handle that was freed must not unbind the slot as if it were None, nor one of another model bind what has its number here."""
+    from ai00_server_b200 import runtime
+    one, other = runtime.Model.__new__(runtime.Model), runtime.Model.__new__(runtime.Model)
+    one._h = other._h = None
+    with pytest.raises(capi.B200Error, match="freed") as ei:
+        one.set_adapter(0, runtime.Adapter(one, 0))
+    assert ei.value.code == capi.ERR_STATE
+    with pytest.raises(capi.B200Error, match="another model") as ei:
+        one.set_adapter(0, runtime.Adapter(other, 3))
+    assert ei.value.code == capi.ERR_STATE
+    for adapter in (None, runtime.Adapter(one, 3)):          # what the engine itself decides
+        with pytest.raises(capi.B200Error, match="null engine"):
+            one.set_adapter(0, adapter)
