@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(TH, (NV <= 4 ? 1536 : (NV <= 8 ? 1024 : 512)) 
     // ---- mask and temperature ----
     again();
     const float temperature = ctl ? ctl[4] : 1.f;
-    // a temperature that is not a positive number makes the row NaN
-    const float scale = temperature > 0.f && temperature < INFINITY ? 1.f / temperature : __int_as_float(0x7fc00000);
+    // a temperature that is not a positive number, or has no reciprocal, makes the row NaN
+    const float over = 1.f / temperature, scale = temperature > 0.f && temperature < INFINITY && over < INFINITY ? over : __int_as_float(0x7fc00000);
     const int allow_row = p.allow ? (p.allow_row ? p.allow_row[row] : row) : -1;
     if (allow_row >= 0 && allow_row < p.allow_rows) {
         const unsigned* const allow = p.allow + (size_t)allow_row * p.words;

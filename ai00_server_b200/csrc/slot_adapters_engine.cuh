@@ -230,7 +230,7 @@ void b200rwkv_engine::sample_rows(int nrows, const b200rwkv_row_controls& q, flo
         REQUIRE(!q.bias_offset || (q.bias_offset[i] >= 0 && q.bias_offset[i] <= q.bias_offset[i + 1]), B200RWKV_ERR_INVALID, "sample_rows: bias offsets must ascend");
         if (!q.controls) continue;
         const float* c = q.controls + 5 * (size_t)i;
-        REQUIRE(c[0] > 0.f && std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]) && c[3] >= 0.f && c[3] <= 1.f && c[4] > 0.f && std::isfinite(c[4]),
+        REQUIRE(c[0] > 0.f && std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]) && c[3] >= 0.f && c[3] <= 1.f && c[4] > 0.f && std::isfinite(c[4]) && std::isfinite(1.f / c[4]),
                 B200RWKV_ERR_INVALID, "sample_rows: repetition and temperature must be positive, decay in [0, 1], presence and frequency numbers");
     }
     const size_t words = (size_t)(V + 31) / 32;

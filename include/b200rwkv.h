@@ -368,7 +368,7 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
  *     where h_j = t for some j >= history_from[i]   l -= presence + frequency * sum over those j of decay^(n - 1 - j)
  *     l += the last bias value listed for t;   l = -inf where bit t of the row's mask is 0;   l /= temperature
  * A row of which the mask leaves nothing has probabilities 0 and log-probabilities -inf; a NaN that the mask leaves makes a row of
- * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number makes any row NaN; decay is
+ * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number, or not above 2^-128, makes any row NaN; decay is
  * taken into [0, 1].  Each decay^(n - 1 - j) is rounded to a multiple of 2^-28, so that the order of a sum does not show: a weight is off by 2^-29 for each of its
  * tokens at most.  Vocabularies of up to 524288 tokens; of a history, the newest 131071 tokens.  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
  * sampler/bnf.rs:35-38, run.rs:679-681 and softmax (run.rs:1179) of the samplers that need whole rows. */

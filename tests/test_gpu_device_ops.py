@@ -496,6 +496,22 @@ def test_logits_temperature_that_is_no_number(ops):
         assert bool(out[:3].isnan().all()) and not bool(out[3].isnan().any())
 
 
+def test_logits_temperatures_at_the_ends_of_the_type(ops):
+    """Up to 2^-127 and 3e38 they are what logits are divided by; one whose reciprocal is infinite is none (zero logits would be NaN beside the infinities of
+    the others)."""
+    rows = torch.tensor([[0.0, 1.0, -2.0, 2.0 ** -126]] * 5, device="cuda")
+    temperatures = [2.0 ** -126, 3.0e38, 2.0 ** -127, 2.0 ** -128, 2.0 ** -149]
+    controls = torch.tensor([[1.0, 0, 0, 1, t] for t in temperatures]).cuda()
+    out = ops.logits(rows, kind="logits", controls=controls).double().cpu().numpy()
+    want = rows[0].double().cpu().numpy()
+    assert np.array_equal(out[0], want * 2.0 ** 126) and np.array_equal(out[2], [0.0, 2.0 ** 127, -np.inf, 2.0])
+    off = np.abs(out[1] - want / float(controls[1, 4]))
+    assert (off <= 2.0 ** -149 * (1 + np.abs(want))).all()                    # (subnormal reciprocal and results: a step of those)
+    for k in ("logits", "probs", "log_probs"):
+        res = ops.logits(rows, kind=k, controls=controls)
+        assert bool(res[3:].isnan().all()) and not bool(res[:3].isnan().any())
+
+
 def test_logits_repeats_and_the_edges_of_decay(ops):
     """One token many times (a count beyond 2^16), decay 0 (the newest token alone), 1 (a count) and beyond its range; a bias listed twice."""
     V, m = 64, 70000
