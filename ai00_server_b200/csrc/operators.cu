@@ -220,6 +220,23 @@ struct OnDevice {
     }
 };
 
+// rows of a buffer: bytes between them and of each (a row is no longer than their distance)
+struct RowSpan {
+    uintptr_t at, step, width, end;
+    RowSpan(const void* p, long long rows, long long stride, long long cols, int size)
+        : at((uintptr_t)p), step((uintptr_t)(stride * size)), width((uintptr_t)(cols * size)), end(at + (uintptr_t)(rows - 1) * step + width) {}
+    bool dense() const { return step == width || end - at == width; }
+};
+// some byte is in both, as far as can be told: rows at one distance are compared modulo it (columns of a wider buffer may lie side by side), rows without gaps
+// as a whole; of other rows nothing is said
+static bool overlap(const RowSpan& a, const RowSpan& b) {
+    if (a.at >= b.end || b.at >= a.end) return false;
+    if (a.dense() && b.dense()) return true;
+    if (a.step != b.step) return false;
+    const uintptr_t d = a.at <= b.at ? (b.at - a.at) % a.step : (a.step - (a.at - b.at) % a.step) % a.step;
+    return d < a.width || a.step - d < b.width;
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -272,10 +289,6 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
         d.K = s.in_features; d.N = s.out_features; d.R = s.rank;
         d.vec = ((uintptr_t)s.out | (uintptr_t)s.base) % (4 * osize) == 0 && s.out_stride % 4 == 0 && (!s.base || s.base_stride % 4 == 0);
         p.rank = std::max(p.rank, s.rank);
-        // (the projections of a call run side by side)
-        for (int j = 0; j < q->num_parts; ++j)
-            REQUIRE(parts[j].x != s.out && (j == i || (parts[j].out != s.out && parts[j].base != s.out)), B200RWKV_ERR_INVALID,
-                    "op_adapters: the out of a part is the x, base or out of another (or its own x)");
         REQUIRE(s.base != s.out || s.base_stride == s.out_stride || q->tokens == 1, B200RWKV_ERR_INVALID, "op_adapters: base is out, but with another stride");
         if (s.base != s.out) p.copy = 1;
     }
@@ -284,6 +297,20 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
     p.nparts = q->num_parts;
     REQUIRE(need == 0 || (q->workspace && (uintptr_t)q->workspace % 16 == 0 && q->workspace_bytes >= need), B200RWKV_ERR_INVALID,
             "op_adapters: workspace is missing, misaligned or smaller than b200rwkv_op_adapters_workspace");
+    // the projections of a call run side by side, and the tokens of each
+    for (int i = 0; i < p.nparts; ++i) {
+        const AdapterPart& s = p.part[i];
+        const RowSpan out(s.out, p.tokens, s.out_stride, s.N, osize);
+        for (int j = 0; j < p.nparts; ++j) {
+            const AdapterPart& t = p.part[j];
+            REQUIRE(!overlap(out, RowSpan(t.x, p.tokens, t.x_stride, t.K, 2)), B200RWKV_ERR_INVALID, i == j ? "op_adapters: the out of a part overlaps its own x" :
+                    "op_adapters: the out of a part overlaps the x of another");
+            REQUIRE(j == i || (!overlap(out, RowSpan(t.out, p.tokens, t.out_stride, t.N, osize)) && !(t.base && overlap(out, RowSpan(t.base, p.tokens, t.base_stride, t.N, osize)))),
+                    B200RWKV_ERR_INVALID, "op_adapters: the out of a part overlaps the base or out of another");
+        }
+        REQUIRE(!s.base || s.base == s.out || !overlap(out, RowSpan(s.base, p.tokens, s.base_stride, s.N, osize)), B200RWKV_ERR_INVALID,
+                "op_adapters: the out of a part overlaps its own base without being it");
+    }
     OnDevice on(device);
     adapters_shape(p, q->workspace, q->type, q->out_type);
     if (p.plan.base) adapters_plan((cudaStream_t)stream, p);
@@ -305,6 +332,8 @@ int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* 
     REQUIRE((uintptr_t)q->logits % size == 0 && (uintptr_t)q->out % 4 == 0, B200RWKV_ERR_INVALID, "op_logits: misaligned logits or out");
     REQUIRE((const void*)q->out != q->logits || (q->type == B200RWKV_TYPE_F32 && (q->rows == 1 || q->logits_stride == q->out_stride)), B200RWKV_ERR_INVALID,
             "op_logits: out is logits, but their rows do not lie alike");
+    REQUIRE((const void*)q->out == q->logits || !overlap(RowSpan(q->out, q->rows, q->out_stride, q->vocab, 4), RowSpan(q->logits, q->rows, q->logits_stride, q->vocab, size)),
+            B200RWKV_ERR_INVALID, "op_logits: out overlaps logits without being it");
     REQUIRE(!q->history_offset || q->history, B200RWKV_ERR_INVALID, "op_logits: history offsets without tokens");
     REQUIRE(!q->bias_offset || (q->bias_token && q->bias_value), B200RWKV_ERR_INVALID, "op_logits: bias offsets without tokens or values");
     REQUIRE(!q->allow || q->allow_rows >= (q->allow_row ? 0 : q->rows), B200RWKV_ERR_INVALID, "op_logits: fewer masks than rows");

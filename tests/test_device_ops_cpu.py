@@ -47,6 +47,41 @@ def test_op_adapters_refuses_parts_that_write_what_another_reads(change):
     assert ei.value.code == capi.ERR_INVALID
 
 
+@pytest.mark.parametrize("change,what", [
+    ({"out": 4096 + 64, "base": None}, "own x"),                                          # rows of out inside rows of x
+    ({"out": 4096 - 64, "base": None}, "own x"),
+    ({"base": 8192 + 4, "out": 8192}, "own base"),                                         # one column further
+    ({"base": 8192 + 3 * 128, "out": 8192}, "own base"),                                   # three rows further
+    ({"base": 8192, "out": 8192 + 128 - 4, "base_stride": 64, "out_stride": 64}, "own base")])
+def test_op_adapters_refuses_rows_that_overlap(change, what):
+    """Not the same rows, but some of the same bytes (x: four rows of 128 bytes at 4096; out and base: 128 bytes a row, here at distances of 128 or 256)."""
+    args = {**dict(base=12288, out=8192), **change}
+    with pytest.raises(capi.B200Error, match=what) as ei:
+        capi.check(capi.lib().b200rwkv_op_adapters(0, None, *_adapters(**args)))
+    assert ei.value.code == capi.ERR_INVALID
+
+
+@pytest.mark.parametrize("change", [{"out": 8192 + 128, "base": None}, {"base": 8192 + 384}, {"x": 8192 + 496}, {"out": 4096 + 64, "base": None}])
+def test_op_adapters_refuses_parts_that_overlap(change):
+    def part(**c):
+        return capi.AdapterPart(**{**dict(x=4096, x_stride=64, a=4096, b=4096, base=16384, base_stride=32, out=16384, out_stride=32, in_features=64, out_features=32, rank=16), **c})
+    parts = (capi.AdapterPart * 2)(part(base=8192, out=8192), part(**change))
+    q = capi.Adapters(struct_bytes=C.sizeof(capi.Adapters), type=capi.TYPE_F16, out_type=capi.TYPE_F32, tokens=4, adapters=2, num_parts=2, index=4096, scale=4096)
+    with pytest.raises(capi.B200Error, match="of another") as ei:
+        capi.check(capi.lib().b200rwkv_op_adapters(0, None, C.byref(q), parts))
+    assert ei.value.code == capi.ERR_INVALID
+
+
+@pytest.mark.parametrize("change", [
+    {"out": 4096 + 4}, {"out": 4096 + 400}, {"logits": 4096 + 796}, {"out": 4096 + 396, "logits_stride": 200, "out_stride": 200},
+    {"type": capi.TYPE_F16, "out": 4096 + 396}, {"type": capi.TYPE_BF16, "logits": 4096 + 796, "out": 4096}])
+def test_op_logits_refuses_rows_that_overlap(change):
+    """Two rows of 100 tokens: 800 bytes of f32 or 400 of f16 from 4096 on."""
+    with pytest.raises(capi.B200Error, match="overlap") as ei:
+        capi.check(capi.lib().b200rwkv_op_logits(0, None, C.byref(_logits(**{**dict(logits=4096, out=4096), **change}))))
+    assert ei.value.code == capi.ERR_INVALID
+
+
 def test_op_adapters_null_struct_and_no_tokens():
     assert capi.lib().b200rwkv_op_adapters(0, None, None, None) == capi.ERR_INVALID
     assert capi.lib().b200rwkv_op_adapters(0, None, *_adapters(tokens=0, index=None, scale=None, x=None, out=None)) == 0

@@ -169,6 +169,28 @@ def test_adapters_several_projections_at_once(ops, T):
         assert torch.equal(o, ops.low_rank(x, a, b, index, scale, base=y))
 
 
+@pytest.mark.parametrize("T", [1, 12, 301])
+def test_adapters_columns_of_one_buffer(ops, T):
+    """x and the outputs of three projections as columns side by side of one buffer, in place: what each adds is what it adds to rows of its own."""
+    n, K, widths = 5, 128, (40, 131, 64)
+    made = [make(T, K, N, 16, n, F16, F16, seed=10 * i) for i, N in enumerate(widths)]
+    index, scale, x = indices(T, n, "mixed"), made[0][3], made[0][0]
+    wide = torch.full((T + 1, K + sum(widths) + 5), 7.0, dtype=F16, device="cuda")
+    wide[:T, :K] = x
+    at = K
+    outs = []
+    for N, m in zip(widths, made):
+        outs.append(wide[:T, at:at + N])
+        outs[-1].copy_(m[4])
+        at += N
+    ops.low_rank([wide[:T, :K]] * 3, [m[1] for m in made], [m[2] for m in made], index, scale, base=outs, out=outs)
+    for o, m in zip(outs, made):
+        check_adapters(o, *adapter_want(x, m[1], m[2], index, scale, m[4], F16))
+    assert torch.equal(wide[:T, :K], x) and bool((wide[:T, at:] == 7.0).all()) and bool((wide[T] == 7.0).all())
+    with pytest.raises(capi.B200Error):
+        ops.low_rank([wide[:T, :K]] * 3, [m[1] for m in made], [m[2] for m in made], index, scale, out=[outs[0], outs[1], wide[:T, at - 65:at - 1]])
+
+
 @pytest.mark.parametrize("dtype,out_dtype", [(F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
 @pytest.mark.parametrize("T,n,how", [(257, 5, "mixed"), (258, 3, "runs"), (259, 40, "tail"), (333, 4, "runs"), (1021, 70, "tail"), (1022, 6, "mixed"), (1023, 2, "one")])
 def test_adapters_several_projections_of_ragged_prompts(ops, dtype, out_dtype, T, n, how):
