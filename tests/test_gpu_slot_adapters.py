@@ -120,6 +120,48 @@ def test_prompts_with_adapters(preset, counts):
         m.close()
 
 
+@pytest.mark.parametrize("preset", ["tiny5", "tiny6", "tiny7"])
+def test_adapters_of_one_projection_at_a_time(preset):
+    """A file that has one of the matrices alone (in all layers), at precision 1, where nothing is rounded: 1e-4 of the oracle, where an adapter that is one percent too
+    large in that projection is further off than four times that."""
+    st = synth.make_st(preset, 0)
+    base = O.parse_st(st)
+    full = O.parse_st(synth.make_lora_st(preset, rank=12, seed=5, targets=ALL))
+    m = runtime.Model(st, max_batch=4, token_chunk_size=32, exact=True)
+    rng = np.random.default_rng(8)
+    served = 0
+    try:
+        for target in (*ALL, "head"):
+            pairs = {k: v for k, v in full.items() if target in k}
+            if not pairs:
+                continue
+            served += 1
+            handle = m.load_adapter(synth.pack_st(pairs), 1.0)
+            oracle, more = (O.Oracle(with_adapter(base, pairs, alpha), "f32") for alpha in (1.0, 1.01))
+            states = [oracle.state_init() for _ in range(3)]
+            beside, off = more.state_init(), 0.0
+            for s in range(4):
+                m.state.load(m.state.init(), s)
+                m.set_adapter(s, handle if s < 3 else None)
+            for counts in ((9, 4, 1, 2), (1, 1, 1, 1), (20, 3, 30, 1)):
+                toks = [rng.integers(1, 500, size=n).tolist() for n in counts]
+                rows = m.infer_raw([0, 1, 2, 3], list(counts), sum(toks, []), [capi.OPTION_LAST] * 4)
+                for s in range(3):
+                    want, states[s] = oracle.run(toks[s], states[s])
+                    assert rel_err(rows[s], want) <= 1e-4, (target, counts, s, rel_err(rows[s], want))
+                    if s == 0:
+                        other, beside = more.run(toks[s], beside)
+                        off = max(off, rel_err(other, want))
+            assert off > 4e-4, (target, off)
+            for s in range(3):
+                assert rel_err(m.state.back(s), states[s]) <= 1e-4
+                m.set_adapter(s, None)
+            handle.free()
+    finally:
+        m.close()
+    assert served == (7 if preset == "tiny7" else 9)
+
+
 def test_slots_without_an_adapter_keep_their_results():
     st = synth.make_st("tiny6", 0)
     toks = [[3, 9, 200], [41, 7], [5]]
