@@ -3,6 +3,7 @@
 //     l = l - said(t) * presence - weight(t) * frequency                     said: it is there at or behind `history_from`,
 //                                                                            weight: sum of decay^age over those places, the newest token has age 0
 //     l = l + bias(t);  l = -inf where the row's mask forbids t;  l = l / temperature
+// (as the reference's sampler has them for a prompt; after generated tokens it decays presence too, which biases can state)
 // written as they are, as softmax or as its logarithm.  Reference: penalties sampler/nucleus.rs:49-67, mask sampler/bnf.rs:37-40, bias run.rs:679-681,
 // softmax run.rs:1179; the samplers that need whole rows are sampler/mirostat.rs:44-90 and sampler/typical.rs:70-131.
 //

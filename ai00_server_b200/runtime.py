@@ -368,7 +368,8 @@ class Model:
     def sample_rows(self, slots, kind: str = "probs", controls=None, history=None, history_from=None, allow=None, bias=None, out: np.ndarray | None = None):
         """Whole rows for samplers (b200rwkv_sample_rows): the slots' last logits rows as [n, V] "logits", "probs" or "log_probs" after
         controls [n, 5] (repetition, presence, frequency, decay, temperature), each row's token history (a list per row, oldest first; tokens
-        before history_from[i] count for repetition alone), its bias dict and its [V] mask of allowed tokens."""
+        before history_from[i] count for repetition alone), its bias dict and its [V] mask of allowed tokens.  What the history takes from a prompt's tokens is what
+        NucleusSampler.init does; for the penalties it keeps after generated tokens pass them as biases (the dict's value minus the penalty) and no history."""
         kinds = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
         if kind not in kinds:
             raise capi.B200Error(capi.ERR_INVALID, "kind must be logits, probs or log_probs")

@@ -231,7 +231,10 @@ int32_t b200rwkv_sample_topk(b200rwkv_engine*, int32_t nrows, const int32_t* slo
  * top_k): the listed slots' most recent logits rows, adjusted on the device as b200rwkv_op_logits states it and written to
  * out [nrows, num_vocab] (host memory; pinned memory of b200rwkv_host_alloc is filled at full rate) as logits, probabilities
  * or log-probabilities.  Replaces a logits copy to the host, the adjustments there and the softmax round trip (run.rs:664-697,
- * 1164-1190); penalties come from each request's token history, or, kept by the caller, as negative biases.  A slot may be listed
+ * 1164-1190).  Penalties come from each request's token history.  Those of a prompt are the sampler's own (nucleus.rs:50-59); those of generated tokens are not:
+ * the sampler decays a token's whole penalty with every token, presence included, and a token's first occurrence adds presence alone
+ * (nucleus.rs:81-123).  A caller who wants its distributions passes its map as biases, without a history: for each token the request's own bias minus the
+ * penalty (of a token listed twice the last value counts, they are not added up).  A slot may be listed
  * more than once (its row under several controls).  All arrays are host memory, in b200rwkv_op_logits' layouts.  Thread contract:
  * the softmax task's (run.rs:1237). */
 typedef struct {
@@ -370,7 +373,7 @@ int32_t b200rwkv_op_adapters(int32_t device, void* stream, const b200rwkv_adapte
  * A row of which the mask leaves nothing has probabilities 0 and log-probabilities -inf; a NaN that the mask leaves makes a row of
  * probabilities or log-probabilities NaN, a masked one does not; a temperature that is not a positive number, or not above 2^-128, makes any row NaN; decay is
  * taken into [0, 1].  Each decay^(n - 1 - j) is rounded to a multiple of 2^-28, so that the order of a sum does not show: a weight is off by 2^-29 for each of its
- * tokens at most.  Vocabularies of up to 524288 tokens; of a history, the newest 131071 tokens.  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67,
+ * tokens at most.  Vocabularies of up to 524288 tokens; of a history, the newest 131071 tokens.  Tokens of histories and bias lists outside the vocabulary are passed over.  In serving: sampler/nucleus.rs:49-67 (of a prompt; b200rwkv_sample_rows says where penalties of generated tokens differ),
  * sampler/bnf.rs:35-38, run.rs:679-681 and softmax (run.rs:1179) of the samplers that need whole rows. */
 typedef struct {
     uint32_t struct_bytes;

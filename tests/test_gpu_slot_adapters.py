@@ -345,6 +345,45 @@ def test_sample_rows(family):
         m.close()
 
 
+def test_sample_rows_with_the_penalties_of_the_sampler():
+    """Histories give NucleusSampler's distribution for a prompt; after generated tokens its map does as biases (b200rwkv_sample_topk with the map is the measure), and
+    histories give another."""
+    m = runtime.Model(synth.make_st("small6", 0), max_batch=2, token_chunk_size=32)
+    try:
+        V = m.info["num_vocab"]
+        prompt = [3, 9, 20, 9, 41, 3, 3]
+        m.state.reset(0)
+        m.infer_raw([0], [len(prompt)], prompt, [capi.OPTION_LAST], keep_on_device=True)
+        sampler = runtime.NucleusSampler(presence_penalty=0.4, frequency_penalty=0.6, penalty_decay=0.9)
+        sampler.init(prompt)
+        controls = np.array([[1.0, 0.4, 0.6, 0.9, 1.0]], np.float32)
+        own = {5: 1.5, 41: -0.5}
+        said = list(prompt)
+
+        def measure(penalties):
+            ids, probs = m.sample_topk([0], [penalties], [own])
+            return ids[0].astype(int), probs[0]
+
+        def near(row, ids, probs):
+            # probabilities of two softmax kernels over the same logits: f32 sums of V terms, penalties of a dozen roundings, logits of some ten in size
+            return np.abs(row[ids] - probs).max() <= 2.0 ** -18 * probs.max()
+
+        ids, probs = measure(sampler.penalties)
+        assert near(m.sample_rows([0], controls=controls, history=[said], bias=[own])[0], ids, probs)
+        apart = 0
+        for step in range(4):
+            token = sampler.sample_candidates(ids, probs, 0.3 + 0.1 * step)
+            said.append(token)
+            m.infer_raw([0], [1], [token], [capi.OPTION_LAST], keep_on_device=True)
+            ids, probs = measure(sampler.penalties)
+            merged = {t: own.get(t, 0.0) - float(sampler.penalties.get(t, 0.0)) for t in {*own, *sampler.penalties}}
+            assert near(m.sample_rows([0], bias=[merged])[0], ids, probs)
+            apart += not near(m.sample_rows([0], controls=controls, history=[said], bias=[own])[0], ids, probs)
+        assert apart == 4 and V > 128
+    finally:
+        m.close()
+
+
 def test_sample_rows_refusals():
     m = runtime.Model(synth.make_st("tiny6", 0), max_batch=2, token_chunk_size=32)
 
