@@ -70,7 +70,41 @@ class RowControls(C.Structure):
                 ("bias_value", C.c_void_p)]
 
 
-TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+class Draw(C.Structure):
+    """b200rwkv_draw."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("reserved", C.c_int32), ("uniform", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p)]
+
+
+class E4m3(C.Structure):
+    """b200rwkv_e4m3."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("rows", C.c_int32), ("width", C.c_int32), ("block_rows", C.c_int32), ("reserved", C.c_int32),
+                ("x", C.c_void_p), ("x_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("scale", C.c_void_p)]
+
+
+class Norm(C.Structure):
+    """b200rwkv_norm."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("residual_type", C.c_int32), ("weight_type", C.c_int32), ("out_type", C.c_int32),
+                ("rows", C.c_int32), ("width", C.c_int32), ("eps", C.c_float), ("offset", C.c_float), ("reserved", C.c_int32), ("x", C.c_void_p),
+                ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64), ("residual_out", C.c_void_p), ("residual_out_stride", C.c_int64),
+                ("weight", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("scale", C.c_void_p)]
+
+
+class LinearE4m3(C.Structure):
+    """b200rwkv_linear_e4m3."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("out_type", C.c_int32), ("tokens", C.c_int32), ("in_features", C.c_int32), ("out_features", C.c_int32),
+                ("reserved", C.c_int32), ("x", C.c_void_p), ("x_stride", C.c_int64), ("x_scale", C.c_void_p), ("w", C.c_void_p), ("w_scale", C.c_void_p),
+                ("base", C.c_void_p), ("base_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+class Sample(C.Structure):
+    """b200rwkv_sample."""
+    _fields_ = [("struct_bytes", C.c_uint32), ("type", C.c_int32), ("rows", C.c_int32), ("vocab", C.c_int32), ("logits", C.c_void_p), ("logits_stride", C.c_int64),
+                ("uniform", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("tokens", C.c_void_p),
+                ("probs", C.c_void_p)]
+
+
+TYPE_F32, TYPE_F16, TYPE_BF16, TYPE_E4M3 = 0, 1, 2, 3
 LOGITS, PROBS, LOG_PROBS = 0, 1, 2
 MAX_PARTS, MAX_RANK, MAX_ADAPTERS = 8, 256, 1024
 ADAPTERS_WITHOUT_WORKSPACE = 256          # tokens of a b200rwkv_op_adapters call that needs none
@@ -117,6 +151,7 @@ SYMBOLS = [
     ("b200rwkv_softmax", C.c_int32, [_P, C.c_int32, _P, _P]),
     ("b200rwkv_sample_topk", C.c_int32, [_P, C.c_int32, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int32, _P, _P]),
     ("b200rwkv_sample_rows", C.c_int32, [_P, C.c_int32, C.POINTER(RowControls), _P]),
+    ("b200rwkv_sample_tokens", C.c_int32, [_P, C.c_int32, C.POINTER(RowControls), C.POINTER(Draw), _P, _P]),
     ("b200rwkv_adapter_load", C.c_int32, [_P, _P, C.c_size_t, C.c_float, C.POINTER(C.c_uint64)]),
     ("b200rwkv_adapter_free", C.c_int32, [_P, C.c_uint64]),
     ("b200rwkv_slot_adapter", C.c_int32, [_P, C.c_int32, C.c_uint64]),
@@ -130,6 +165,10 @@ SYMBOLS = [
     ("b200rwkv_op_adapters_workspace", C.c_int64, [C.c_int32] * 4),
     ("b200rwkv_op_adapters", C.c_int32, [C.c_int32, _P, _P, _P]),
     ("b200rwkv_op_logits", C.c_int32, [C.c_int32, _P, _P]),
+    ("b200rwkv_op_e4m3", C.c_int32, [C.c_int32, _P, _P]),
+    ("b200rwkv_op_norm", C.c_int32, [C.c_int32, _P, _P]),
+    ("b200rwkv_op_linear_e4m3", C.c_int32, [C.c_int32, _P, _P]),
+    ("b200rwkv_op_sample", C.c_int32, [C.c_int32, _P, _P]),
     ("b200rwkv_launch_count", C.c_int32, [_P, C.POINTER(C.c_int64)]),
     ("b200rwkv_keep_hidden", C.c_int32, [_P, C.c_int32]),
     ("b200rwkv_last_hidden", C.c_int32, [_P, _P, C.c_size_t]),

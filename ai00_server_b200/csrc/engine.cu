@@ -645,7 +645,12 @@ struct b200rwkv_engine {
 
     float* sr_out = nullptr;           // device rows of sample_rows
     int sr_cap = 0;
+    void check_rows(const char* call, int nrows, const int* slots);
+    void send_pieces(const RowPieces& x, size_t room);
+    LogitsParams adjusted_rows(const char* call, int nrows, const b200rwkv_row_controls& q, RowPieces& x);
+    void adjust_rows(LogitsParams p, int nrows);
     void sample_rows(int nrows, const b200rwkv_row_controls& q, float* out);
+    void sample_tokens(int nrows, const b200rwkv_row_controls& q, const b200rwkv_draw& d, int* tokens, float* probs);
 
     std::mutex mu, sm_mu;
 
@@ -2878,6 +2883,16 @@ int32_t b200rwkv_sample_rows(b200rwkv_engine* e, int32_t nrows, const b200rwkv_r
     std::lock_guard<std::mutex> lk(e->sm_mu);
     CK(cudaSetDevice(e->dev));
     e->sample_rows(nrows, *q, out);
+    API_END
+}
+
+int32_t b200rwkv_sample_tokens(b200rwkv_engine* e, int32_t nrows, const b200rwkv_row_controls* q, const b200rwkv_draw* d, int32_t* tokens, float* probs) {
+    API_BEGIN(e)
+    REQUIRE(e && q && q->struct_bytes == sizeof(*q) && d && d->struct_bytes == sizeof(*d), B200RWKV_ERR_INVALID,
+            "sample_tokens: null engine, or struct_bytes is not sizeof(b200rwkv_row_controls) or sizeof(b200rwkv_draw)");
+    std::lock_guard<std::mutex> lk(e->sm_mu);
+    CK(cudaSetDevice(e->dev));
+    e->sample_tokens(nrows, *q, *d, tokens, probs);
     API_END
 }
 

@@ -5,6 +5,9 @@
 // the activations in launches of their own 1592).
 #pragma once
 #include "operators.cuh"
+#include "token_ops.cuh"
+
+#include <vector>
 
 namespace b200 {
 
@@ -83,5 +86,20 @@ __global__ void __launch_bounds__(256) adapter_finish_kernel(const __grid_consta
         *reinterpret_cast<uint4*>(o + a16_index(m, n, p.ldo)) = hi;
     }
 }
+
+// host arrays of a sampling call on their way to the device: places in one buffer, copied there at once
+struct RowPieces {
+    struct Piece { const void* src; size_t bytes, at; };
+    std::vector<Piece> pieces;
+    size_t total = 0;
+    size_t add(const void* src, size_t bytes) {
+        const size_t at = total;
+        if (src && bytes) {
+            pieces.push_back({src, bytes, at});
+            total = (total + bytes + 15) & ~(size_t)15;
+        }
+        return at;
+    }
+};
 
 }  // namespace b200

@@ -208,88 +208,143 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
     }
 }
 
-// rows that b200rwkv_sample_rows adjusts (logits.cuh), on the sampling stream: see sample_topk
-void b200rwkv_engine::sample_rows(int nrows, const b200rwkv_row_controls& q, float* out) {
-    REQUIRE(rank == 0, B200RWKV_ERR_INVALID, "sample_rows: only rank 0 holds the gathered logits");
-    REQUIRE(d_keep, B200RWKV_ERR_UNSUPPORTED, "sample_rows: the model keeps no logits rows");
-    REQUIRE(V <= LOGITS_MAX_VOCAB, B200RWKV_ERR_UNSUPPORTED, "sample_rows: vocabularies above 524288 are not supported");
-    REQUIRE(nrows >= 0 && nrows <= 4096 && (nrows == 0 || (q.slots && out)), B200RWKV_ERR_INVALID, "sample_rows: bad argument");
-    REQUIRE(q.kind >= B200RWKV_LOGITS && q.kind <= B200RWKV_LOG_PROBS, B200RWKV_ERR_INVALID, "sample_rows: kind must be logits, probabilities or log-probabilities");
-    if (nrows == 0) return;
-    {
-        std::lock_guard<std::mutex> lk(keep_mu);
-        for (int i = 0; i < nrows; ++i) {
-            REQUIRE(q.slots[i] >= 0 && q.slots[i] < S, B200RWKV_ERR_STATE, "sample_rows: slot out of range");
-            REQUIRE(keep_valid[q.slots[i]], B200RWKV_ERR_STATE, "sample_rows: slot " + std::to_string(q.slots[i]) + " has produced no logits row yet");
-        }
-    }
-    const int nh = q.history_offset ? q.history_offset[nrows] : 0, nb = q.bias_offset ? q.bias_offset[nrows] : 0;
-    REQUIRE(nh >= 0 && nb >= 0 && (nh == 0 || q.history) && (nb == 0 || (q.bias_token && q.bias_value)), B200RWKV_ERR_INVALID, "sample_rows: bad lists");
+// what the callers of the listed slots' rows have to get right
+void b200rwkv_engine::check_rows(const char* call, int nrows, const int* slots) {
+    auto need = [&](bool fine, int code, const std::string& what) { REQUIRE(fine, code, std::string(call) + ": " + what); };
+    need(rank == 0, B200RWKV_ERR_INVALID, "only rank 0 holds the gathered logits");
+    need(d_keep, B200RWKV_ERR_UNSUPPORTED, "the model keeps no logits rows");
+    need(V <= LOGITS_MAX_VOCAB, B200RWKV_ERR_UNSUPPORTED, "vocabularies above 524288 are not supported");
+    need(nrows >= 0 && nrows <= 4096 && (nrows == 0 || slots), B200RWKV_ERR_INVALID, "bad argument");
+    std::lock_guard<std::mutex> lk(keep_mu);
     for (int i = 0; i < nrows; ++i) {
-        REQUIRE(!q.history_offset || (q.history_offset[i] >= 0 && q.history_offset[i] <= q.history_offset[i + 1]), B200RWKV_ERR_INVALID, "sample_rows: history offsets must ascend");
-        REQUIRE(!q.bias_offset || (q.bias_offset[i] >= 0 && q.bias_offset[i] <= q.bias_offset[i + 1]), B200RWKV_ERR_INVALID, "sample_rows: bias offsets must ascend");
-        if (!q.controls) continue;
-        const float* c = q.controls + 5 * (size_t)i;
-        REQUIRE(c[0] > 0.f && std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]) && c[3] >= 0.f && c[3] <= 1.f && c[4] > 0.f && std::isfinite(c[4]) && std::isfinite(1.f / c[4]),
-                B200RWKV_ERR_INVALID, "sample_rows: repetition and temperature must be positive, decay in [0, 1], presence and frequency numbers");
+        need(slots[i] >= 0 && slots[i] < S, B200RWKV_ERR_STATE, "slot out of range");
+        need(keep_valid[slots[i]], B200RWKV_ERR_STATE, "slot " + std::to_string(slots[i]) + " has produced no logits row yet");
     }
-    const size_t words = (size_t)(V + 31) / 32;
-    struct Piece { const void* src; size_t bytes, at; };
-    std::vector<Piece> pieces;
-    size_t total = 0;
-    auto add = [&](const void* src, size_t bytes) {
-        const size_t at = total;
-        if (src && bytes) {
-            pieces.push_back({src, bytes, at});
-            total = (total + bytes + 15) & ~(size_t)15;
-        }
-        return at;
-    };
-    const size_t o_slot = add(q.slots, (size_t)nrows * 4), o_ctl = add(q.controls, (size_t)nrows * 20), o_ho = add(nh ? q.history_offset : nullptr, (size_t)(nrows + 1) * 4),
-                 o_h = add(nh ? q.history : nullptr, (size_t)nh * 4), o_hf = add(nh ? q.history_from : nullptr, (size_t)nrows * 4),
-                 o_bo = add(nb ? q.bias_offset : nullptr, (size_t)(nrows + 1) * 4), o_bt = add(nb ? q.bias_token : nullptr, (size_t)nb * 4),
-                 o_bv = add(nb ? q.bias_value : nullptr, (size_t)nb * 4), o_al = add(q.allow_bits, (size_t)nrows * words * 4);
-    if (total > tk_cap) {
+}
+
+// copies the pieces, behind the step that wrote the rows; `room` more bytes stand behind them on both sides
+void b200rwkv_engine::send_pieces(const RowPieces& x, size_t room) {
+    if (x.total + room > tk_cap) {
         if (tk_dev) { CK(cudaFree(tk_dev)); tk_dev = nullptr; }
         if (tk_host) { CK(cudaFreeHost(tk_host)); tk_host = nullptr; }
         tk_cap = 0;
-        const size_t want = std::max<size_t>(total * 2, 1 << 20);
+        const size_t want = std::max<size_t>((x.total + room) * 2, 1 << 20);
         CK(cudaMalloc(&tk_dev, want));
         CK(cudaMallocHost(&tk_host, want));
         tk_cap = want;
     }
+    for (const auto& q : x.pieces) memcpy(tk_host + q.at, q.src, q.bytes);
+    CK(cudaStreamWaitEvent(sm_stream, step_done, 0));
+    CK(cudaMemcpyAsync(tk_dev, tk_host, x.total, cudaMemcpyHostToDevice, sm_stream));
+}
+
+// the rows' adjustments: checked, and put among the pieces; the call itself once these are on their way (pointers are places until then)
+LogitsParams b200rwkv_engine::adjusted_rows(const char* call, int nrows, const b200rwkv_row_controls& q, RowPieces& x) {
+    auto need = [&](bool fine, const char* what) { REQUIRE(fine, B200RWKV_ERR_INVALID, std::string(call) + ": " + what); };
+    const int nh = q.history_offset ? q.history_offset[nrows] : 0, nb = q.bias_offset ? q.bias_offset[nrows] : 0;
+    need(nh >= 0 && nb >= 0 && (nh == 0 || q.history) && (nb == 0 || (q.bias_token && q.bias_value)), "bad lists");
+    for (int i = 0; i < nrows; ++i) {
+        need(!q.history_offset || (q.history_offset[i] >= 0 && q.history_offset[i] <= q.history_offset[i + 1]), "history offsets must ascend");
+        need(!q.bias_offset || (q.bias_offset[i] >= 0 && q.bias_offset[i] <= q.bias_offset[i + 1]), "bias offsets must ascend");
+        if (!q.controls) continue;
+        const float* c = q.controls + 5 * (size_t)i;
+        need(c[0] > 0.f && std::isfinite(c[0]) && std::isfinite(c[1]) && std::isfinite(c[2]) && c[3] >= 0.f && c[3] <= 1.f && c[4] > 0.f && std::isfinite(c[4]) && std::isfinite(1.f / c[4]),
+             "repetition and temperature must be positive, decay in [0, 1], presence and frequency numbers");
+    }
+    const size_t words = (size_t)(V + 31) / 32, row4 = (size_t)nrows * 4;
+    LogitsParams p;
+    memset(&p, 0, sizeof(p));
+    p.in = d_keep; p.in_stride = V;
+    p.out_stride = V;
+    p.V = V; p.kind = q.kind;
+    auto place = [&](auto& to, const void* src, size_t bytes) {           // (one more, so that none is null)
+        if (src && bytes) to = (std::remove_reference_t<decltype(to)>)(uintptr_t)(x.add(src, bytes) + 1);
+    };
+    place(p.in_row, q.slots, row4);
+    place(p.controls, q.controls, (size_t)nrows * 20);
+    if (nh) {
+        place(p.hist_off, q.history_offset, row4 + 4);
+        place(p.hist, q.history, (size_t)nh * 4);
+        place(p.hist_from, q.history_from, row4);
+    }
+    if (nb) {
+        place(p.bias_off, q.bias_offset, row4 + 4);
+        place(p.bias_tok, q.bias_token, (size_t)nb * 4);
+        place(p.bias_val, q.bias_value, (size_t)nb * 4);
+    }
+    if (q.allow_bits) {
+        place(p.allow, q.allow_bits, (size_t)nrows * words * 4);
+        p.words = (int)words;
+        p.allow_rows = nrows;
+    }
+    return p;
+}
+
+// into sr_out
+void b200rwkv_engine::adjust_rows(LogitsParams p, int nrows) {
     if (nrows > sr_cap) {
         if (sr_out) { CK(cudaFree(sr_out)); sr_out = nullptr; }
         sr_cap = 0;
         CK(cudaMalloc(&sr_out, (size_t)nrows * V * 4));
         sr_cap = nrows;
     }
-    for (const Piece& x : pieces) memcpy(tk_host + x.at, x.src, x.bytes);
-    CK(cudaStreamWaitEvent(sm_stream, step_done, 0));
-    CK(cudaMemcpyAsync(tk_dev, tk_host, total, cudaMemcpyHostToDevice, sm_stream));
-    LogitsParams p;
-    memset(&p, 0, sizeof(p));
-    p.in = d_keep; p.in_stride = V;
-    p.out = sr_out; p.out_stride = V;
-    p.V = V; p.kind = q.kind;
-    p.in_row = (const int*)(tk_dev + o_slot);
-    if (q.controls) p.controls = (const float*)(tk_dev + o_ctl);
-    if (nh) {
-        p.hist_off = (const int*)(tk_dev + o_ho);
-        p.hist = (const int*)(tk_dev + o_h);
-        if (q.history_from) p.hist_from = (const int*)(tk_dev + o_hf);
-    }
-    if (nb) {
-        p.bias_off = (const int*)(tk_dev + o_bo);
-        p.bias_tok = (const int*)(tk_dev + o_bt);
-        p.bias_val = (const float*)(tk_dev + o_bv);
-    }
-    if (q.allow_bits) {
-        p.allow = (const unsigned*)(tk_dev + o_al);
-        p.words = (int)words;
-        p.allow_rows = nrows;
-    }
+    p.out = sr_out;
+    auto real = [&](auto& at) {
+        if (at) at = (std::remove_reference_t<decltype(at)>)(tk_dev + (uintptr_t)at - 1);
+    };
+    real(p.in_row); real(p.controls); real(p.hist_off); real(p.hist); real(p.hist_from); real(p.bias_off); real(p.bias_tok); real(p.bias_val); real(p.allow);
     logits_rows(sm_stream, p, nrows, B200RWKV_TYPE_F32);
+}
+
+// rows that b200rwkv_sample_rows adjusts (logits.cuh), on the sampling stream: see sample_topk
+void b200rwkv_engine::sample_rows(int nrows, const b200rwkv_row_controls& q, float* out) {
+    check_rows("sample_rows", nrows, q.slots);
+    REQUIRE(nrows == 0 || out, B200RWKV_ERR_INVALID, "sample_rows: bad argument");
+    REQUIRE(q.kind >= B200RWKV_LOGITS && q.kind <= B200RWKV_LOG_PROBS, B200RWKV_ERR_INVALID, "sample_rows: kind must be logits, probabilities or log-probabilities");
+    if (nrows == 0) return;
+    RowPieces x;
+    const LogitsParams p = adjusted_rows("sample_rows", nrows, q, x);
+    send_pieces(x, 0);
+    adjust_rows(p, nrows);
     CK(cudaMemcpyAsync(out, sr_out, (size_t)nrows * V * 4, cudaMemcpyDeviceToHost, sm_stream));
     CK(cudaStreamSynchronize(sm_stream));
+}
+
+// a token for each of these rows (sample_tokens.cuh): from the kept rows themselves where nothing is to be adjusted
+void b200rwkv_engine::sample_tokens(int nrows, const b200rwkv_row_controls& q, const b200rwkv_draw& d, int* tokens, float* probs) {
+    check_rows("sample_tokens", nrows, q.slots);
+    REQUIRE(nrows == 0 || (d.uniform && tokens), B200RWKV_ERR_INVALID, "sample_tokens: null uniform or tokens_out");
+    if (nrows == 0) return;
+    for (int i = 0; i < nrows; ++i) {
+        REQUIRE(d.uniform[i] >= 0.f && d.uniform[i] < 1.f, B200RWKV_ERR_INVALID, "sample_tokens: uniform must be in [0, 1)");
+        REQUIRE(!d.temperature || (d.temperature[i] >= 0.f && std::isfinite(d.temperature[i])), B200RWKV_ERR_INVALID, "sample_tokens: temperature must not be negative");
+        REQUIRE((!d.top_p || !std::isnan(d.top_p[i])) && (!d.min_p || !std::isnan(d.min_p[i])), B200RWKV_ERR_INVALID, "sample_tokens: top_p and min_p must be numbers");
+    }
+    RowPieces x;
+    LogitsParams p = adjusted_rows("sample_tokens", nrows, q, x);
+    p.kind = LOGITS_ROWS;
+    const size_t row4 = (size_t)nrows * 4;
+    const size_t o_u = x.add(d.uniform, row4), o_t = x.add(d.temperature, row4), o_k = x.add(d.top_k, row4), o_p = x.add(d.top_p, row4), o_m = x.add(d.min_p, row4);
+    send_pieces(x, 2 * row4);
+    const bool as_they_are = !p.controls && !p.hist_off && !p.bias_off && !p.allow;
+    if (!as_they_are) adjust_rows(p, nrows);
+    DrawParams w;
+    memset(&w, 0, sizeof(w));
+    w.in = as_they_are ? d_keep : sr_out;
+    w.in_stride = V;
+    if (as_they_are) w.in_row = (const int*)(tk_dev + (uintptr_t)p.in_row - 1);
+    w.uniform = (const float*)(tk_dev + o_u);
+    if (d.temperature) w.temperature = (const float*)(tk_dev + o_t);
+    if (d.top_k) w.top_k = (const int*)(tk_dev + o_k);
+    if (d.top_p) w.top_p = (const float*)(tk_dev + o_p);
+    if (d.min_p) w.min_p = (const float*)(tk_dev + o_m);
+    w.tokens = (int*)(tk_dev + x.total);
+    w.probs = (float*)(tk_dev + x.total + row4);
+    w.V = V;
+    w.type = B200RWKV_TYPE_F32;
+    draw_rows(sm_stream, w, nrows);
+    CK(cudaMemcpyAsync(tk_host + x.total, tk_dev + x.total, 2 * row4, cudaMemcpyDeviceToHost, sm_stream));
+    CK(cudaStreamSynchronize(sm_stream));
+    memcpy(tokens, tk_host + x.total, row4);
+    if (probs) memcpy(probs, tk_host + x.total + row4, row4);
 }

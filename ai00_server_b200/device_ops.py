@@ -3,6 +3,13 @@ requests of a batch, for programs that hold theirs as torch tensors.
 
   low_rank   low-rank adapters of many requests beside shared projections
   logits     rows of logits adjusted by penalties, biases and grammar masks, as logits, probabilities or log-probabilities
+  sample     a token for each row of logits, from given random numbers
+
+and what stands in front of them in a step:
+
+  rms_norm      the residual's addition and a root-mean-square norm, with its output in 8 bits (e4m3) and a scale for every 128 columns
+  to_e4m3       rows or weights in 8 bits, with a scale for every 128 columns or every block of 128 x 128
+  linear_e4m3   products of such rows and such weights
 
 A call enqueues kernels on the current stream of its tensors' device and returns; it can be captured into a graph.  Arguments that
 do not fit raise capi.B200Error before anything is enqueued, and so do tensors that ask for a gradient: the operators serve, they have none.
@@ -15,11 +22,12 @@ import torch
 
 from . import capi
 
-_TYPE = {torch.float32: capi.TYPE_F32, torch.float16: capi.TYPE_F16, torch.bfloat16: capi.TYPE_BF16}
+_TYPE = {torch.float32: capi.TYPE_F32, torch.float16: capi.TYPE_F16, torch.bfloat16: capi.TYPE_BF16, torch.float8_e4m3fn: capi.TYPE_E4M3}
 _KIND = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
-# b200rwkv_adapter_part, b200rwkv_adapters and b200rwkv_logits as bytes: a call for a few microseconds of work has no time for a store by field
+# the structs of include/b200rwkv.h as bytes: a call for a few microseconds of work has no time for a store by field
 _PART, _ADAPTERS, _LOGITS = struct.Struct("@PqPPPqPqiiii"), struct.Struct("@IiiiiiPPPN"), struct.Struct("@IiiiiiPqPqPPPPPPPPP")
-_I32, _F32 = torch.int32, torch.float32
+_E4M3_ROWS, _NORM, _LINEAR, _SAMPLE = struct.Struct("@IiiiiiPqPqP"), struct.Struct("@IiiiiiiffiPqPqPqPPqP"), struct.Struct("@IiiiiiPqPPPPqPq"), struct.Struct("@IiiiPqPPPPPPP")
+_I32, _F32, _E4M3 = torch.int32, torch.float32, torch.float8_e4m3fn
 _stream = torch._C._cuda_getCurrentRawStream        # the current stream of a device as a number
 
 
@@ -156,3 +164,126 @@ def logits(rows, kind="probs", controls=None, history=None, history_offset=None,
     if code < 0:
         capi.check(code)
     return out
+
+
+def to_e4m3(x, rows=1, out=None, scale=None):
+    """x [n, width] (f32, f16 or bf16) in 8 bits: (out [n, width] float8_e4m3fn, scale f32) with x = out * scale, a scale for 128 neighbouring columns of a row
+    (rows=1: scale [n, ceil(width / 128)], activations) or for a block of 128 rows of them (rows=128: scale [ceil(n / 128), ceil(width / 128)], weights).
+
+    scale is the largest magnitude of its values (2^-100 at least) over 448, the largest e4m3 number."""
+    dtype, where = x.dtype, x.get_device()
+    if x.dim() != 2 or where < 0:
+        _bad("to_e4m3: x must be a [rows, width] tensor in GPU memory")
+    if rows != 1 and rows != 128:
+        _bad("to_e4m3: a scale is for 1 or 128 rows")
+    shape = x.shape
+    n, width = shape
+    scales = -(-n // rows) * -(-width // 128)
+    if out is None:
+        out = torch.empty(n, width, dtype=_E4M3, device=x.device)
+    if scale is None:
+        scale = torch.empty(-(-n // rows), -(-width // 128), dtype=_F32, device=x.device)
+    q = _E4M3_ROWS.pack(_E4M3_ROWS.size, _TYPE.get(dtype, -1), n, width, rows, 0, x.data_ptr(), _row_stride(x, "x", shape, dtype, where), out.data_ptr(),
+                        _row_stride(out, "out", shape, _E4M3, where), _list(scale, "scale", _F32, where, scales))
+    code = capi.lib().b200rwkv_op_e4m3(where, _stream(where), q)
+    if code < 0:
+        capi.check(code)
+    return out, scale
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-5, offset=0.0, out=None, scale=None, residual_out=None, out_dtype=None):
+    """h = x + residual;  residual_out = h;  y = h / sqrt(mean(h ** 2) + eps) * (offset + weight);  out, scale = y in 8 bits (to_e4m3), or out = y.
+
+    x [n, width] is f32, f16 or bf16 (width up to 32768), residual and residual_out are of that type or f32, weight [width] any of the three (None: ones).  out is
+    float8_e4m3fn with scale [n, ceil(width / 128)] f32, or, with out or out_dtype of the type of x, the rows themselves.  Sums are f32, and the norm reads h before it is
+    rounded.  residual_out may be residual or x itself.  Returns (out, scale, residual_out), None for what is not there."""
+    dtype, where = x.dtype, x.get_device()
+    if x.dim() != 2 or where < 0:
+        _bad("rms_norm: x must be a [rows, width] tensor in GPU memory")
+    shape = x.shape
+    n, width = shape
+    if out is None:
+        out = torch.empty(n, width, dtype=out_dtype or _E4M3, device=x.device)
+    o_dtype = out.dtype
+    w = s = r = ro = r_stride = ro_stride = 0
+    w_type = r_type = _TYPE.get(dtype, -1)
+    if weight is not None:
+        w, w_type = _list(weight, "weight", weight.dtype, where, width), _TYPE.get(weight.dtype, -1)
+    if o_dtype is _E4M3:
+        if scale is None:
+            scale = torch.empty(n, -(-width // 128), dtype=_F32, device=x.device)
+        s = _list(scale, "scale", _F32, where, n * -(-width // 128))
+    elif scale is not None:
+        _bad("rms_norm: scales come with an 8-bit out")
+    if residual is not None:
+        r_dtype = residual.dtype
+        if residual_out is None:
+            residual_out = torch.empty(n, width, dtype=r_dtype, device=x.device)
+        r_type = _TYPE.get(r_dtype, -1)
+        r, r_stride = residual.data_ptr(), _row_stride(residual, "residual", shape, r_dtype, where)
+        ro, ro_stride = residual_out.data_ptr(), _row_stride(residual_out, "residual_out", shape, r_dtype, where)
+    elif residual_out is not None:
+        _bad("rms_norm: residual_out comes with a residual")
+    q = _NORM.pack(_NORM.size, _TYPE.get(dtype, -1), r_type, w_type, _TYPE.get(o_dtype, -1), n, width, eps, offset, 0, x.data_ptr(), _row_stride(x, "x", shape, dtype, where),
+                   r, r_stride, ro, ro_stride, w, out.data_ptr(), _row_stride(out, "out", shape, o_dtype, where), s)
+    code = capi.lib().b200rwkv_op_norm(where, _stream(where), q)
+    if code < 0:
+        capi.check(code)
+    return out, scale, residual_out
+
+
+def linear_e4m3(x, x_scale, w, w_scale, base=None, out=None, out_dtype=None):
+    """out[t, n] = base[t, n] + sum over blocks b of 128 inputs of x_scale[t, b] * w_scale[n // 128, b] * (x[t, b] @ w[n, b]).
+
+    x [tokens, in] and w [out, in] are float8_e4m3fn as rms_norm and to_e4m3 make them (in a multiple of 16), x_scale [tokens, ceil(in / 128)] and w_scale
+    [ceil(out / 128), ceil(in / 128)] f32; base and out [tokens, out] f32, f16 or bf16 (without either: out_dtype, or bf16).  `out` may be `base`.  Sums are f32."""
+    where = x.get_device()
+    if where < 0:
+        _bad("linear_e4m3: tensors must be in GPU memory")
+    if x.dim() != 2 or w.dim() != 2:
+        _bad("linear_e4m3: x is [tokens, in], w is [out, in]")
+    tokens, k = x.shape
+    n, kw = w.shape
+    if kw != k:
+        _bad("linear_e4m3: shapes of x and w do not match")
+    if out is None:
+        out = torch.empty(tokens, n, dtype=out_dtype or (torch.bfloat16 if base is None else base.dtype), device=x.device)
+    o_dtype, blocks = out.dtype, -(-k // 128)
+    b = b_stride = 0
+    if base is not None:
+        b, b_stride = base.data_ptr(), _row_stride(base, "base", (tokens, n), o_dtype, where)
+    q = _LINEAR.pack(_LINEAR.size, _TYPE.get(o_dtype, -1), tokens, k, n, 0, x.data_ptr(), _row_stride(x, "x", (tokens, k), _E4M3, where),
+                     _list(x_scale, "x_scale", _F32, where, tokens * blocks), _list(w, "w", _E4M3, where, None), _list(w_scale, "w_scale", _F32, where, -(-n // 128) * blocks),
+                     b, b_stride, out.data_ptr(), _row_stride(out, "out", (tokens, n), o_dtype, where))
+    code = capi.lib().b200rwkv_op_linear_e4m3(where, _stream(where), q)
+    if code < 0:
+        capi.check(code)
+    return out
+
+
+def sample(rows, uniform, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None, probs=None):
+    """A token for each row of logits [n, vocab] (f32, f16 or bf16) from uniform [n] f32 in [0, 1), as (tokens [n] int32, probs [n] f32).
+
+    With w = exp((logit - largest) / temperature): kept are the row's first top_k tokens (larger logits first, of equal ones the lower id); of these the first so many that
+    their weights reach top_p of all of these; of these the ones with w >= min_p.  The token is the lowest id at which the sum of kept weights, ids ascending, exceeds uniform times all
+    of it, prob its share.  temperature, top_p, min_p [n] f32 and top_k [n] int32, None for 1 and no limits; temperature 0 takes the best token.  Logits of -inf are never drawn;
+    a row of nothing else has token -1 and prob 0, one with a NaN token -1 and prob NaN.  The result does not depend on the order of any sum."""
+    dtype, where = rows.dtype, rows.get_device()
+    if rows.dim() != 2 or where < 0:
+        _bad("sample: rows must be a [rows, vocab] tensor in GPU memory")
+    shape = rows.shape
+    n, vocab = shape
+    if tokens is None:
+        tokens = torch.empty(n, dtype=_I32, device=rows.device)
+    if probs is None:
+        probs = torch.empty(n, dtype=_F32, device=rows.device)
+    t = 0 if temperature is None else _list(temperature, "temperature", _F32, where, n)
+    k = 0 if top_k is None else _list(top_k, "top_k", _I32, where, n)
+    p = 0 if top_p is None else _list(top_p, "top_p", _F32, where, n)
+    m = 0 if min_p is None else _list(min_p, "min_p", _F32, where, n)
+    q = _SAMPLE.pack(_SAMPLE.size, _TYPE.get(dtype, -1), n, vocab, rows.data_ptr(), _row_stride(rows, "rows", shape, dtype, where), _list(uniform, "uniform", _F32, where, n),
+                     t, k, p, m, _list(tokens, "tokens", _I32, where, n), _list(probs, "probs", _F32, where, n))
+    code = capi.lib().b200rwkv_op_sample(where, _stream(where), q)
+    if code < 0:
+        capi.check(code)
+    return tokens, probs

@@ -365,14 +365,8 @@ class Model:
             raise capi.B200Error(capi.ERR_STATE, "set_adapter: the adapter was freed")
         capi.check(capi.lib().b200rwkv_slot_adapter(self._h, slot, adapter.id if adapter is not None else 0), self._h)
 
-    def sample_rows(self, slots, kind: str = "probs", controls=None, history=None, history_from=None, allow=None, bias=None, out: np.ndarray | None = None):
-        """Whole rows for samplers (b200rwkv_sample_rows): the slots' last logits rows as [n, V] "logits", "probs" or "log_probs" after
-        controls [n, 5] (repetition, presence, frequency, decay, temperature), each row's token history (a list per row, oldest first; tokens
-        before history_from[i] count for repetition alone), its bias dict and its [V] mask of allowed tokens.  What the history takes from a prompt's tokens is what
-        NucleusSampler.init does; for the penalties it keeps after generated tokens pass them as biases (the dict's value minus the penalty) and no history."""
-        kinds = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
-        if kind not in kinds:
-            raise capi.B200Error(capi.ERR_INVALID, "kind must be logits, probs or log_probs")
+    def _row_controls(self, slots, controls, history, history_from, allow, bias):
+        """(b200rwkv_row_controls, the arrays it points to) of sample_rows' arguments."""
         n, V = len(slots), self.info["num_vocab"]
         keep = {}
 
@@ -384,7 +378,7 @@ class Model:
                 setattr(q, name, keep[name].ctypes.data)
 
         q = capi.RowControls()
-        q.struct_bytes, q.kind = C.sizeof(capi.RowControls), kinds[kind]
+        q.struct_bytes = C.sizeof(capi.RowControls)
         give("slots", slots, np.int32)
         give("controls", controls, np.float32, n * 5)
         if history is not None:
@@ -402,12 +396,47 @@ class Model:
             give("bias_value", [float(v) for m in maps for v in m.values()], np.float32)
         if allow is not None:
             give("allow_bits", pack_allow(allow, n, V), np.uint32)
+        return q, keep
+
+    def sample_rows(self, slots, kind: str = "probs", controls=None, history=None, history_from=None, allow=None, bias=None, out: np.ndarray | None = None):
+        """Whole rows for samplers (b200rwkv_sample_rows): the slots' last logits rows as [n, V] "logits", "probs" or "log_probs" after
+        controls [n, 5] (repetition, presence, frequency, decay, temperature), each row's token history (a list per row, oldest first; tokens
+        before history_from[i] count for repetition alone), its bias dict and its [V] mask of allowed tokens.  What the history takes from a prompt's tokens is what
+        NucleusSampler.init does; for the penalties it keeps after generated tokens pass them as biases (the dict's value minus the penalty) and no history."""
+        kinds = {"logits": capi.LOGITS, "probs": capi.PROBS, "log_probs": capi.LOG_PROBS}
+        if kind not in kinds:
+            raise capi.B200Error(capi.ERR_INVALID, "kind must be logits, probs or log_probs")
+        n, V = len(slots), self.info["num_vocab"]
+        q, keep = self._row_controls(slots, controls, history, history_from, allow, bias)
+        q.kind = kinds[kind]
         if out is None:
             out = np.empty((n, V), np.float32)
         elif out.dtype != np.float32 or out.shape != (n, V) or not out.flags.c_contiguous:
             raise capi.B200Error(capi.ERR_INVALID, "out must be a contiguous f32 [slots, vocabulary] array")
         capi.check(capi.lib().b200rwkv_sample_rows(self._h, n, C.byref(q), out.ctypes.data), self._h)
         return out
+
+    def sample_tokens(self, slots, uniform, temperature=None, top_k=None, top_p=None, min_p=None, controls=None, history=None, history_from=None, allow=None, bias=None):
+        """A token for each of the slots, drawn on the device (b200rwkv_sample_tokens), as (tokens [n] int32, probs [n] f32): its last logits row with the adjustments of
+        sample_rows, then device_ops.sample with a uniform number in [0, 1) for each slot.  temperature, top_k, top_p, min_p: a number, or one for each slot."""
+        n = len(slots)
+        q, keep = self._row_controls(slots, controls, history, history_from, allow, bias)
+        d = capi.Draw()
+        d.struct_bytes = C.sizeof(capi.Draw)
+        for name, x, dtype in (("uniform", uniform, np.float32), ("temperature", temperature, np.float32), ("top_k", top_k, np.int32), ("top_p", top_p, np.float32),
+                               ("min_p", min_p, np.float32)):
+            if x is None:
+                continue
+            a = np.asarray(x, dtype)
+            if a.ndim == 0 and name != "uniform":
+                a = np.full(n, a, dtype)
+            if a.shape != (n,):
+                raise capi.B200Error(capi.ERR_INVALID, f"{name}: a number for each slot")
+            keep[name] = np.ascontiguousarray(a)
+            setattr(d, name, keep[name].ctypes.data)
+        tokens, probs = np.empty(n, np.int32), np.empty(n, np.float32)
+        capi.check(capi.lib().b200rwkv_sample_tokens(self._h, n, C.byref(q), C.byref(d), tokens.ctypes.data, probs.ctypes.data), self._h)
+        return tokens, probs
 
     def sample_topk(self, slots, penalties=None, bias=None, allow=None, top_k: int = 128):
         """GPU front half of sampling (b200rwkv_sample_topk): for each slot the `top_k` most probable tokens of its last

@@ -255,6 +255,23 @@ typedef struct {
 #define B200RWKV_LOG_PROBS 2
 int32_t b200rwkv_sample_rows(b200rwkv_engine*, int32_t nrows, const b200rwkv_row_controls* controls, float* out);
 
+/* A token for each of the listed slots, drawn on the device: the slots' most recent logits rows, adjusted as b200rwkv_sample_rows does it (controls->kind
+ * does not matter; without controls, history, biases and masks the rows as they are), then temperature, top-k, top-p, min-p and the draw as b200rwkv_op_sample states them.  Eight bytes a row come
+ * back in place of a row or of 128 candidates.  tokens_out [nrows]: -1 where a row leaves nothing, or holds a NaN; probs_out [nrows] or NULL: each token's share of what was kept.
+ * The host samplers of the reference cut and draw in their own orders (nucleus.rs:69-123 takes top_p before the temperature): whoever needs those stays with
+ * b200rwkv_sample_topk or b200rwkv_sample_rows.  The numbers of `draw` are host arrays of nrows each; uniform in [0, 1).  Thread contract: the softmax task's (run.rs:1237). */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t reserved;
+    const float* uniform;            /* [nrows] */
+    const float* temperature;        /* [nrows] or NULL (1): behind the controls' own; 0: the best token */
+    const int32_t* top_k;            /* [nrows] or NULL; 0: no limit */
+    const float* top_p;              /* [nrows] or NULL; 1: no limit */
+    const float* min_p;              /* [nrows] or NULL; 0: no limit */
+} b200rwkv_draw;
+int32_t b200rwkv_sample_tokens(b200rwkv_engine*, int32_t nrows, const b200rwkv_row_controls* controls, const b200rwkv_draw* draw, int32_t* tokens_out,
+                               float* probs_out);
+
 /* Adapters of requests: LoRA files that stay apart from the weights, so that the slots of a batch can have different ones
  * (b200rwkv_options.lora_st blends a file into the weights for all).  Same files: `<name>.lora.1` [out, r] and `<name>.lora.0` [in, r] in F16
  * on att.{receptance,key,value,gate,output} / ffn.{key,value,receptance} / head, r <= 256; every projection of a slot's tokens is then
@@ -315,8 +332,8 @@ int32_t b200rwkv_op_wkv(int32_t device, int32_t version, int32_t T, int32_t H, c
                         const float* g, const float* lnx_w, const float* lnx_b, float* state, float* out);
 
 /* ---- Operators on device memory --------------------------------------------------------------------------------------------
- * What the engine runs on its own buffers for the requests of a batch, for callers that hold theirs on the GPU.  All pointers
- * in the two structs are device memory of `device` (the parts array and the structs themselves are host memory, read
+ * What the engine runs on its own buffers for the requests of a batch, and what a program needs beside it, for callers that hold theirs on the GPU.  All pointers
+ * in the structs are device memory of `device` (the parts array and the structs themselves are host memory, read
  * during the call).  A call only enqueues kernels on `stream` (a cudaStream_t of that device; NULL: its default stream): it neither
  * allocates nor synchronises, can be captured into a graph, and leaves the calling thread's current device as it was.  Calls
  * on different streams may overlap; each needs its own workspace for that long, and so does every graph that may run beside
@@ -325,6 +342,7 @@ int32_t b200rwkv_op_wkv(int32_t device, int32_t version, int32_t T, int32_t H, c
 #define B200RWKV_TYPE_F32 0
 #define B200RWKV_TYPE_F16 1
 #define B200RWKV_TYPE_BF16 2
+#define B200RWKV_TYPE_E4M3 3
 
 /* Low-rank adapters of many requests beside shared projections: for every part (a projection) and token t with a = index[t]
  *     out[t, n] = base[t, n] + scale[a] * sum_r (sum_k x[t, k] A[a][r, k]) B[a][n, r]
@@ -397,6 +415,99 @@ typedef struct {
     const float* bias_value;
 } b200rwkv_logits;
 int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* args);
+
+/* Rows in 8-bit floating point.  An e4m3 number (B200RWKV_TYPE_E4M3) has a sign, four bits of exponent and three of mantissa; the largest is 448, there are no infinities.  A scale belongs to
+ * 128 neighbouring columns of a row (activations) or to a block of 128 rows by 128 columns (weights); the last of a row or column may hold fewer:
+ *     scale = max(max |x|, 2^-100) / 448,   out = x / scale, rounded to nearest
+ * so that scale times number is off by 2^-4 of the value at most, or by 2^-10 of a scale where the value is below 2^-6 of it.  A NaN stays with its number; an infinity makes its number NaN, and the scale infinite. */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t type;                /* B200RWKV_TYPE_F32, _F16, _BF16: x */
+    int32_t rows;
+    int32_t width;
+    int32_t block_rows;          /* rows that share a scale: 1 or 128 */
+    int32_t reserved;
+    const void* x;               /* [rows, width], x_stride elements apart */
+    int64_t x_stride;
+    void* out;                   /* [rows, width] bytes, out_stride apart */
+    int64_t out_stride;
+    float* scale;                /* [ceil(rows / block_rows), ceil(width / 128)] */
+} b200rwkv_e4m3;
+int32_t b200rwkv_op_e4m3(int32_t device, void* stream, const b200rwkv_e4m3* args);
+
+/* The residual's addition and a root-mean-square norm, with its output in 8 bits (a scale for 128 columns, as above) or in the type of x:
+ *     h = x + residual;   residual_out = h;   y = h / sqrt(mean(h^2) + eps) * (offset + weight);   out, scale = y in e4m3,  or  out = y
+ * h is f32: the norm reads it before it is rounded to residual_type.  Sums are f32. */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t type;                /* B200RWKV_TYPE_F32, _F16, _BF16: x */
+    int32_t residual_type;       /* `type`, or B200RWKV_TYPE_F32: residual, residual_out */
+    int32_t weight_type;         /* B200RWKV_TYPE_F32, _F16, _BF16 */
+    int32_t out_type;            /* B200RWKV_TYPE_E4M3, or `type` (then without scales) */
+    int32_t rows;
+    int32_t width;               /* up to 32768 */
+    float eps;
+    float offset;                /* 0; 1 for weights that are stored as offsets from one */
+    int32_t reserved;
+    const void* x;               /* [rows, width], x_stride elements apart, as the strides of the others are theirs */
+    int64_t x_stride;
+    const void* residual;        /* NULL: h = x */
+    int64_t residual_stride;
+    void* residual_out;          /* with residual; may be residual or x itself where their rows lie alike */
+    int64_t residual_out_stride;
+    const void* weight;          /* [width] or NULL: ones */
+    void* out;
+    int64_t out_stride;
+    float* scale;                /* [rows, ceil(width / 128)] */
+} b200rwkv_norm;
+int32_t b200rwkv_op_norm(int32_t device, void* stream, const b200rwkv_norm* args);
+
+/* Products of e4m3 rows and e4m3 weights with their scales, b counting blocks of 128 inputs:
+ *     out[t, n] = base[t, n] + sum_b x_scale[t, b] w_scale[n / 128, b] sum over k in b of x[t, k] w[n, k]
+ * Products of two numbers are exact, the sums of a block and over blocks f32; the result is rounded once to out_type. */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t out_type;            /* B200RWKV_TYPE_F32, _F16, _BF16: base, out */
+    int32_t tokens;              /* 0 .. 2^20 */
+    int32_t in_features;         /* a multiple of 16 */
+    int32_t out_features;
+    int32_t reserved;
+    const void* x;               /* [tokens, in_features], x_stride bytes apart; rows start on 16-byte boundaries */
+    int64_t x_stride;
+    const float* x_scale;        /* [tokens, ceil(in_features / 128)] */
+    const void* w;               /* [out_features, in_features] */
+    const float* w_scale;        /* [ceil(out_features / 128), ceil(in_features / 128)] */
+    const void* base;            /* [tokens, out_features], or NULL; may be `out` itself, else apart from it */
+    int64_t base_stride;
+    void* out;
+    int64_t out_stride;
+} b200rwkv_linear_e4m3;
+int32_t b200rwkv_op_linear_e4m3(int32_t device, void* stream, const b200rwkv_linear_e4m3* args);
+
+/* A token for each row of logits l from a given random number u, under the row's limits.  With m the largest logit, w_t = exp((l_t - m) / temperature), and tokens in
+ * the order of their logits (the largest first, of equal ones the lower id):
+ *     kept are the first top_k tokens; of these the first so many that their weights reach top_p times the sum of all of these; of these the ones with w_t >= min_p
+ *     token = the lowest id at which the sum of kept weights, ids ascending, exceeds u times all of it;   prob = its weight over all of it
+ * The first of the order is always kept; temperature 0 takes it alone.  u is taken into [0, 1) (1 and more: the last kept token).  top_k <= 0, top_p >= 1 and min_p <= 0 limit nothing, min_p > 1 counts as 1.
+ * Weights are whole numbers of 2^-40 (of the largest, which is 1), each off by half of that and by 2^-42 of itself at most; their sums are exact, so that a row's token does not depend on the
+ * order of anything.  Tokens that weigh less than half of 2^-40 are not drawn.  token -1, prob NaN: a NaN among the logits or the row's numbers, a temperature that is negative or infinite.  token -1, prob 0: every logit is -inf.
+ * Vocabularies of up to 524288 tokens. */
+typedef struct {
+    uint32_t struct_bytes;
+    int32_t type;                /* B200RWKV_TYPE_F32, _F16, _BF16: logits */
+    int32_t rows;
+    int32_t vocab;
+    const void* logits;          /* [rows, vocab], logits_stride elements apart */
+    int64_t logits_stride;
+    const float* uniform;        /* [rows] */
+    const float* temperature;    /* [rows] or NULL: 1 */
+    const int32_t* top_k;        /* [rows] or NULL: no limit, as for the next two */
+    const float* top_p;
+    const float* min_p;
+    int32_t* tokens;             /* [rows] */
+    float* probs;                /* [rows] or NULL */
+} b200rwkv_sample;
+int32_t b200rwkv_op_sample(int32_t device, void* stream, const b200rwkv_sample* args);
 
 /* Kernels launched by this engine's forward steps since creation (graph replays counted by their kernel nodes). */
 int32_t b200rwkv_launch_count(b200rwkv_engine*, int64_t* total);
