@@ -65,36 +65,44 @@ struct LinearCall {
         rows_map(&p.tx, q->x, q->tokens, q->in_features, q->x_stride, x_rows);
         rows_map(&p.tw, q->w, q->out_features, q->in_features, q->in_features, w_rows);
     }
+    // CTAs of a cluster, among which e4_few_kernel deals the blocks of inputs: as many as run at once, with four blocks each at least
+    template <int TT>
+    int splits() const {
+        const long long tiles = (long long)((q->out_features + 127) / 128) * ((q->tokens + TT - 1) / TT);
+        int split = 1;
+        while (split < 8 && tiles * split * 2 <= E4Few<TT>::PER_SM * sm_count() && p.kblocks >= split * 8) split *= 2;
+        return split;
+    }
     template <int TT>
     void few() {
         using C = E4Few<TT>;
-        const int tiles = (q->out_features + 127) / 128, ttiles = (q->tokens + TT - 1) / TT, room = 2 * sm_count();
-        // as many CTAs as run at once, of two blocks of inputs at least
-        int split = 1;
-        while (split < 8 && (long long)tiles * ttiles * split * 2 <= room && p.kblocks >= split * 4) split *= 2;
-        p.split = split;
+        p.split = splits<TT>();
         maps(TT, 128);
         of_type(q->out_type, [&](auto o) {
             prepare<e4_few_kernel<TT, decltype(o)>>(C::SMEM);
-            launch(e4_few_kernel<TT, decltype(o)>, dim3(tiles * split, ttiles), C::THREADS, C::SMEM, s, p, split);
+            launch(e4_few_kernel<TT, decltype(o)>, dim3((q->out_features + 127) / 128 * p.split, (q->tokens + TT - 1) / TT), C::THREADS, C::SMEM, s, p, p.split);
         });
     }
-    template <int BN>
+    long long pairs() const { return (long long)((q->tokens + 255) / 256) * ((q->out_features + E4Pair::BN - 1) / E4Pair::BN); }
     void pair() {
-        using C = E4Pair<BN>;
-        const long long units = (long long)((q->tokens + 255) / 256) * ((q->out_features + BN - 1) / BN);
-        maps(128, BN / 2);
+        using C = E4Pair;
+        maps(128, C::BN / 2);
         of_type(q->out_type, [&](auto o) {
-            prepare<e4_pair_kernel<BN, decltype(o)>>(C::SMEM);
-            launch(e4_pair_kernel<BN, decltype(o)>, dim3((unsigned)(2 * std::min<long long>(units, sm_count() / 2))), C::THREADS, C::SMEM, s, p);
+            prepare<e4_pair_kernel<decltype(o)>>(C::SMEM);
+            launch(e4_pair_kernel<decltype(o)>, dim3((unsigned)(2 * std::min<long long>(pairs(), sm_count() / 2))), C::THREADS, C::SMEM, s, p);
         });
     }
     void run() {
-        const long long pairs = (long long)((q->tokens + 255) / 256) * ((q->out_features + 255) / 256);
-        if (q->tokens > 128 && pairs * 2 >= sm_count() / 2) pair<256>();
-        else if (q->tokens <= 16) few<16>();
-        else if (q->tokens <= 32) few<32>();
-        else if (q->tokens <= 64) few<64>();
+        if (q->tokens <= 16) return few<16>();
+        if (q->tokens <= 32) return few<32>();
+        if (q->tokens <= 64) return few<64>();
+        if (q->tokens <= 128) return few<128>();
+        // Beyond, the form whose SMs go through fewer blocks of inputs, in rounds of all SMs; one of a pair's tiles takes 0.55 us, of 128 tokens and outputs 0.47.  Both, us: 333 tokens 8960 -> 2560
+        // 44 and 23, 2560 -> 8960 18 and 32; 512 tokens 4096 -> 4096 24 and 22; 1024 tokens 24 and 43; 200 tokens 4096 -> 14336 25 and 41
+        const int split = splits<128>(), sms = sm_count();
+        const long long ctas = (long long)((q->out_features + 127) / 128) * ((q->tokens + 127) / 128) * split;
+        const long long in_few = (ctas + sms - 1) / sms * ((p.kblocks + split - 1) / split), in_pairs = (pairs() + sms / 2 - 1) / (sms / 2) * p.kblocks;
+        if (in_pairs * 55 < in_few * 47) pair();
         else few<128>();
     }
 };
