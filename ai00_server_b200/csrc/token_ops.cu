@@ -109,20 +109,29 @@ struct LinearCall {
 
 // ---- tokens ----
 void draw_rows(cudaStream_t s, DrawParams p, int rows) {
-    const int size = size_of(p.type);
-    // sixteen CTAs a row while all rows find room at once, eight beyond; a thousand tokens each at least
-    int log = rows * 16 <= sm_count() || p.V > 8 * DRAW_MAX_SLICE ? 4 : 3;
-    while (log > 0 && p.V >> log < 1024) --log;
+    // a CTA for every SM that there is for a row, of a thousand tokens at least
+    const int size = size_of(p.type), sms = sm_count();
+    int log = 0;
+    while (log < 4 && (long long)rows << (log + 1) <= sms && p.V >> (log + 1) >= 1024) ++log;
+    if (p.V > DRAW_ALONE_SLICE) log = max(log, 1);
+    while (log > 0 && log < 4 && ((p.V + (1 << log) - 1) >> log) + 3 > DRAW_CLUSTER_SLICE) ++log;
     p.ctas_log = log;
     p.slice = (((p.V + (1 << log) - 1) >> log) + 3) & ~3;
-    p.vec = on(p.in, p.in_stride, size, 4 * size);
-    auto form = [&](auto th) {
-        constexpr int TH = decltype(th)::value;
-        prepare<draw_kernel<TH>>(DRAW_MAX_SLICE * 4, true);
-        launch(draw_kernel<TH>, dim3(rows << log), TH, (size_t)p.slice * 4, s, p, 1 << log);
+    const bool vec = on(p.in, p.in_stride, size, 4 * size);
+    auto form = [&](auto e, auto resident, auto aligned, auto per_sm) {
+        constexpr bool RESIDENT = decltype(resident)::value;
+        constexpr auto KERN = draw_kernel<decltype(e), DRAW_THREADS, RESIDENT, decltype(aligned)::value, decltype(per_sm)::value>;
+        prepare<KERN>(draw_smem<DRAW_THREADS, RESIDENT>(RESIDENT ? DRAW_SHARED_SLICE : DRAW_MAX_VOCAB), true);
+        launch(KERN, dim3(rows << log), DRAW_THREADS, draw_smem<DRAW_THREADS, RESIDENT>(p.slice), s, p, 1 << log);
     };
-    if ((rows << log) > sm_count() || p.slice <= 1024) form(std::integral_constant<int, 256>{});
-    else form(std::integral_constant<int, 512>{});
+    using std::integral_constant;
+    auto shape = [&](auto e, auto aligned) {
+        // (registers for two CTAs an SM spill, which many rows take for the second: 512 rows of 65536, top-p 0.9, 235 us and 273 with one; 96 rows of 100003 164 and 131)
+        if (((long long)rows << log) > sms) form(e, std::false_type{}, aligned, integral_constant<int, 2>{});
+        else if (p.slice > DRAW_SHARED_SLICE) form(e, std::false_type{}, aligned, integral_constant<int, 1>{});
+        else form(e, std::true_type{}, aligned, integral_constant<int, 1>{});
+    };
+    of_type(p.type, [&](auto e) { vec ? shape(e, std::true_type{}) : shape(e, std::false_type{}); });
 }
 
 }  // namespace b200

@@ -7,7 +7,11 @@ namespace b200 {
 
 constexpr int DRAW_MOST_CTAS = 16;
 constexpr int DRAW_MAX_VOCAB = 1 << 19;
-constexpr int DRAW_MAX_SLICE = DRAW_MAX_VOCAB / DRAW_MOST_CTAS;      // tokens of a CTA
+constexpr int DRAW_THREADS = 512;
+constexpr int DRAW_SHARED_SLICE = 40960;         // tokens of a CTA that stay in its shared memory
+constexpr int DRAW_CLUSTER_SLICE = 65535;        // tokens of a cluster's CTA: its bins hold 16 bits
+constexpr int DRAW_ALONE_SLICE = 1 << 18;          // of a CTA that has a row: its bins hold sums of 14 bits each in 32
+static_assert(DRAW_MAX_VOCAB / DRAW_MOST_CTAS <= DRAW_CLUSTER_SLICE, "the widest rows fit");
 
 struct DrawParams {
     const void* in;
@@ -21,7 +25,6 @@ struct DrawParams {
     int* tokens;
     float* probs;                    // null: not wanted
     int V, type;                     // B200RWKV_TYPE_*
-    int vec;                         // fours of a CTA's run lie on boundaries
     int ctas_log, slice;             // CTAs of a row, tokens of each (a multiple of four)
 };
 

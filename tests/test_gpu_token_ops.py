@@ -395,6 +395,48 @@ def test_tokens_that_are_equal(ops, V, dtype):
     assert best[0].tolist() == [0, 0, 0] and best[1].tolist() == [1.0, 1.0, 1.0]
 
 
+@pytest.mark.parametrize("n,V", [(150, 70001), (80, 200003), (76, 300001)])
+def test_tokens_of_wide_rows_that_are_equal(ops, n, V):
+    """More rows than pairs of SMs, so that a row is one CTA's: tens of thousands of equal tokens, in front of the end of top-p and at it."""
+    rows = (torch.randint(0, 3, (5, V), generator=torch.Generator().manual_seed(V)).cuda() * 0.5).float()
+    rows[3] = 2.0
+    rows[4] = rows[4] * 1e-3
+    rows = rows.repeat(-(-n // 5), 1)[:n].contiguous()
+    g = torch.Generator().manual_seed(n)
+    u, p, k = (torch.rand(n, generator=g) for _ in range(3))
+    kw = dict(top_p=(0.02 + 0.98 * p).cuda(), top_k=torch.where(k < 0.5, 0, (k * V).int()).to(torch.int32).cuda())
+    tokens, probs = ops.sample(rows, u.cuda(), **kw)
+    check_draws(tokens, probs, rows, u, **kw)
+
+
+@pytest.mark.parametrize("n,V", [(2, 9001), (24, 70001), (150, 20010), (80, 60000)])
+def test_tokens_where_half_are_masked(ops, n, V):
+    """Every other token, or all of a stretch, is -inf: nothing of these may reach a sum, whichever way a step takes the tokens."""
+    rows = rnd(n, V, std=1.5, seed=V)
+    rows[rnd(n, V, seed=V + 1) > 0] = -float("inf")
+    rows[:, V // 3:V // 2] = -float("inf")
+    rows[1::2, V // 4:] = torch.finfo(F32).min
+    g = torch.Generator().manual_seed(n)
+    u, p = torch.rand(n, generator=g), torch.rand(n, generator=g)
+    for kw in ({}, {"top_p": 0.5 + 0.5 * p}, {"top_p": 1 - 0.01 * p}, {"top_k": (p * V * 0.3).int() + 600}, {"top_k": (p * V * 0.3).int() + 600, "top_p": 1 - 0.1 * p}, {"min_p": 0.3 * p, "top_p": 0.9 + 0 * p}):
+        kw = {name: x.cuda() for name, x in kw.items()}
+        tokens, probs = ops.sample(rows, u.cuda(), **kw)
+        check_draws(tokens, probs, rows, u, **kw)
+
+
+@pytest.mark.parametrize("n,V", [(3, 30000), (100, 50001)])
+def test_tokens_where_the_nucleus_ends_in_the_tail(ops, n, V):
+    """top-p of nearly one, where what is behind the end is counted instead of what is in front, and flat or steep rows, where thousands of tokens lie beside it."""
+    g = torch.Generator().manual_seed(n)
+    u, p = torch.rand(n, generator=g), torch.rand(n, generator=g)
+    for std, t in ((1.0, 1.0), (3.0, 0.5), (6.0, 0.4), (0.001, 1.0), (2.0, 30.0)):
+        rows = rnd(n, V, std=std, seed=V)
+        for top_p in (1 - 10 ** -(1 + 6 * p), 0.5 + 1e-3 * (p - 0.5)):
+            kw = dict(top_p=top_p.float().cuda(), temperature=torch.full((n,), t).cuda())
+            tokens, probs = ops.sample(rows, u.cuda(), **kw)
+            check_draws(tokens, probs, rows, u, **kw)
+
+
 def test_tokens_of_rows_with_nothing_or_no_number(ops):
     V = 5000
     inf, nan = float("inf"), float("nan")
