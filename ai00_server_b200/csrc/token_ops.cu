@@ -25,12 +25,17 @@ static bool on(const void* p, long long stride, int size, int boundary) { return
 // ---- norms ----
 template <typename E, typename R>
 static void norm_form(cudaStream_t s, const NormParams& p, int rows) {
-    // few rows: a thread for every eight columns; many: sixteen or 32 columns a thread, so that an SM has several rows in flight (rows of 4096: 256 threads)
-    const int eights = (p.width + 7) / 8;
+    const int eights = (p.width + 7) / 8, pairs = ((eights + 1) / 2 + 31) / 32 * 32;
+    // more rows than CTAs that stay (2048 rows of 4096 bf16 12.8 us; a CTA a row 15.7, with 256 threads or 512)
+    if (p.vec && p.vec_out && p.width % 8 == 0 && pairs <= NORM_MANY_THREADS) {
+        const int ctas = sm_count() * (norm_many_per_sm<E, R>() * NORM_MANY_THREADS / pairs);
+        if (rows > ctas) return launch(rms_norm_kernel<E, R, 2, true>, dim3(ctas), pairs, 0, s, p);
+    }
+    // few rows: a thread for every eight columns; many: sixteen, so that an SM has several rows in flight (1024 rows of 8192 16.6 us and 19.8); wider ones what the largest CTA needs
     int nv = 1;
-    if (eights > 1024 || (rows > 2 * sm_count() && eights > 256)) nv = eights <= 512 ? 2 : (eights <= 2048 ? 4 : 8);
+    if (eights > 1024 || (rows > 2 * sm_count() && eights > 256)) nv = eights <= 1024 ? 2 : (eights <= 2048 ? 4 : 8);
     const int threads = ((eights + nv - 1) / nv + 31) / 32 * 32;
-    auto form = [&](auto n) { launch(rms_norm_kernel<E, R, decltype(n)::value>, dim3(rows), threads, 0, s, p); };
+    auto form = [&](auto n) { launch(rms_norm_kernel<E, R, decltype(n)::value, false>, dim3(rows), threads, 0, s, p); };
     if (nv == 1) form(std::integral_constant<int, 1>{});
     else if (nv == 2) form(std::integral_constant<int, 2>{});
     else if (nv == 4) form(std::integral_constant<int, 4>{});
@@ -181,7 +186,7 @@ int32_t b200rwkv_op_norm(int32_t device, void* stream, const b200rwkv_norm* q) {
     p.weight = q->weight; p.weight_type = q->weight_type;
     p.out = q->out; p.out_stride = q->out_stride;
     p.scale = eight ? q->scale : nullptr;
-    p.width = q->width; p.groups = groups;
+    p.rows = q->rows; p.width = q->width; p.groups = groups;
     p.eps = q->eps; p.offset = q->offset;
     p.vec = on(q->x, q->x_stride, size, 16) && (uintptr_t)q->weight % 16 == 0 &&
             (!q->residual || (on(q->residual, q->residual_stride, rsize, 16) && on(q->residual_out, q->residual_out_stride, rsize, 16)));
@@ -210,9 +215,10 @@ int32_t b200rwkv_op_e4m3(int32_t device, void* stream, const b200rwkv_e4m3* q) {
     const long long units = blocks * groups;
     const RowSpan x(q->x, q->rows, q->x_stride, q->width, size), out(q->out, q->rows, q->out_stride, q->width, 1), scale(q->scale, 1, units, units, 4);
     REQUIRE(!overlap(out, x) && !overlap(scale, x) && !overlap(scale, out), B200RWKV_ERR_INVALID, "op_e4m3: x, out and scale overlap");
-    const long long ctas = q->block_rows == 1 ? (units * 16 + E4_THREADS * E4_UNITS - 1) / (E4_THREADS * E4_UNITS) : units;
+    const long long ctas = q->block_rows == 1 ? (units * E4_PER_ROW + E4_THREADS - 1) / E4_THREADS : units;
     REQUIRE(ctas <= 0x7FFFFFFFll, B200RWKV_ERR_UNSUPPORTED, "op_e4m3: too many values for one call");
-    E4Params p{q->x, q->x_stride, (uint8_t*)q->out, q->out_stride, q->scale, q->rows, q->width, groups, on(q->x, q->x_stride, size, 16) && on(q->out, q->out_stride, 1, 8)};
+    E4Params p{q->x, q->x_stride, (uint8_t*)q->out, q->out_stride, q->scale, q->rows, q->width, groups, 0};
+    if (on(q->x, q->x_stride, size, 16) && on(q->out, q->out_stride, 1, 8)) p.vec = on(q->out, q->out_stride, 1, 16) ? 2 : 1;
     OnDevice here(device);
     of_type(q->type, [&](auto e) {
         launch(q->block_rows == 1 ? e4_rows_kernel<decltype(e)> : e4_blocks_kernel<decltype(e)>, dim3((unsigned)ctas), E4_THREADS, 0, (cudaStream_t)stream, p);

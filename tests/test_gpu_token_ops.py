@@ -177,6 +177,23 @@ def test_norm_offset_in_place_and_strides(ops, dtype, res, n):
             assert torch.equal(wide_x[keep], before_x[keep])
 
 
+@pytest.mark.parametrize("dtype,res,weight,out", [(F32, F32, F32, E4M3), (F32, None, None, F32), (F16, F32, F16, F16), (BF16, BF16, BF16, E4M3), (BF16, None, F32, E4M3), (F16, F32, BF16, E4M3)])
+@pytest.mark.parametrize("n,w", [(7301, 8), (5000, 136), (4000, 1000), (2001, 2560), (1100, 4096)])
+def test_norm_of_more_rows_than_stay_on_the_gpu(ops, dtype, res, weight, out, n, w):
+    """CTAs take several rows one after another: each row as if it were alone, its residual in place."""
+    x = rnd(n, w, std=2.0, dtype=dtype, seed=w)
+    r = rnd(n, w, std=5.0, dtype=res, seed=w + 1) if res else None
+    g = (1 + rnd(w, std=0.3, seed=2)).to(weight) if weight else None
+    got = ops.rms_norm(x, g, residual=r, eps=1e-5, offset=0.25, out_dtype=out)
+    check_norm(ops, x, g, r, 1e-5, 0.25, out, got)
+    few = ops.rms_norm(x[-3:], g, residual=None if r is None else r[-3:], eps=1e-5, offset=0.25, out_dtype=out)
+    if r is not None:
+        assert torch.equal(few[2], got[2][-3:])
+        again = r.clone()
+        ops.rms_norm(x, g, residual=again, eps=1e-5, offset=0.25, out_dtype=out, residual_out=again)
+        assert torch.equal(again, got[2])
+
+
 def test_norm_rows_that_are_zero_or_no_number(ops):
     x = rnd(4, 300, seed=1)
     x[1] = 0.0
