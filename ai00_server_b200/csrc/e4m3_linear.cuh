@@ -112,8 +112,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 e4l_round<__nv_bfloat16>(fl
 // ---- few tokens: the weights' bytes are what a call costs ----
 // 128 weight rows are the rows of the accumulator (a lane an output), up to TT tokens its columns; a cluster of `split` CTAs deals the blocks of inputs among
 // itself, so that all SMs stream weights, and adds its sums in the order of its CTAs: CTA r finishes tokens r, r + split, ...
-// Measured: 16 tokens 4096 -> 14336 14.5 us (58.7 MB of weights: 4.1 TB/s; the start and the end of a launch are 4 of them), 8192 -> 65536 99 us (5.4 TB/s), one token 2560 -> 2560 6;
-// 128 tokens 4096 -> 14336 23, 333 tokens 8960 -> 2560 23.  Clusters of five to seven CTAs leave SMs idle (22 us for 14.5); a request for the weights in L2 ahead of the wait for the kernel in
+// Measured: 16 tokens 4096 -> 14336 14.2 us (58.7 MB of weights: 4.1 TB/s; the start and the end of a launch are 4 of them), 8192 -> 65536 99 us (5.4 TB/s), one token 2560 -> 2560 6;
+// 32 tokens 4096 -> 14336 16, 64 tokens 18, 333 tokens 8960 -> 2560 24.  Of those 24, loads alone take 15.5 and loads with products 21: 32 KB a block of inputs come in and are read by the
+// products at 128 bytes a cycle.  Clusters of five to seven CTAs leave SMs idle (22 us for 14.5); a request for the weights in L2 ahead of the wait for the kernel in
 // front lost (16 to 17 us).
 template <int TT>
 struct E4Few {
@@ -122,7 +123,7 @@ struct E4Few {
     static constexpr int PER_SM = TT <= 32 ? 4 : (TT == 64 ? 2 : 1);              // CTAs
     static constexpr int W_BYTES = 128 * E4L_KB, STAGE = W_BYTES + TT * E4L_KB, STAGES = TT <= 32 ? 2 : (TT == 64 ? 4 : 6);
     static constexpr int BUFS = 4, COLUMNS = BUFS * TT < 32 ? 32 : BUFS * TT;      // 64 .. 256
-    static constexpr int CHUNK = TT <= 32 ? 32 : 16;             // blocks of inputs whose scales lie in shared memory at a time
+    static constexpr int CHUNK = TT <= 16 ? 32 : 16;             // blocks of inputs whose scales lie in shared memory at a time
     static constexpr int SCALES = STAGES * STAGE, BARS = SCALES + CHUNK * TT * 4, SMEM = BARS + (2 * STAGES + 2 * BUFS) * 8 + 16 + 1024;
     static_assert(TT * 128 * 4 <= STAGES * STAGE, "the sums of a CTA fit where the operands were");
     static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024 && PER_SM * COLUMNS <= 512, "CTAs of an SM");
@@ -195,13 +196,14 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
         // took 8 000 cycles)
         constexpr int THREADS = C::EPI * 32, NS = TT * C::CHUNK / THREADS;
         const int sj = tid % C::CHUNK, st = tid / C::CHUNK;
-        const float* const xs = p.xs + (size_t)(t0 + st) * p.kblocks + b0 + sj;
-        const float* const ws = p.ws + (size_t)tile * p.kblocks + b0 + sj;
+        const float* const xs = p.xs + (size_t)t0 * p.kblocks + b0;
+        const float* const ws = p.ws + (size_t)tile * p.kblocks + b0;
         float sx[NS], sw = 0.f;
-        auto ask = [&](int i) {
-            sw = i + sj < nb ? ws[i] : 0.f;
+        auto ask = [&](int i) {                              // (blocks and tokens that are not there read the last ones': loads under conditions of their own take as long as one after the other)
+            const int at = min(i + sj, nb - 1);
+            sw = ws[at];
 #pragma unroll
-            for (int k = 0; k < NS; ++k) sx[k] = i + sj < nb && st + k * (THREADS / C::CHUNK) < nt ? xs[(size_t)k * (THREADS / C::CHUNK) * p.kblocks + i] : 0.f;
+            for (int k = 0; k < NS; ++k) sx[k] = xs[(size_t)min(st + k * (THREADS / C::CHUNK), nt - 1) * p.kblocks + at];
         };
         ask(0);
         unsigned b = 0, bphase = 0;
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
     if (warp < C::EPI) {
         const int n = tile * 128 + (tid & 127);
         O* const out = reinterpret_cast<O*>(p.out) + n;
-        const O* const base = p.base ? reinterpret_cast<const O*>(p.base) + n : nullptr;
+        const O* const base = p.base ? reinterpret_cast<const O*>(p.base) + min(n, p.N - 1) : nullptr;
         unsigned bad = 0;
         for (int c = 0; c < split; ++c) {
             unsigned x;
@@ -264,7 +266,7 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
             bad |= x;
         }
         // several tokens at a time: their parts are on their way from the other CTAs together (one after the other, 32 tokens of two CTAs took 10 us)
-        constexpr int EVERY = C::EPI / 4, BATCH = TT <= 32 ? 4 : 8;
+        constexpr int EVERY = C::EPI / 4, BATCH = TT <= 32 ? 4 : 16;
         const int step = split * EVERY;
         for (int tb = rank * EVERY + (warp >> 2); tb < nt; tb += step * BATCH) {
             float v[BATCH];
@@ -272,7 +274,11 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
                 v[j] = bad ? __int_as_float(0x7fc00000) : 0.f;
-                old[j] = base && n < p.N && tb + j * step < nt ? base[(size_t)(t0 + tb + j * step) * p.base_stride] : e4l_round<O>(0.f);
+                old[j] = e4l_round<O>(0.f);
+            }
+            if (base) {
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) old[j] = base[(size_t)(t0 + min(tb + j * step, nt - 1)) * p.base_stride];
             }
             const uint32_t at = smem_u32(sums + tb * 128 + (tid & 127));
 #pragma unroll 2
@@ -301,9 +307,10 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
 // SM for 128 inputs, where one SM alone would take in 48 KB for the same products.  A lane is a token, so that a thread has one factor for all of its columns in a block
 // of inputs.  Persistent clusters walk the tiles, tokens first, so that those that run together share weights in L2.
 // What bounds it: a block of inputs is 512 cycles of the tensor cores and 1 000 of the eight warps that scale its sums, a chain of a wait, four reads of tensor memory and their
-// multiply-adds (without scales, a whole k range summed in tensor memory, 2048 tokens 4096 -> 14336 take 108 us in place of 133).  Those warps have 224 registers, so that a read is in flight
+// multiply-adds (without scales, a whole k range summed in tensor memory, 2048 tokens 4096 -> 14336 took 108 us where these took 133).  Those warps have 224 registers, so that a read is in flight
 // beside each quarter's multiply-adds; scales come through shared memory by warps of their own; sums leave through shared memory.
-// Measured: 2048 tokens 4096 -> 14336 133 us, 1.8 PFLOP/s (151 on normal values, where the power limit shows), 4096 tokens 8192 -> 8192 261 us, 2.1 PFLOP/s.
+// Measured: 2048 tokens 4096 -> 14336 118 to 140 us, 1.7 to 2.0 PFLOP/s (140 behind other work, where the power limit shows), with a base 133, to 14337 outputs with a base 166;
+// 4096 tokens 8192 -> 8192 238 us, 2.3 PFLOP/s; 256 tokens 192 -> 75776 19 us, with a base 26.
 // Tried: sixteen warps for the sums (146 us), a read ahead over the ends of blocks (140: registers spill, and spilled ones are waited for at every arrival), tiles of 128 outputs (160), the
 // last tiles of a launch in halves and quarters (133).
 struct E4Pair {
@@ -460,6 +467,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
         bool fine = true;
         for (int u = u0; u < units; u += step) {
             const int n0 = u / ttiles * BN + half * C::MINE;
+            const int tw = u % ttiles * 256 + rank * 128 + (warp & 3) * 32, rows = min(32, p.tokens - tw);
+            // base of the tile to L2, a token's columns a lane, while its products are summed
+            if (p.base && lane < rows) {
+                const char* const at = reinterpret_cast<const char*>(reinterpret_cast<const O*>(p.base) + (size_t)(tw + lane) * p.base_stride + n0);
+                const int bytes = min(C::MINE, p.N - n0) * (int)sizeof(O);
+                for (int i = 0; i < bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + i));
+            }
             f32x2 acc[C::MINE / 2];
 #pragma unroll
             for (int c = 0; c < C::MINE / 2; ++c) acc[c] = 0ull;
@@ -497,7 +511,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
             // out through the warp's piece of shared memory, 128 bytes of its 32 tokens at a time, so that accesses to base and out are runs of 128 bytes
             constexpr int PER = 16 / (int)sizeof(O), COLS = PER * 8;
             uint8_t* const mine = ring_p + C::OUT + warp * (32 * C::PITCH);
-            const int tw = u % ttiles * 256 + rank * 128 + (warp & 3) * 32, rows = min(32, p.tokens - tw);
 #pragma unroll
             for (int c0 = 0; c0 < C::MINE; c0 += COLS) {
                 const int cols = min(COLS, p.N - n0 - c0);
@@ -505,21 +518,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                 O* const out = reinterpret_cast<O*>(p.out) + (size_t)tw * p.out_stride + n0 + c0;
                 const O* const base = p.base ? reinterpret_cast<const O*>(p.base) + (size_t)tw * p.base_stride + n0 + c0 : nullptr;
                 const int r4 = lane >> 3, c8 = (lane & 7) * PER;
+                // (rows and columns that are not there read the last ones': loads under a condition of their own each take as long as one after the other)
                 if (base) {
-                    if (p.vec) {
+                    const int whole = p.vec ? cols / PER * PER : 0;
+                    if (whole) {
                         uint4 w[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (k * 4 + r4 < rows && c8 + PER <= cols) w[k] = *reinterpret_cast<const uint4*>(base + (size_t)(k * 4 + r4) * p.base_stride + c8);
+                        for (int k = 0; k < 8; ++k) w[k] = *reinterpret_cast<const uint4*>(base + (size_t)min(k * 4 + r4, rows - 1) * p.base_stride + min(c8, whole - PER));
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            if (k * 4 + r4 < rows && c8 + PER <= cols) *reinterpret_cast<uint4*>(mine + (k * 4 + r4) * C::PITCH + (lane & 7) * 16) = w[k];
+                        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(mine + (k * 4 + r4) * C::PITCH + (lane & 7) * 16) = w[k];
+                        __syncwarp();
                     }
-                    // (where rows start off boundaries, and what is left of a row)
-                    const int from = p.vec ? cols / PER * PER : 0;
-                    if (from < cols)
-                        for (int r = 0; r < rows; ++r)
-                            for (int e = from + lane; e < cols; e += 32) reinterpret_cast<O*>(mine + r * C::PITCH)[e] = base[(size_t)r * p.base_stride + e];
+                    // where rows start off boundaries, and what is left of a row: a lane a column
+                    for (int e0 = whole; e0 < cols; e0 += 32) {
+                        const int e = min(e0 + lane, cols - 1);
+                        O w[32];
+#pragma unroll
+                        for (int r = 0; r < 32; ++r) w[r] = base[(size_t)min(r, rows - 1) * p.base_stride + e];
+#pragma unroll
+                        for (int r = 0; r < 32; ++r) reinterpret_cast<O*>(mine + r * C::PITCH)[e] = w[r];
+                    }
                     __syncwarp();
                 }
 #pragma unroll
@@ -552,10 +570,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                         if (k * 4 + r4 < rows && c8 + PER <= cols)
                             *reinterpret_cast<uint4*>(out + (size_t)(k * 4 + r4) * p.out_stride + c8) = *reinterpret_cast<const uint4*>(mine + (k * 4 + r4) * C::PITCH + (lane & 7) * 16);
                 }
-                const int from = p.vec ? cols / PER * PER : 0;
-                if (from < cols)
-                    for (int r = 0; r < rows; ++r)
-                        for (int e = from + lane; e < cols; e += 32) out[(size_t)r * p.out_stride + e] = reinterpret_cast<const O*>(mine + r * C::PITCH)[e];
+                for (int e = (p.vec ? cols / PER * PER : 0) + lane; e < cols; e += 32) {
+#pragma unroll
+                    for (int r = 0; r < 32; ++r)
+                        if (r < rows) out[(size_t)r * p.out_stride + e] = reinterpret_cast<const O*>(mine + r * C::PITCH)[e];
+                }
                 __syncwarp();
             }
         }

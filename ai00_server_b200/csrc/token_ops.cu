@@ -101,13 +101,13 @@ struct LinearCall {
         if (q->tokens <= 16) return few<16>();
         if (q->tokens <= 32) return few<32>();
         if (q->tokens <= 64) return few<64>();
-        if (q->tokens <= 128) return few<128>();
-        // Beyond, the form whose SMs go through fewer blocks of inputs, in rounds of all SMs; one of a pair's tiles takes 0.55 us, of 128 tokens and outputs 0.47.  Both, us: 333 tokens 8960 -> 2560
-        // 44 and 23, 2560 -> 8960 18 and 32; 512 tokens 4096 -> 4096 24 and 22; 1024 tokens 24 and 43; 200 tokens 4096 -> 14336 25 and 41
+        // Beyond, the form that is through earlier, in rounds of all SMs: of a pair's tile a block of inputs takes 0.45 us, its ends 2.7, and a launch 4.6; of 128 tokens and outputs 0.47 and, with
+        // CTAs that come and go, 7.  Both, us: 333 tokens 8960 -> 2560 44 and 23, 2560 -> 8960 18 and 32; 512 tokens 4096 -> 4096 24 and 22; 1024 tokens 24 and 43; 200 tokens
+        // 4096 -> 14336 25 and 41; 128 tokens 25 and 23, 192 -> 75776 21 and 39
         const int split = splits<128>(), sms = sm_count();
         const long long ctas = (long long)((q->out_features + 127) / 128) * ((q->tokens + 127) / 128) * split;
-        const long long in_few = (ctas + sms - 1) / sms * ((p.kblocks + split - 1) / split), in_pairs = (pairs() + sms / 2 - 1) / (sms / 2) * p.kblocks;
-        if (in_pairs * 55 < in_few * 47) pair();
+        const long long in_few = (ctas + sms - 1) / sms * ((p.kblocks + split - 1) / split * 47 + 700), in_pairs = (pairs() + sms / 2 - 1) / (sms / 2) * (p.kblocks * 45 + 270) + 460;
+        if (in_pairs < in_few) pair();
         else few<128>();
     }
 };

@@ -310,6 +310,26 @@ def test_linear_no_tokens_and_far_rows(ops):
     check_linear(out.contiguous(), x, xs, w, ws, None)
 
 
+@pytest.mark.parametrize("T,K,N,out", [(133, 192, 61143, BF16), (128, 144, 75777, F16), (300, 272, 20001, F32), (257, 128, 19009, BF16), (700, 1040, 9999, F16)])
+def test_linear_of_many_outputs_and_few_inputs(ops, T, K, N, out):
+    """Tiles whose ends cost more than their products: rows of base and out that start off boundaries, the base in place, part of a wider buffer."""
+    x, xs = e4m3_of(rnd(T, K, seed=1), 1)
+    w, ws = e4m3_of(rnd(N, K, std=K ** -0.5, seed=2), 128)
+    wide = rnd(T + 1, N + 3, dtype=out, seed=3)
+    before, part = wide.clone(), wide[:T, 1:1 + N]
+    exact = (x.double() * spread(xs, 1, x.shape)) @ (w.double() * spread(ws, 128, w.shape)).T
+    most = (x.double() * spread(xs, 1, x.shape)).abs() @ (w.double() * spread(ws, 128, w.shape)).abs().T
+    ops.linear_e4m3(x, xs, w, ws, base=part, out=part)
+    want = exact + before[:T, 1:1 + N].double()
+    # (the steps' bound of the head of this file for up to nine blocks of inputs, the addition of the base, the rounding of what comes out)
+    bound = most * 9 * 2.0 ** -20 + want.abs() * (2.0 ** -23 + torch.finfo(out).eps / 2) + torch.finfo(out).smallest_normal * torch.finfo(out).eps
+    assert bool(((part.double() - want).abs() <= bound).all())
+    wide[:T, 1:1 + N] = before[:T, 1:1 + N]
+    assert torch.equal(wide, before)
+    plain = ops.linear_e4m3(x, xs, w, ws, out_dtype=out)
+    assert bool(((plain.double() - exact).abs() <= most * 9 * 2.0 ** -20 + exact.abs() * torch.finfo(out).eps / 2 + torch.finfo(out).smallest_normal * torch.finfo(out).eps).all())
+
+
 # ---- sample ---------------------------------------------------------------------------------------------------------------------------------
 def draw_want(logits, u, temperature, top_k, top_p, min_p):
     """(token, share) of a row, from the definition."""
