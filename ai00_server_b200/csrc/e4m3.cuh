@@ -7,9 +7,11 @@
 // Bound: memory, each value read once and written once, as far as the instructions let it: two divisions for every scale in all of its lanes, conversions two values at a time, sixteen columns
 // of a scale to a lane where no row has to stay.  Measured, with inputs larger than L2: rows of 4096 bf16 (14336 of them) 29 us, 6.0 TB/s, as a plain copy of these bytes (sixteen lanes of eight
 // columns, two to a thread: 35); blocks 28 us, 6.4 TB/s (with a test at every load and widened values kept instead of made again: 65).
-// A row of the norm stays in the registers of its CTA between the statistics and the outputs.  Few rows take a thread for every eight columns (latency).  Many rows: CTAs that stay, sixteen
-// columns a thread, with the next row on its way while one is worked on and the weights kept: 2048 rows of 4096, residual and all in bf16, 12.7 us, 4.6 TB/s (a CTA a row 15.7;
-// a copy of these bytes 12.2).
+// Rows that start anywhere: a lane has every 32nd column, so that a warp's accesses are runs, all asked for at once (14336 rows of 4095 bf16 with a scale a row 88 us and blocks 60, of which
+// eight neighbours a lane, one value at a time, took 141 and 112; 2539 rows of 1364 f16 6.9 and 12.6).
+// A row of the norm stays in the registers of its CTA between the statistics and the outputs.  Few rows take a thread for every eight columns (latency; one row of 2560 2.0 us).  Many rows: CTAs
+// that stay, sixteen columns a thread, with the next row on its way while one is worked on and the weights kept: 2048 rows of 4096, residual and all in bf16, 12.8 us, 4.6 TB/s (a CTA a row 15.7;
+// a copy of these bytes 12.2; values computed outside the condition behind which they are stored 15.6); rows of 4095 34 (48).
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -33,19 +35,21 @@ template <> __device__ __forceinline__ float e4_round<float>(float v) { return v
 template <> __device__ __forceinline__ __half e4_round<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 e4_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// eight neighbouring values as they lie in memory
+// eight values of a thread as they lie in memory.  EIGHTS: neighbours, on a boundary of 16 bytes.  Else: of 256 columns that a warp has, those of each 32 that are its lane's, so that a
+// warp's accesses to rows that start anywhere are runs of 32 columns
 template <typename E> struct E4Raw { uint4 u[sizeof(E) * 8 / 16]; };
-// eight values from p on, of which n are there (the others read as zeros); whole: all are there, on a boundary of 16 bytes
-template <typename E>
-__device__ __forceinline__ E4Raw<E> e4_load(const E* p, int n, bool whole) {
+__device__ __forceinline__ int e4_column(int i) { return (i >> 2) * 128 + (i & 3) * 32; }            // from the lane's first column
+// eights: from p on.  Else: p[first + ...], of columns below `width`, whose last stands for those behind it (loads under a condition of their own take as long as one after the other)
+template <bool EIGHTS, typename E>
+__device__ __forceinline__ E4Raw<E> e4_load(const E* p, int first, int width) {
     E4Raw<E> r;
-    if (whole) {
+    if constexpr (EIGHTS) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+        for (int i = 0; i < (int)sizeof(E) / 2; ++i) r.u[i] = reinterpret_cast<const uint4*>(p + first)[i];
     } else {
         E e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : e4_round<E>(0.f);
+        for (int i = 0; i < 8; ++i) e[i] = p[min(first + e4_column(i), width - 1)];
         memcpy(&r, e, sizeof(r));
     }
     return r;
@@ -88,35 +92,32 @@ __device__ __forceinline__ E4Raw<E> e4_rounded(const float (&v)[8]) {
     }
     return r;
 }
-template <typename E>
-__device__ __forceinline__ void e4_store(E* p, const float (&v)[8], int n, bool whole) {
+template <bool EIGHTS, typename E>
+__device__ __forceinline__ void e4_store(E* p, int first, int width, const float (&v)[8]) {
     const E4Raw<E> r = e4_rounded<E>(v);
-    if (whole) {
+    if constexpr (EIGHTS) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(E) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = r.u[i];
+        for (int i = 0; i < (int)sizeof(E) / 2; ++i) reinterpret_cast<uint4*>(p + first)[i] = r.u[i];
     } else {
         E e[8];
         memcpy(e, &r, sizeof(r));
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = e[i];
+            if (first + e4_column(i) < width) p[first + e4_column(i)] = e[i];
     }
 }
-// eight values times inv as e4m3.  (satfinite: the group's largest times the rounded reciprocal may come out a hair above 448; NaN stays NaN)
-__device__ __forceinline__ uint2 e4_pack(const float (&v)[8], float inv) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-    return make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+// values times inv as e4m3.  (satfinite: the group's largest times the rounded reciprocal may come out a hair above 448; NaN stays NaN)
+__device__ __forceinline__ uint32_t e4_four(const float* v, float inv) {
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3),
+                   b = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3);
+    return a | b << 16;
 }
-__device__ __forceinline__ void e4_put(uint8_t* p, uint2 q, int n, bool whole) {
-    if (whole) {
-        *reinterpret_cast<uint2*>(p) = q;
-        return;
-    }
+__device__ __forceinline__ uint2 e4_pack(const float (&v)[8], float inv) { return make_uint2(e4_four(v, inv), e4_four(v + 4, inv)); }
+// four values of a lane, 32 columns apart
+__device__ __forceinline__ void e4_put(uint8_t* p, int first, int width, uint32_t q) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) p[i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    for (int i = 0; i < 4; ++i)
+        if (first + 32 * i < width) p[first + 32 * i] = (uint8_t)(q >> (8 * i));
 }
 __device__ __forceinline__ float e4_most(const float (&v)[8]) {
     float m = 0.f;
@@ -140,20 +141,20 @@ struct NormParams {
     float* scale;                    // [rows][groups]; null: `out` has the type of x
     int rows, width, groups;
     float eps, offset;
-    int vec;                         // eights of a row lie on 16-byte boundaries in x, residual, residual_out and weight
-    int vec_out;                     // and, as they have to, in out
 };
 
-// E: x; R: residual and the sum that is handed on.  NV: eights of a thread; MANY: a CTA takes row after row, all of whole eights
+// E: x; R: residual and the sum that is handed on.  NV: eight values of a thread so many times; EIGHTS: neighbours, on 16-byte boundaries in all rows (out's, too: 8 of 8-bit
+// ones); MANY: a CTA takes row after row
 constexpr int NORM_MANY_THREADS = 256;
-template <typename E, typename R> constexpr int norm_many_per_sm() { return sizeof(E) == 4 || sizeof(R) == 4 ? 2 : 3; }         // CTAs of so many threads
-template <typename E, typename R, int NV, bool MANY>
-__global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 512), MANY ? norm_many_per_sm<E, R>() : 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
+template <typename E, typename R, bool EIGHTS> constexpr int norm_many_per_sm() { return sizeof(E) == 4 || sizeof(R) == 4 || !EIGHTS ? 2 : 3; }         // CTAs of so many threads
+template <typename E, typename R, int NV, bool EIGHTS, bool MANY>
+__global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 512), MANY ? norm_many_per_sm<E, R, EIGHTS>() : 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ float red[2][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const bool add = p.residual != nullptr;
-    auto column = [&](int k) { return (k * (int)blockDim.x + tid) * 8; };
-    auto whole_in = [&](int n) { return MANY || (p.vec && n >= 8); };
+    auto column = [&](int k) { return EIGHTS ? (k * (int)blockDim.x + tid) * 8 : (k * warps + warp) * 256 + lane; };
+    // (a thread none of whose columns are there; others read the last one's)
+    auto none = [&](int k) { return EIGHTS && column(k) >= p.width; };
     E4Raw<E> a[NV];
     E4Raw<R> b[NV];
     auto fetch = [&](int row) {
@@ -161,20 +162,18 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
         const R* const res = reinterpret_cast<const R*>(p.residual) + row * p.residual_stride;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = column(k), n = p.width - c;
-            if (n <= 0) continue;
-            a[k] = e4_load<E>(x + c, n, whole_in(n));
-            if (add) b[k] = e4_load<R>(res + c, n, whole_in(n));
+            if (none(k)) continue;
+            a[k] = e4_load<EIGHTS, E>(x, column(k), p.width);
+            if (add) b[k] = e4_load<EIGHTS, R>(res, column(k), p.width);
         }
     };
     auto weights = [&](int k, float (&g)[8]) {   // offset + weight
-        const int c = column(k), n = p.width - c;
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = 1.f;
-        if (n > 0 && p.weight) {
-            if (p.weight_type == B200RWKV_TYPE_F32) e4_values<float>(e4_load<float>(reinterpret_cast<const float*>(p.weight) + c, n, whole_in(n)), g);
-            else if (p.weight_type == B200RWKV_TYPE_F16) e4_values<__half>(e4_load<__half>(reinterpret_cast<const __half*>(p.weight) + c, n, whole_in(n)), g);
-            else e4_values<__nv_bfloat16>(e4_load<__nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(p.weight) + c, n, whole_in(n)), g);
+        if (p.weight && !none(k)) {
+            if (p.weight_type == B200RWKV_TYPE_F32) e4_values<float>(e4_load<EIGHTS, float>(reinterpret_cast<const float*>(p.weight), column(k), p.width), g);
+            else if (p.weight_type == B200RWKV_TYPE_F16) e4_values<__half>(e4_load<EIGHTS, __half>(reinterpret_cast<const __half*>(p.weight), column(k), p.width), g);
+            else e4_values<__nv_bfloat16>(e4_load<EIGHTS, __nv_bfloat16>(reinterpret_cast<const __nv_bfloat16*>(p.weight), column(k), p.width), g);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] += p.offset;
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
         float h[NV][8];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            if (p.width - column(k) <= 0) {
+            if (none(k)) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[k][i] = 0.f;
                 continue;
@@ -203,6 +202,10 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
                 e4_values<R>(b[k], r);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) h[k][i] += r[i];
+            }
+            if (!EIGHTS) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[k][i] = column(k) + e4_column(i) < p.width ? h[k][i] : 0.f;
             }
         }
         const int next = row + (int)gridDim.x;
@@ -219,30 +222,42 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
         const float over = rsqrtf(sum / (float)p.width + p.eps);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const int c = column(k), n = p.width - c;
-            // (all sixteen lanes of a scale take part in its maximum, those behind the row with zeros)
-            const bool whole = whole_in(n), whole_out = MANY || (p.vec_out && n >= 8);
+            const int c = column(k);
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = 0.f;
-            if (n > 0) {
-                if (add) e4_store<R>(reinterpret_cast<R*>(p.residual_out) + row * p.residual_out_stride + c, h[k], n, whole);
+            if (!none(k)) {
+                if (add) e4_store<EIGHTS, R>(reinterpret_cast<R*>(p.residual_out) + row * p.residual_out_stride, c, p.width, h[k]);
                 if (!EARLY) weights(k, g[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (whole || i < n) y[i] = h[k][i] * over * g[EARLY ? k : 0][i];
+                for (int i = 0; i < 8; ++i) y[i] = h[k][i] * over * g[EARLY ? k : 0][i];
             }
-            if (p.scale) {
+            if (!p.scale) {
+                if (!none(k)) e4_store<EIGHTS, E>(reinterpret_cast<E*>(p.out) + row * p.out_stride, c, p.width, y);
+                continue;
+            }
+            uint8_t* const out = reinterpret_cast<uint8_t*>(p.out) + row * p.out_stride;
+            float* const scale = p.scale + (long long)row * p.groups;
+            if (EIGHTS) {                        // (all sixteen lanes of a scale take part in its maximum, those behind the row with zeros)
                 float most = e4_most(y);
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const float s = e4_scale(most);
-                if (n > 0) {
-                    e4_put(reinterpret_cast<uint8_t*>(p.out) + row * p.out_stride + c, e4_pack(y, __frcp_rn(s)), n, whole_out);
-                    if ((lane & 15) == 0) p.scale[(long long)row * p.groups + c / E4_GROUP] = s;
+                if (!none(k)) {
+                    *reinterpret_cast<uint2*>(out + c) = e4_pack(y, __frcp_rn(s));
+                    if ((lane & 15) == 0) scale[c / E4_GROUP] = s;
                 }
-            } else if (n > 0) {
-                e4_store<E>(reinterpret_cast<E*>(p.out) + row * p.out_stride + c, y, n, whole_out);
+            } else {                             // (a warp has two scales; behind the row its values are zeros)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int at = c + j * E4_GROUP;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[4 * j + i] = at + 32 * i < p.width ? y[4 * j + i] : 0.f;
+                    const float most = warp_max(fmaxf(fmaxf(fabsf(y[4 * j]), fabsf(y[4 * j + 1])), fmaxf(fabsf(y[4 * j + 2]), fabsf(y[4 * j + 3]))));
+                    const float s = e4_scale(most);
+                    e4_put(out, at, p.width, e4_four(y + 4 * j, __frcp_rn(s)));
+                    if (lane == 0 && at < p.width) scale[at / E4_GROUP] = s;
+                }
             }
         }
         row = next;
@@ -257,45 +272,61 @@ struct E4Params {
     long long out_stride;
     float* scale;                    // [rows, or blocks of 128 rows][groups]
     int rows, width, groups;
-    int vec;                         // eights of a row lie on 16-byte boundaries in x, on 8-byte ones in out; 2: sixteens of out on 16-byte ones
+    int wide;                        // sixteens of out lie on 16-byte boundaries
 };
 
 constexpr int E4_THREADS = 256, E4_PER_ROW = E4_GROUP / 16;         // lanes of a scale in a row
-// a scale for 128 columns of a row: eight lanes of sixteen columns.  They lie one behind another over the rows
-template <typename E>
+// A scale for 128 columns of a row.  EIGHTS: eight lanes of sixteen columns, which lie one behind another over the rows.  Else: a warp for two of them
+template <bool EIGHTS, typename E>
 __global__ void __launch_bounds__(E4_THREADS) e4_rows_kernel(const __grid_constant__ E4Params p) {
     pdl_wait();
-    const unsigned per_row = (unsigned)p.groups * E4_PER_ROW;
-    const unsigned long long at = (unsigned long long)blockIdx.x * E4_THREADS + threadIdx.x;
-    const unsigned row = at >> 32 ? (unsigned)(at / per_row) : (unsigned)at / per_row;
-    const int col = (int)(unsigned)(at - (unsigned long long)row * per_row) * 16, n = row < (unsigned)p.rows ? p.width - col : 0;
-    const E* const x = reinterpret_cast<const E*>(p.x) + (long long)row * p.x_stride + col;
-    auto whole = [&](int left) { return p.vec && left >= 8; };
-    E4Raw<E> a[2];
-    float v[2][8], most = 0.f;
+    const unsigned per_row = EIGHTS ? (unsigned)p.groups * E4_PER_ROW : ((unsigned)p.groups + 1) / 2;
+    const unsigned long long thread = (unsigned long long)blockIdx.x * E4_THREADS + threadIdx.x, at = EIGHTS ? thread : thread >> 5;
+    const unsigned row = at >> 32 ? (unsigned)(at / per_row) : (unsigned)at / per_row, unit = (unsigned)(at - (unsigned long long)row * per_row);
+    const E* const x = reinterpret_cast<const E*>(p.x) + (long long)row * p.x_stride;
+    uint8_t* const out = p.out + (long long)row * p.out_stride;
+    float* const scale = p.scale + (long long)row * p.groups;
+    if (EIGHTS) {
+        const int col = (int)unit * 16, n = row < (unsigned)p.rows ? p.width - col : 0;
+        E4Raw<E> a[2];
+        float v[2][8], most = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-        if (n > 8 * j) a[j] = e4_load<E>(x + 8 * j, n - 8 * j, whole(n - 8 * j));
+        for (int j = 0; j < 2; ++j)
+            if (n > 8 * j) a[j] = e4_load<true, E>(x, col + 8 * j, p.width);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-        if (n > 8 * j) e4_values<E>(a[j], v[j]);
-        most = fmaxf(most, e4_most(v[j]));
-    }
+            for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
+            if (n > 8 * j) e4_values<E>(a[j], v[j]);
+            most = fmaxf(most, e4_most(v[j]));
+        }
 #pragma unroll
-    for (int o = E4_PER_ROW / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    const float s = e4_scale(most), inv = __frcp_rn(s);
-    if (n <= 0) return;
-    uint8_t* const out = p.out + (long long)row * p.out_stride + col;
-    const uint2 q[2] = {e4_pack(v[0], inv), e4_pack(v[1], inv)};
-    if (p.vec > 1 && n >= 16) {
-        *reinterpret_cast<uint4*>(out) = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+        for (int o = E4_PER_ROW / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float s = e4_scale(most), inv = __frcp_rn(s);
+        if (n <= 0) return;
+        const uint2 q[2] = {e4_pack(v[0], inv), e4_pack(v[1], inv)};
+        if (p.wide && n >= 16) {
+            *reinterpret_cast<uint4*>(out + col) = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
+        } else {
+            *reinterpret_cast<uint2*>(out + col) = q[0];
+            if (n > 8) *reinterpret_cast<uint2*>(out + col + 8) = q[1];
+        }
+        if (threadIdx.x % E4_PER_ROW == 0) scale[col / E4_GROUP] = s;
     } else {
-        e4_put(out, q[0], n, whole(n));
-        e4_put(out + 8, q[1], n - 8, whole(n - 8));
+        if (row >= (unsigned)p.rows) return;     // (a warp as one)
+        const int lane = threadIdx.x & 31, col = (int)unit * 2 * E4_GROUP + lane;
+        float v[8];
+        e4_values<E>(e4_load<false, E>(x, col, p.width), v);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int c = col + j * E4_GROUP;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = c + 32 * i < p.width ? v[4 * j + i] : 0.f;
+            const float s = e4_scale(warp_max(fmaxf(fmaxf(fabsf(v[4 * j]), fabsf(v[4 * j + 1])), fmaxf(fabsf(v[4 * j + 2]), fabsf(v[4 * j + 3])))));
+            e4_put(out, c, p.width, e4_four(v + 4 * j, __frcp_rn(s)));
+            if (lane == 0 && c < p.width) scale[c / E4_GROUP] = s;
+        }
     }
-    if (threadIdx.x % E4_PER_ROW == 0) p.scale[(long long)row * p.groups + col / E4_GROUP] = s;
 }
 
 // the same bits, of which the compiler knows nothing: what was made of them is made again instead of kept
@@ -305,51 +336,66 @@ __device__ __forceinline__ void e4_anew(E4Raw<E>& r) {
     for (int i = 0; i < (int)sizeof(E) / 2; ++i) asm volatile("" : "+r"(r.u[i].x), "+r"(r.u[i].y), "+r"(r.u[i].z), "+r"(r.u[i].w));
 }
 
-// a scale for a block of 128 x 128: a CTA, in its registers; sixteen lanes along a row, sixteen rows at a time
-template <typename E>
-__global__ void __launch_bounds__(E4_THREADS, sizeof(E) == 4 ? 2 : 4) e4_blocks_kernel(const __grid_constant__ E4Params p) {
+// A scale for a block of 128 x 128: a CTA, in its registers.  EIGHTS: sixteen lanes along a row, sixteen rows at a time.  Else: a warp along a row.  Rows and columns that are not there
+// read the last ones', which changes no maximum
+template <bool EIGHTS, typename E>
+__global__ void __launch_bounds__(E4_THREADS, EIGHTS && sizeof(E) == 2 ? 4 : 2) e4_blocks_kernel(const __grid_constant__ E4Params p) {
     __shared__ float red[E4_THREADS / 32];
-    constexpr int ROWS = E4_THREADS / 16, N = E4_GROUP / ROWS;
     pdl_wait();
-    const int g = blockIdx.x % p.groups, b = blockIdx.x / p.groups, c = g * E4_GROUP + (threadIdx.x & 15) * 8, n = p.width - c;
-    const long long first = (long long)b * E4_GROUP + (threadIdx.x >> 4);
-    const E* const x = reinterpret_cast<const E*>(p.x) + first * p.x_stride + c;
-    uint8_t* const out = p.out + first * p.out_stride + c;
-    auto work = [&](auto inside) {               // whether all rows and columns are
-        constexpr bool INSIDE = decltype(inside)::value;
-        const bool whole = INSIDE || (p.vec && n >= 8);
-        auto there = [&](int i) { return INSIDE || (first + i * ROWS < p.rows && n > 0); };
+    const int g = blockIdx.x % p.groups, b = blockIdx.x / p.groups, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rows = min(E4_GROUP, p.rows - b * E4_GROUP), last = min(E4_GROUP, p.width - g * E4_GROUP) - (EIGHTS ? 8 : 1);      // of the block; the first column of its last eight
+    const E* const x = reinterpret_cast<const E*>(p.x) + (long long)b * E4_GROUP * p.x_stride + (long long)g * E4_GROUP;
+    uint8_t* const out = p.out + (long long)b * E4_GROUP * p.out_stride + (long long)g * E4_GROUP;
+    auto scale_of = [&](float most) {
+        most = warp_max(most);
+        if (lane == 0) red[warp] = most;
+        __syncthreads();
+        most = 0.f;
+#pragma unroll
+        for (int i = 0; i < E4_THREADS / 32; ++i) most = fmaxf(most, red[i]);
+        const float s = e4_scale(most);
+        if (threadIdx.x == 0) p.scale[(long long)b * p.groups + g] = s;
+        return s;
+    };
+    float most = 0.f;
+    if (EIGHTS) {
+        constexpr int ROWS = E4_THREADS / 16, N = E4_GROUP / ROWS;
+        const int first = threadIdx.x >> 4, c = (threadIdx.x & 15) * 8;
         E4Raw<E> a[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (there(i)) a[i] = e4_load<E>(x + i * ROWS * p.x_stride, n, whole);
-        float most = 0.f;
+        for (int i = 0; i < N; ++i) a[i] = e4_load<true, E>(x + min(first + i * ROWS, rows - 1) * p.x_stride, min(c, last), 0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (!there(i)) continue;
             float v[8];
             e4_values<E>(a[i], v);
             most = fmaxf(most, e4_most(v));
             e4_anew(a[i]);
         }
-        most = warp_max(most);
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = most;
-        __syncthreads();
-        most = 0.f;
-#pragma unroll
-        for (int i = 0; i < E4_THREADS / 32; ++i) most = fmaxf(most, red[i]);
-        const float s = e4_scale(most), inv = __frcp_rn(s);
+        const float inv = __frcp_rn(scale_of(most));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (!there(i)) continue;
             float v[8];
             e4_values<E>(a[i], v);
-            e4_put(out + i * ROWS * p.out_stride, e4_pack(v, inv), n, whole);
+            if (first + i * ROWS < rows && c <= last) *reinterpret_cast<uint2*>(out + (first + i * ROWS) * p.out_stride + c) = e4_pack(v, inv);
         }
-        if (threadIdx.x == 0) p.scale[(long long)b * p.groups + g] = s;
-    };
-    if (p.vec && (g + 1) * E4_GROUP <= p.width && (b + 1) * E4_GROUP <= p.rows) work(std::true_type{});
-    else work(std::false_type{});
+    } else {
+        constexpr int ROWS = E4_THREADS / 32, N = E4_GROUP / ROWS;
+        E a[N][4];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[i][j] = x[min(warp + i * ROWS, rows - 1) * p.x_stride + min(lane + 32 * j, last)];
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(e4_widen<E>(a[i][j])));
+        const float inv = __frcp_rn(scale_of(most));
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float v[4] = {e4_widen<E>(a[i][0]), e4_widen<E>(a[i][1]), e4_widen<E>(a[i][2]), e4_widen<E>(a[i][3])};
+            if (warp + i * ROWS < rows) e4_put(out + (warp + i * ROWS) * p.out_stride, lane, last + 1, e4_four(v, inv));
+        }
+    }
 }
 
 }  // namespace b200

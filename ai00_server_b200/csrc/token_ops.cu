@@ -23,19 +23,21 @@ static void of_type(int type, F&& f) {
 static bool on(const void* p, long long stride, int size, int boundary) { return (uintptr_t)p % boundary == 0 && (stride * size) % boundary == 0; }
 
 // ---- norms ----
-template <typename E, typename R>
+// EIGHTS: all rows on 16-byte boundaries, of whole eights
+template <bool EIGHTS, typename E, typename R>
 static void norm_form(cudaStream_t s, const NormParams& p, int rows) {
-    const int eights = (p.width + 7) / 8, pairs = ((eights + 1) / 2 + 31) / 32 * 32;
+    // threads of so many times eight values (of which a warp has two groups of 128 columns where rows start anywhere)
+    const int eights = EIGHTS ? p.width / 8 : (p.width + 255) / 256 * 32;
+    auto threads = [&](int nv) { return ((eights + nv - 1) / nv + 31) / 32 * 32; };
     // more rows than CTAs that stay (2048 rows of 4096 bf16 12.8 us; a CTA a row 15.7, with 256 threads or 512)
-    if (p.vec && p.vec_out && p.width % 8 == 0 && pairs <= NORM_MANY_THREADS) {
-        const int ctas = sm_count() * (norm_many_per_sm<E, R>() * NORM_MANY_THREADS / pairs);
-        if (rows > ctas) return launch(rms_norm_kernel<E, R, 2, true>, dim3(ctas), pairs, 0, s, p);
+    if (threads(2) <= NORM_MANY_THREADS) {
+        const int ctas = sm_count() * (norm_many_per_sm<E, R, EIGHTS>() * NORM_MANY_THREADS / threads(2));
+        if (rows > ctas) return launch(rms_norm_kernel<E, R, 2, EIGHTS, true>, dim3(ctas), threads(2), 0, s, p);
     }
     // few rows: a thread for every eight columns; many: sixteen, so that an SM has several rows in flight (1024 rows of 8192 16.6 us and 19.8); wider ones what the largest CTA needs
     int nv = 1;
     if (eights > 1024 || (rows > 2 * sm_count() && eights > 256)) nv = eights <= 1024 ? 2 : (eights <= 2048 ? 4 : 8);
-    const int threads = ((eights + nv - 1) / nv + 31) / 32 * 32;
-    auto form = [&](auto n) { launch(rms_norm_kernel<E, R, decltype(n)::value, false>, dim3(rows), threads, 0, s, p); };
+    auto form = [&](auto n) { launch(rms_norm_kernel<E, R, decltype(n)::value, EIGHTS, false>, dim3(rows), threads(nv), 0, s, p); };
     if (nv == 1) form(std::integral_constant<int, 1>{});
     else if (nv == 2) form(std::integral_constant<int, 2>{});
     else if (nv == 4) form(std::integral_constant<int, 4>{});
@@ -188,14 +190,17 @@ int32_t b200rwkv_op_norm(int32_t device, void* stream, const b200rwkv_norm* q) {
     p.scale = eight ? q->scale : nullptr;
     p.rows = q->rows; p.width = q->width; p.groups = groups;
     p.eps = q->eps; p.offset = q->offset;
-    p.vec = on(q->x, q->x_stride, size, 16) && (uintptr_t)q->weight % 16 == 0 &&
-            (!q->residual || (on(q->residual, q->residual_stride, rsize, 16) && on(q->residual_out, q->residual_out_stride, rsize, 16)));
-    p.vec_out = on(q->out, q->out_stride, osize, eight ? 8 : 16);
+    const bool eights = q->width % 8 == 0 && on(q->x, q->x_stride, size, 16) && (uintptr_t)q->weight % 16 == 0 && on(q->out, q->out_stride, osize, eight ? 8 : 16) &&
+                        (!q->residual || (on(q->residual, q->residual_stride, rsize, 16) && on(q->residual_out, q->residual_out_stride, rsize, 16)));
     OnDevice here(device);
     of_type(q->type, [&](auto e) {
         using E = decltype(e);
-        if (q->residual_type == q->type) norm_form<E, E>((cudaStream_t)stream, p, q->rows);
-        else if constexpr (!std::is_same_v<E, float>) norm_form<E, float>((cudaStream_t)stream, p, q->rows);
+        auto form = [&](auto r) {
+            if (eights) norm_form<true, E, decltype(r)>((cudaStream_t)stream, p, q->rows);
+            else norm_form<false, E, decltype(r)>((cudaStream_t)stream, p, q->rows);
+        };
+        if (q->residual_type == q->type) form(e);
+        else if constexpr (!std::is_same_v<E, float>) form(0.f);
     });
     API_END
 }
@@ -215,13 +220,19 @@ int32_t b200rwkv_op_e4m3(int32_t device, void* stream, const b200rwkv_e4m3* q) {
     const long long units = blocks * groups;
     const RowSpan x(q->x, q->rows, q->x_stride, q->width, size), out(q->out, q->rows, q->out_stride, q->width, 1), scale(q->scale, 1, units, units, 4);
     REQUIRE(!overlap(out, x) && !overlap(scale, x) && !overlap(scale, out), B200RWKV_ERR_INVALID, "op_e4m3: x, out and scale overlap");
-    const long long ctas = q->block_rows == 1 ? (units * E4_PER_ROW + E4_THREADS - 1) / E4_THREADS : units;
+    const bool eights = q->width % 8 == 0 && on(q->x, q->x_stride, size, 16) && on(q->out, q->out_stride, 1, 8);
+    const long long threads = eights ? units * E4_PER_ROW : q->rows * (long long)((groups + 1) / 2) * 32, ctas = q->block_rows == 1 ? (threads + E4_THREADS - 1) / E4_THREADS : units;
     REQUIRE(ctas <= 0x7FFFFFFFll, B200RWKV_ERR_UNSUPPORTED, "op_e4m3: too many values for one call");
-    E4Params p{q->x, q->x_stride, (uint8_t*)q->out, q->out_stride, q->scale, q->rows, q->width, groups, 0};
-    if (on(q->x, q->x_stride, size, 16) && on(q->out, q->out_stride, 1, 8)) p.vec = on(q->out, q->out_stride, 1, 16) ? 2 : 1;
+    const E4Params p{q->x, q->x_stride, (uint8_t*)q->out, q->out_stride, q->scale, q->rows, q->width, groups, on(q->out, q->out_stride, 1, 16)};
     OnDevice here(device);
     of_type(q->type, [&](auto e) {
-        launch(q->block_rows == 1 ? e4_rows_kernel<decltype(e)> : e4_blocks_kernel<decltype(e)>, dim3((unsigned)ctas), E4_THREADS, 0, (cudaStream_t)stream, p);
+        using E = decltype(e);
+        auto form = [&](auto whole) {
+            constexpr bool EIGHTS = decltype(whole)::value;
+            launch(q->block_rows == 1 ? e4_rows_kernel<EIGHTS, E> : e4_blocks_kernel<EIGHTS, E>, dim3((unsigned)ctas), E4_THREADS, 0, (cudaStream_t)stream, p);
+        };
+        if (eights) form(std::true_type{});
+        else form(std::false_type{});
     });
     API_END
 }

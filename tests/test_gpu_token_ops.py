@@ -178,7 +178,7 @@ def test_norm_offset_in_place_and_strides(ops, dtype, res, n):
 
 
 @pytest.mark.parametrize("dtype,res,weight,out", [(F32, F32, F32, E4M3), (F32, None, None, F32), (F16, F32, F16, F16), (BF16, BF16, BF16, E4M3), (BF16, None, F32, E4M3), (F16, F32, BF16, E4M3)])
-@pytest.mark.parametrize("n,w", [(7301, 8), (5000, 136), (4000, 1000), (2001, 2560), (1100, 4096)])
+@pytest.mark.parametrize("n,w", [(7301, 8), (5000, 136), (4000, 1000), (2001, 2560), (1100, 4096), (7301, 3), (3700, 1001), (1100, 4095)])
 def test_norm_of_more_rows_than_stay_on_the_gpu(ops, dtype, res, weight, out, n, w):
     """CTAs take several rows one after another: each row as if it were alone, its residual in place."""
     x = rnd(n, w, std=2.0, dtype=dtype, seed=w)
