@@ -30,10 +30,6 @@ template <typename E> __device__ __forceinline__ float e4_widen(E v);
 template <> __device__ __forceinline__ float e4_widen<float>(float v) { return v; }
 template <> __device__ __forceinline__ float e4_widen<__half>(__half v) { return __half2float(v); }
 template <> __device__ __forceinline__ float e4_widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename E> __device__ __forceinline__ E e4_round(float v);
-template <> __device__ __forceinline__ float e4_round<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half e4_round<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 e4_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // eight values of a thread as they lie in memory.  EIGHTS: neighbours, on a boundary of 16 bytes.  Else: of 256 columns that a warp has, those of each 32 that are its lane's, so that a
 // warp's accesses to rows that start anywhere are runs of 32 columns
