@@ -1,12 +1,12 @@
 // Rows in 8-bit floating point (e4m3) with a scale for every 128 columns of a row, or for every block of 128 x 128: as they are, or behind a root-mean-square
 // norm that first adds the residual:
 //     h = x + residual (f32; handed on rounded to the residual's type),  y = h rsqrt(mean(h^2) + eps) (offset + weight)
-//     s = max(max |y| over the group, 2^-100) / 448,  q = y / s rounded once, to nearest
-// (the floor keeps 1 / s a number; a group of zeros is zeros.)
+//     s = max(max |y| over the group, 2^-100) / 448,  q = y / s
+// s and y / s are f32, rounded to nearest, and q is the e4m3 number nearest to that.  (The floor keeps 1 / s a number; a group of zeros is zeros.)
 //
 // Bound: memory, each value read once and written once, as far as the instructions let it: two divisions for every scale in all of its lanes, conversions two values at a time, sixteen columns
 // of a scale to a lane where no row has to stay.  Measured, with inputs larger than L2: rows of 4096 bf16 (14336 of them) 29 us, 6.0 TB/s, as a plain copy of these bytes (sixteen lanes of eight
-// columns, two to a thread: 35); blocks 28 us, 6.4 TB/s (with a test at every load and widened values kept instead of made again: 65).
+// columns, two to a thread: 35); blocks 29 us, 6.0 TB/s (with a test at every load and widened values kept instead of made again: 65).
 // Rows that start anywhere: a lane has every 32nd column, so that a warp's accesses are runs, all asked for at once (14336 rows of 4095 bf16 with a scale a row 88 us and blocks 60, of which
 // eight neighbours a lane, one value at a time, took 141 and 112; 2539 rows of 1364 f16 6.9 and 12.6).
 // A row of the norm stays in the registers of its CTA between the statistics and the outputs.  Few rows take a thread for every eight columns (latency; one row of 2560 2.0 us).  Many rows: CTAs
@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace b200 {
 
@@ -102,13 +103,26 @@ __device__ __forceinline__ void e4_store(E* p, int first, int width, const float
             if (first + e4_column(i) < width) p[first + e4_column(i)] = e[i];
     }
 }
-// values times inv as e4m3.  (satfinite: the group's largest times the rounded reciprocal may come out a hair above 448; NaN stays NaN)
-__device__ __forceinline__ uint32_t e4_four(const float* v, float inv) {
-    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3),
-                   b = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3);
-    return a | b << 16;
+// What a group's values are divided by: they become the f32 quotient as a division rounds it, to nearest, and that to nearest e4m3, so that the numbers are those that (y / s), converted
+// anywhere else, has.  The reciprocal comes in two parts, 1 / s = high + low to 2^-45 of itself: with e = 1 - s high, low = high (e + e^2).  A quotient y high + y low is off by 2^-44 before it
+// is rounded: as a division has it for every value of 16 bits (tried out), and for one of f32 but where y / s is that near to the middle of two f32 numbers beside a tie.  (The product with a
+// rounded reciprocal alone lay a step beside it where a value is on a tie of its group: 5 in 10 000 bf16 weights.)  high stays below 1 / s (the unit's is a step off at most): no low is
+// negative, and zeros keep their signs.  An infinite scale makes zeros of numbers and NaN of infinities
+struct E4Over { f32x2 high, low; };
+__device__ __forceinline__ E4Over e4_over(float s) {
+    float high;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(high) : "f"(s));
+    high *= 1.f - 0x1p-22f;
+    const float e = s < INFINITY ? fmaf(-s, high, 1.f) : 0.f, low = high * fmaf(e, e, e);
+    return {pack2(high, high), pack2(low, low)};
 }
-__device__ __forceinline__ uint2 e4_pack(const float (&v)[8], float inv) { return make_uint2(e4_four(v, inv), e4_four(v + 4, inv)); }
+__device__ __forceinline__ uint32_t e4_two(float a, float b, const E4Over& o) {
+    const f32x2 y = pack2(a, b);
+    // (satfinite: the group's largest may come out a hair above 448; NaN stays NaN)
+    return __nv_cvt_float2_to_fp8x2(unpack2(fmadd2(y, o.high, prod2(y, o.low))), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint32_t e4_four(const float* v, const E4Over& o) { return e4_two(v[0], v[1], o) | e4_two(v[2], v[3], o) << 16; }
+__device__ __forceinline__ uint2 e4_pack(const float (&v)[8], const E4Over& o) { return make_uint2(e4_four(v, o), e4_four(v + 4, o)); }
 // four values of a lane, 32 columns apart
 __device__ __forceinline__ void e4_put(uint8_t* p, int first, int width, uint32_t q) {
 #pragma unroll
@@ -240,7 +254,7 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
                 for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const float s = e4_scale(most);
                 if (!none(k)) {
-                    *reinterpret_cast<uint2*>(out + c) = e4_pack(y, __frcp_rn(s));
+                    *reinterpret_cast<uint2*>(out + c) = e4_pack(y, e4_over(s));
                     if ((lane & 15) == 0) scale[c / E4_GROUP] = s;
                 }
             } else {                             // (a warp has two scales; behind the row its values are zeros)
@@ -251,7 +265,7 @@ __global__ void __launch_bounds__(MANY ? NORM_MANY_THREADS : (NV == 1 ? 1024 : 5
                     for (int i = 0; i < 4; ++i) y[4 * j + i] = at + 32 * i < p.width ? y[4 * j + i] : 0.f;
                     const float most = warp_max(fmaxf(fmaxf(fabsf(y[4 * j]), fabsf(y[4 * j + 1])), fmaxf(fabsf(y[4 * j + 2]), fabsf(y[4 * j + 3]))));
                     const float s = e4_scale(most);
-                    e4_put(out, at, p.width, e4_four(y + 4 * j, __frcp_rn(s)));
+                    e4_put(out, at, p.width, e4_four(y + 4 * j, e4_over(s)));
                     if (lane == 0 && at < p.width) scale[at / E4_GROUP] = s;
                 }
             }
@@ -298,9 +312,10 @@ __global__ void __launch_bounds__(E4_THREADS) e4_rows_kernel(const __grid_consta
         }
 #pragma unroll
         for (int o = E4_PER_ROW / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float s = e4_scale(most), inv = __frcp_rn(s);
+        const float s = e4_scale(most);
+        const E4Over over = e4_over(s);
         if (n <= 0) return;
-        const uint2 q[2] = {e4_pack(v[0], inv), e4_pack(v[1], inv)};
+        const uint2 q[2] = {e4_pack(v[0], over), e4_pack(v[1], over)};
         if (p.wide && n >= 16) {
             *reinterpret_cast<uint4*>(out + col) = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y);
         } else {
@@ -319,7 +334,7 @@ __global__ void __launch_bounds__(E4_THREADS) e4_rows_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * j + i] = c + 32 * i < p.width ? v[4 * j + i] : 0.f;
             const float s = e4_scale(warp_max(fmaxf(fmaxf(fabsf(v[4 * j]), fabsf(v[4 * j + 1])), fmaxf(fabsf(v[4 * j + 2]), fabsf(v[4 * j + 3])))));
-            e4_put(out, c, p.width, e4_four(v + 4 * j, __frcp_rn(s)));
+            e4_put(out, c, p.width, e4_four(v + 4 * j, e4_over(s)));
             if (lane == 0 && c < p.width) scale[c / E4_GROUP] = s;
         }
     }
@@ -367,12 +382,12 @@ __global__ void __launch_bounds__(E4_THREADS, EIGHTS && sizeof(E) == 2 ? 4 : 2) 
             most = fmaxf(most, e4_most(v));
             e4_anew(a[i]);
         }
-        const float inv = __frcp_rn(scale_of(most));
+        const E4Over over = e4_over(scale_of(most));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float v[8];
             e4_values<E>(a[i], v);
-            if (first + i * ROWS < rows && c <= last) *reinterpret_cast<uint2*>(out + (first + i * ROWS) * p.out_stride + c) = e4_pack(v, inv);
+            if (first + i * ROWS < rows && c <= last) *reinterpret_cast<uint2*>(out + (first + i * ROWS) * p.out_stride + c) = e4_pack(v, over);
         }
     } else {
         constexpr int ROWS = E4_THREADS / 32, N = E4_GROUP / ROWS;
@@ -385,11 +400,11 @@ __global__ void __launch_bounds__(E4_THREADS, EIGHTS && sizeof(E) == 2 ? 4 : 2) 
         for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(e4_widen<E>(a[i][j])));
-        const float inv = __frcp_rn(scale_of(most));
+        const E4Over over = e4_over(scale_of(most));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float v[4] = {e4_widen<E>(a[i][0]), e4_widen<E>(a[i][1]), e4_widen<E>(a[i][2]), e4_widen<E>(a[i][3])};
-            if (warp + i * ROWS < rows) e4_put(out + (warp + i * ROWS) * p.out_stride, lane, last + 1, e4_four(v, inv));
+            if (warp + i * ROWS < rows) e4_put(out + (warp + i * ROWS) * p.out_stride, lane, last + 1, e4_four(v, over));
         }
     }
 }
