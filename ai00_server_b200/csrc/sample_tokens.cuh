@@ -703,7 +703,10 @@ __global__ void __launch_bounds__(TH, PER_SM) draw_kernel(const __grid_constant_
         last = nearest = draw_logit(key);
         tied = true;
         last_id = (1 << DRAW_ID_BITS) - 1 - (int)(key & ((1u << DRAW_ID_BITS) - 1));
-        if (shift < 64) return UNENDED;          // (equal logits: what lies between the list and narrower bins is not in the sums)
+        if (shift < 64) {                        // (equal logits: what lies between the list and narrower bins is not in the sums)
+            __syncthreads();                     // (all have read their entry: the warps' queues lie over the list)
+            return UNENDED;
+        }
         // the list's part of the sums
         const bool kept = tid <= end;
         const u64 listed = draw_warp_sum(kept ? w : 0);
