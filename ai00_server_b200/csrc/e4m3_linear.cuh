@@ -60,22 +60,26 @@ __device__ __forceinline__ bool e4l_elect() {
     return is != 0;
 }
 // waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and what hangs on it becomes NaN.  A role that
-// lost a wait arrives nowhere any more, so that those behind it lose theirs
-// (the clock is asked every 256 tries: reading it takes longer than most waits)
-template <typename F>
-__device__ __forceinline__ bool e4l_wait_for(F&& there) {
+// lost a wait arrives nowhere any more, so that those behind it lose theirs; before its CTA ends it waits once more, as long again at most, for the copies and products that it
+// asked for: nothing is written to shared memory that is another's by then
+// (the clock is asked every 256 tries: reading it takes longer than most waits).  WARP: all of a warp have the same answer, or, where one had lost its wait, the others would
+// elect a lane without it
+template <bool WARP>
+__device__ __forceinline__ bool e4l_wait_as(uint32_t bar, uint32_t parity) {
     unsigned long long t0 = 0;
     for (;;) {
-        for (int i = 0; i < 256; ++i)
-            if (there()) return true;
-        const unsigned long long t = globaltimer_ns();
+        for (int i = 0; i < 256; ++i) {
+            const bool there = mbar_try(bar, parity);
+            if (WARP ? __all_sync(0xffffffffu, there) : there) return true;
+        }
+        unsigned long long t = globaltimer_ns();
+        if (WARP) t = __shfl_sync(0xffffffffu, t, 0);
         if (t0 == 0) t0 = t;
         else if (t - t0 > 1000000000ull) return false;
     }
 }
-__device__ __forceinline__ bool e4l_wait(uint32_t bar, uint32_t parity) {
-    return e4l_wait_for([&] { return mbar_try(bar, parity); });
-}
+__device__ __forceinline__ bool e4l_wait(uint32_t bar, uint32_t parity) { return e4l_wait_as<false>(bar, parity); }
+__device__ __forceinline__ bool e4l_wait_warp(uint32_t bar, uint32_t parity) { return e4l_wait_as<true>(bar, parity); }
 template <int N>
 __device__ __forceinline__ void e4l_tmem(uint32_t at, float (&v)[N]) {
     static_assert(N == 16 || N == 32, "columns");
@@ -158,8 +162,9 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
     f32x2 acc[C::MINE / 2];                                  // of two tokens each
     if (warp == C::EPI) {
         unsigned s = 0, phase = 1;
-        for (int i = 0; i < nb; ++i) {
-            if (i >= C::STAGES && !e4l_wait(empty + s * 8, phase)) break;
+        int i = 0;
+        for (; i < nb; ++i) {
+            if (i >= C::STAGES && !e4l_wait_warp(empty + s * 8, phase)) break;
             if (e4l_elect()) {
                 mbar_expect_tx(full + s * 8, C::STAGE);
                 e4l_load(ring + s * C::STAGE, &p.tw, (b0 + i) * E4L_KB, tile * 128, full + s * 8);
@@ -168,12 +173,15 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
             __syncwarp();
             if (++s == C::STAGES) { s = 0; phase ^= 1u; }
         }
+        bool fine = true;
+        for (int k = 1; fine && k <= min(i, C::STAGES); ++k) fine = e4l_wait(full + (i - k) % C::STAGES * 8, (unsigned)((i - k) / C::STAGES) & 1u);      // the copies of this CTA have landed
     } else if (warp == C::EPI + 1) {
         constexpr uint32_t IDESC = e4l_idesc(128, TT);
         unsigned s = 0, phase = 0, b = 0, bphase = 1;
-        for (int i = 0; i < nb; ++i) {
-            if (!e4l_wait(full + s * 8, phase)) break;
-            if (i >= C::BUFS && !e4l_wait(tempty + b * 8, bphase)) break;
+        int i = 0;
+        for (; i < nb; ++i) {
+            if (!e4l_wait_warp(full + s * 8, phase)) break;
+            if (i >= C::BUFS && !e4l_wait_warp(tempty + b * 8, bphase)) break;
             tc_fence_after();
             if (e4l_elect()) {
                 const uint64_t w = e4l_desc(ring + s * C::STAGE), x = e4l_desc(ring + s * C::STAGE + C::W_BYTES);
@@ -186,6 +194,7 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
             if (++s == C::STAGES) { s = 0; phase ^= 1u; }
             if (++b == C::BUFS) { b = 0; bphase ^= 1u; }
         }
+        if (i > 0) e4l_wait(empty + (i - 1) % C::STAGES * 8, (unsigned)((i - 1) / C::STAGES) & 1u);      // and its products, too
     } else {
 #pragma unroll
         for (int t = 0; t < C::MINE / 2; ++t) acc[t] = 0ull;
@@ -408,8 +417,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                     e4l_load2(st + C::X_BYTES, &p.tw, b * E4L_KB, wrow, lead + s * 8);
                 }
             }
-            // every stage in use is released before this CTA may end: the leader's last commits arrive here
+            // every stage in use is released before this CTA may end: the leader's last commits arrive here.  Where a wait was lost, the leader waits for the pair's copies at least
             for (unsigned k = 1; fine && k <= min(i, (unsigned)C::STAGES); ++k) fine = e4l_wait(empty + ((i - k) % C::STAGES) * 8, ((i - k) / C::STAGES) & 1u);
+            bool landed = !fine && rank == 0;
+            for (unsigned k = 1; landed && k <= min(i, (unsigned)C::STAGES); ++k) landed = e4l_wait(full + ((i - k) % C::STAGES) * 8, ((i - k) / C::STAGES) & 1u);
         } else if (warp == C::EPI_WARPS && rank == 0) {
             constexpr uint32_t IDESC = e4l_idesc(256, BN);
             unsigned i = 0, s = 0, phase = 0;
@@ -417,8 +428,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
             for (int u = u0; u < units && fine; u += step)
                 for (int b = 0; b < nb; ++b, ++i) {
                     const unsigned acc = i & 1u;
-                    if (!(fine = e4l_wait(full + s * 8, phase))) break;
-                    if (i >= 2 && !(fine = e4l_wait(tempty + acc * 8, (i / 2 - 1) & 1u))) break;
+                    if (!(fine = e4l_wait_warp(full + s * 8, phase))) break;
+                    if (i >= 2 && !(fine = e4l_wait_warp(tempty + acc * 8, (i / 2 - 1) & 1u))) break;
                     tc_fence_after();
                     if (e4l_elect()) {
                         const uint64_t x = e4l_desc(ring + s * C::STAGE), w = e4l_desc(ring + s * C::STAGE + C::X_BYTES);
@@ -430,6 +441,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                     __syncwarp();
                     if (++s == C::STAGES) { s = 0; phase ^= 1u; }
                 }
+            if (!fine && i > 0) e4l_wait(empty + ((i - 1) % C::STAGES) * 8, ((i - 1) / C::STAGES) & 1u);       // the products that were asked for have ended
         } else if (warp >= C::EPI_WARPS + 2) {
             // scales of the tile's tokens and outputs, a token of a block beside the next
             const int me = tid - (C::EPI_WARPS + 2) * 32;
