@@ -169,6 +169,7 @@ SYMBOLS = [
     ("b200rwkv_op_norm", C.c_int32, [C.c_int32, _P, _P]),
     ("b200rwkv_op_linear_e4m3", C.c_int32, [C.c_int32, _P, _P]),
     ("b200rwkv_op_sample", C.c_int32, [C.c_int32, _P, _P]),
+    ("b200rwkv_op_lost_waits", C.c_int32, [C.c_int32, C.POINTER(C.c_int64)]),
     ("b200rwkv_launch_count", C.c_int32, [_P, C.POINTER(C.c_int64)]),
     ("b200rwkv_keep_hidden", C.c_int32, [_P, C.c_int32]),
     ("b200rwkv_last_hidden", C.c_int32, [_P, _P, C.c_size_t]),

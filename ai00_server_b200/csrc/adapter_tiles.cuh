@@ -16,6 +16,7 @@
 //     next unit arrive while one is written, its product runs during the last rows.
 #pragma once
 #include "adapters.cuh"
+#include "lost_waits.cuh"
 
 namespace b200 {
 
@@ -63,7 +64,7 @@ __device__ __forceinline__ void adt_fence() { asm volatile("fence.proxy.async.sh
 __device__ __forceinline__ void adt_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void adt_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t adt_swizzled(int row, int chunk) { return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4)); }
-// waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and makes NaN of what hangs on it
+// waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and makes NaN of what hangs on it, which is counted at its end
 __device__ __forceinline__ bool adt_bar_wait(uint32_t bar, uint32_t parity) {
     if (mbar_try(bar, parity)) return true;
     const unsigned long long t0 = globaltimer_ns();
@@ -169,7 +170,10 @@ __global__ void __cluster_dims__(ADP_CTAS, 1, 1) __launch_bounds__(ADT_LOW_THREA
         if (fine) tc_commit(bar_s);
     }
     fine = fine && adt_bar_wait(bar_s, 0);
-    if (!fine) adt_bar_wait(bar_s, 0);               // (the slabs are not written over while another thread may still see the products end)
+    if (!fine) {
+        adt_bar_wait(bar_s, 0);                      // (the slabs are not written over while another thread may still see the products end)
+        lost_wait();
+    }
     __syncwarp();
     tc_fence_after();
 
@@ -521,6 +525,7 @@ __global__ void __launch_bounds__(ADT_THREADS, 2) adapter_out_kernel(const __gri
         have = more;
         buf = buf_next;
     }
+    if (!fine) lost_wait();
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tc_dealloc(tmem, 2 * TT);

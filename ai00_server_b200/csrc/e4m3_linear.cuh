@@ -10,6 +10,7 @@
 
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "lost_waits.cuh"
 #include "sm_pair.cuh"
 
 namespace b200 {
@@ -59,7 +60,7 @@ __device__ __forceinline__ bool e4l_elect() {
         : "=r"(is));
     return is != 0;
 }
-// waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and what hangs on it becomes NaN.  A role that
+// waits of these kernels end: a thread whose barrier does not come within about a second goes on without it, and what hangs on it becomes NaN, and is counted (once for each thread of outputs, at its end: in the wait itself, 3 in 100 of a call).  A role that
 // lost a wait arrives nowhere any more, so that those behind it lose theirs; before its CTA ends it waits once more, as long again at most, for the copies and products that it
 // asked for: nothing is written to shared memory that is another's by then
 // (the clock is asked every 256 tries: reading it takes longer than most waits).  WARP: all of a warp have the same answer, or, where one had lost its wait, the others would
@@ -248,7 +249,10 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
             if (++b == C::BUFS) { b = 0; bphase ^= 1u; }
         }
         // a thread whose waits came has seen every copy and product of its CTA end; sums beside a lost wait may be written over by a late copy, and are not used
-        if (!fine) *lost = 1u;
+        if (!fine) {
+            *lost = 1u;
+            lost_wait();
+        }
     }
     // (nothing is in flight any more, or lost: the operands' place is free)
     __syncthreads();
@@ -590,6 +594,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                 __syncwarp();
             }
         }
+        if (!fine) lost_wait();
     }
     tc_fence_before();
     __syncthreads();

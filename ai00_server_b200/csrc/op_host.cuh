@@ -84,4 +84,7 @@ static bool overlap(const RowSpan& a, const RowSpan& b) {
     return d < a.width || a.step - d < b.width;
 }
 
+// waits of adapters that ran out on the current device (operators.cu)
+B200_HIDDEN unsigned adapters_lost_waits();
+
 }  // namespace b200

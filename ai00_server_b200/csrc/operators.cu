@@ -161,6 +161,12 @@ void logits_rows(cudaStream_t s, LogitsParams p, int rows, int type) {
     else typed(__nv_bfloat16{});
 }
 
+unsigned adapters_lost_waits() {
+    unsigned n = 0;
+    CK(cudaMemcpyFromSymbol(&n, lost_waits, sizeof(n)));
+    return n;
+}
+
 }  // namespace b200
 
 using namespace b200;

@@ -301,4 +301,14 @@ int32_t b200rwkv_op_sample(int32_t device, void* stream, const b200rwkv_sample* 
     API_END
 }
 
+int32_t b200rwkv_op_lost_waits(int32_t device, int64_t* total) {
+    API_BEGIN((b200rwkv_engine*)nullptr)
+    REQUIRE(total, B200RWKV_ERR_INVALID, "op_lost_waits: null total");
+    OnDevice here(device);
+    unsigned n = 0;
+    CK(cudaMemcpyFromSymbol(&n, lost_waits, sizeof(n)));
+    *total = (int64_t)n + adapters_lost_waits();
+    API_END
+}
+
 }  // extern "C"

@@ -13,9 +13,12 @@ and what stands in front of them in a step:
 
 A call enqueues kernels on the current stream of its tensors' device and returns; it can be captured into a graph.  Arguments that
 do not fit raise capi.B200Error before anything is enqueued, and so do tensors that ask for a gradient: the operators serve, they have none.
+
+  lost_waits    waits in such kernels that ran out, on a device that does not get on: what hung on them is NaN
 """
 from __future__ import annotations
 
+import ctypes
 import struct
 
 import torch
@@ -287,3 +290,10 @@ def sample(rows, uniform, temperature=None, top_k=None, top_p=None, min_p=None, 
     if code < 0:
         capi.check(code)
     return tokens, probs
+
+
+def lost_waits(device=None):
+    """Waits that ran out on a device (an index; None: the current one) in kernels of low_rank and linear_e4m3 that have ended: 0, or outputs that are NaN may be so for that reason."""
+    total = ctypes.c_int64()
+    capi.check(capi.lib().b200rwkv_op_lost_waits(torch.cuda.current_device() if device is None else device, ctypes.byref(total)))
+    return total.value

@@ -511,6 +511,11 @@ typedef struct {
 } b200rwkv_sample;
 int32_t b200rwkv_op_sample(int32_t device, void* stream, const b200rwkv_sample* args);
 
+/* Waits that ran out on a device since the library was loaded, in kernels of b200rwkv_op_adapters (adapters of slots among them) and b200rwkv_op_linear_e4m3 that have ended: one for each thread
+ * of their sums that went on without one, 0 in a healthy process.  Such a wait ends after about a second, and the outputs that hang on it are NaN: this tells them from those of inputs that are NaN.  The call waits for
+ * the device's default stream, and is none for a capture. */
+int32_t b200rwkv_op_lost_waits(int32_t device, int64_t* total);
+
 /* Kernels launched by this engine's forward steps since creation (graph replays counted by their kernel nodes). */
 int32_t b200rwkv_launch_count(b200rwkv_engine*, int64_t* total);
 

@@ -81,3 +81,10 @@ extern "C" int waits_run(int kernel, int block, int thread, int form, int split,
     }
     return e != cudaSuccess ? (int)e : (int)cudaDeviceSynchronize();
 }
+
+// waits that ran out so far
+extern "C" unsigned waits_lost() {
+    unsigned n = ~0u;
+    cudaMemcpyFromSymbol(&n, lost_waits, sizeof(n));
+    return n;
+}

@@ -104,3 +104,23 @@ def test_pairs_scales(lib, block, thread):
     u = block // 2 + 4
     want[u % 2 * 256:u % 2 * 256 + 256, u // 2 * 256:u // 2 * 256 + 256] = True
     assert torch.equal(nan, want)
+
+
+def test_lost_waits_are_counted(lib):
+    """One for each thread that lost one, in every kernel; none without."""
+    lib.waits_lost.restype = C.c_uint
+    before = lib.waits_lost()
+    for form, split, T, N, threads, thread in ((16, 4, 10, 300, FEW, 77), (128, 1, 100, 300, MANY, 5), (256, 2, 300, 600, PAIR, 131)):
+        run(lib, form, split, T, N)
+        assert lib.waits_lost() == before
+        run(lib, form, split, T, N, threads, 0, thread)
+        assert lib.waits_lost() >= before + 1
+        before = lib.waits_lost()
+
+
+def test_none_in_the_library():
+    from ai00_server_b200 import device_ops
+    x, w = torch.randn(300, 256, device="cuda"), torch.randn(400, 256, device="cuda")
+    device_ops.linear_e4m3(*device_ops.to_e4m3(x), *device_ops.to_e4m3(w, rows=128))
+    torch.cuda.synchronize()
+    assert device_ops.lost_waits() == 0 and device_ops.lost_waits(0) == 0
