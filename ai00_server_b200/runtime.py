@@ -428,6 +428,8 @@ class Model:
             if x is None:
                 continue
             a = np.asarray(x, dtype)
+            if name == "uniform":                # (doubles from 1 - 2^-25 on would be 1)
+                a = np.where((a == 1) & (np.asarray(x) < 1), np.nextafter(dtype(1), dtype(0)), a)
             if a.ndim == 0 and name != "uniform":
                 a = np.full(n, a, dtype)
             if a.shape != (n,):
