@@ -49,6 +49,13 @@ def _list(t, name, dtype, where, size):
     return t.data_ptr()
 
 
+def _scales(t, name, n, m, where):
+    """Address of contiguous f32 scales [n, m]: as many in another shape would be other blocks'."""
+    if t.shape != (n, m):
+        _bad(f"{name} must be [{n}, {m}]")
+    return _list(t, name, _F32, where, None)
+
+
 def _row_stride(t, name, shape, dtype, where):
     """Elements between the rows of a [rows, cols] tensor with neighbouring columns."""
     if t.dtype is not dtype or t.shape != shape or t.get_device() != where:
@@ -181,13 +188,13 @@ def to_e4m3(x, rows=1, out=None, scale=None):
         _bad("to_e4m3: a scale is for 1 or 128 rows")
     shape = x.shape
     n, width = shape
-    scales = -(-n // rows) * -(-width // 128)
+    down, across = -(-n // rows), -(-width // 128)
     if out is None:
         out = torch.empty(n, width, dtype=_E4M3, device=x.device)
     if scale is None:
-        scale = torch.empty(-(-n // rows), -(-width // 128), dtype=_F32, device=x.device)
+        scale = torch.empty(down, across, dtype=_F32, device=x.device)
     q = _E4M3_ROWS.pack(_E4M3_ROWS.size, _TYPE.get(dtype, -1), n, width, rows, 0, x.data_ptr(), _row_stride(x, "x", shape, dtype, where), out.data_ptr(),
-                        _row_stride(out, "out", shape, _E4M3, where), _list(scale, "scale", _F32, where, scales))
+                        _row_stride(out, "out", shape, _E4M3, where), _scales(scale, "scale", down, across, where))
     code = capi.lib().b200rwkv_op_e4m3(where, _stream(where), q)
     if code < 0:
         capi.check(code)
@@ -215,7 +222,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-5, offset=0.0, out=None, scal
     if o_dtype is _E4M3:
         if scale is None:
             scale = torch.empty(n, -(-width // 128), dtype=_F32, device=x.device)
-        s = _list(scale, "scale", _F32, where, n * -(-width // 128))
+        s = _scales(scale, "scale", n, -(-width // 128), where)
     elif scale is not None:
         _bad("rms_norm: scales come with an 8-bit out")
     if residual is not None:
@@ -256,7 +263,7 @@ def linear_e4m3(x, x_scale, w, w_scale, base=None, out=None, out_dtype=None):
     if base is not None:
         b, b_stride = base.data_ptr(), _row_stride(base, "base", (tokens, n), o_dtype, where)
     q = _LINEAR.pack(_LINEAR.size, _TYPE.get(o_dtype, -1), tokens, k, n, 0, x.data_ptr(), _row_stride(x, "x", (tokens, k), _E4M3, where),
-                     _list(x_scale, "x_scale", _F32, where, tokens * blocks), _list(w, "w", _E4M3, where, None), _list(w_scale, "w_scale", _F32, where, -(-n // 128) * blocks),
+                     _scales(x_scale, "x_scale", tokens, blocks, where), _list(w, "w", _E4M3, where, None), _scales(w_scale, "w_scale", -(-n // 128), blocks, where),
                      b, b_stride, out.data_ptr(), _row_stride(out, "out", (tokens, n), o_dtype, where))
     code = capi.lib().b200rwkv_op_linear_e4m3(where, _stream(where), q)
     if code < 0:
