@@ -210,7 +210,7 @@ void b200rwkv_engine::adapter_add(const GemmLaunch& g, const GemmParams& was, co
 
 // what the callers of the listed slots' rows have to get right
 void b200rwkv_engine::check_rows(const char* call, int nrows, const int* slots) {
-    auto need = [&](bool fine, int code, const std::string& what) { REQUIRE(fine, code, std::string(call) + ": " + what); };
+    auto need = [&](bool fine, int code, const char* what) { REQUIRE(fine, code, std::string(call) + ": " + what); };
     need(rank == 0, B200RWKV_ERR_INVALID, "only rank 0 holds the gathered logits");
     need(d_keep, B200RWKV_ERR_UNSUPPORTED, "the model keeps no logits rows");
     need(V <= LOGITS_MAX_VOCAB, B200RWKV_ERR_UNSUPPORTED, "vocabularies above 524288 are not supported");
@@ -218,7 +218,7 @@ void b200rwkv_engine::check_rows(const char* call, int nrows, const int* slots) 
     std::lock_guard<std::mutex> lk(keep_mu);
     for (int i = 0; i < nrows; ++i) {
         need(slots[i] >= 0 && slots[i] < S, B200RWKV_ERR_STATE, "slot out of range");
-        need(keep_valid[slots[i]], B200RWKV_ERR_STATE, "slot " + std::to_string(slots[i]) + " has produced no logits row yet");
+        REQUIRE(keep_valid[slots[i]], B200RWKV_ERR_STATE, std::string(call) + ": slot " + std::to_string(slots[i]) + " has produced no logits row yet");
     }
 }
 
