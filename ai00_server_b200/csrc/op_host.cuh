@@ -75,10 +75,15 @@ struct RowSpan {
     bool dense() const { return step == width || end - at == width; }
 };
 // some byte is in both, as far as can be told: rows at one distance are compared modulo it (columns of a wider buffer may lie side by side), rows without gaps
-// as a whole; of other rows nothing is said
+// as a whole, with each other and with rows that have some; of two at different distances nothing is said
 static bool overlap(const RowSpan& a, const RowSpan& b) {
     if (a.at >= b.end || b.at >= a.end) return false;
     if (a.at == b.at || (a.dense() && b.dense())) return true;
+    if (b.dense()) return overlap(b, a);
+    if (a.dense()) {                                 // (one that starts in front reaches the first row; one in a gap has a row behind it)
+        const uintptr_t d = a.at < b.at ? 0 : (a.at - b.at) % b.step;
+        return d < b.width || b.step - d < a.end - a.at;
+    }
     if (a.step != b.step) return false;
     const uintptr_t d = a.at <= b.at ? (b.at - a.at) % a.step : (a.step - (a.at - b.at) % a.step) % a.step;
     return d < a.width || a.step - d < b.width;
