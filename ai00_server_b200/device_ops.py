@@ -51,9 +51,11 @@ def _list(t, name, dtype, where, size):
 
 def _scales(t, name, n, m, where):
     """Address of contiguous f32 scales [n, m]: as many in another shape would be other blocks'."""
-    if t.shape != (n, m):
-        _bad(f"{name} must be [{n}, {m}]")
-    return _list(t, name, _F32, where, None)
+    if t.dtype is not _F32 or t.shape != (n, m) or t.get_device() != where or not t.is_contiguous():
+        _bad(f"{name} must be a contiguous [{n}, {m}] {_F32} tensor on cuda:{where}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _bad(f"{name} requires a gradient: these operators have none (call them under torch.no_grad())")
+    return t.data_ptr()
 
 
 def _row_stride(t, name, shape, dtype, where):
