@@ -22,9 +22,9 @@ NVCC_FLAGS = [
 KERNELS_OF_OPERATORS = ["adapters.cuh", "adapter_tiles.cuh", "logits.cuh"]
 KERNELS_OF_TOKENS = ["e4m3.cuh", "e4m3_linear.cuh", "sample_tokens.cuh"]
 UNITS = {
-    "engine.cu": [f for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh") and f not in [*KERNELS_OF_OPERATORS, *KERNELS_OF_TOKENS, "lost_waits.cuh", "op_host.cuh"]],
+    "engine.cu": [f for f in sorted(os.listdir(CSRC)) if f.endswith(".cuh") and f not in [*KERNELS_OF_OPERATORS, *KERNELS_OF_TOKENS, "lost_waits.cuh", "float_types.cuh", "op_host.cuh"]],
     "operators.cu": [*KERNELS_OF_OPERATORS, "lost_waits.cuh", "operators.cuh", "op_host.cuh", "common.cuh", "host.cuh"],
-    "token_ops.cu": [*KERNELS_OF_TOKENS, "lost_waits.cuh", "token_ops.cuh", "op_host.cuh", "common.cuh", "host.cuh", "sm_pair.cuh", "f32x2.cuh"],
+    "token_ops.cu": [*KERNELS_OF_TOKENS, "lost_waits.cuh", "token_ops.cuh", "op_host.cuh", "common.cuh", "host.cuh", "sm_pair.cuh", "f32x2.cuh", "float_types.cuh"],
 }
 
 

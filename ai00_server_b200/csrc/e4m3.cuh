@@ -13,24 +13,19 @@
 // that stay, sixteen columns a thread, with the next row on its way while one is worked on and the weights kept: 2048 rows of 4096, residual and all in bf16, 12.8 us, 4.6 TB/s (a CTA a row 15.7;
 // a copy of these bytes 12.2; values computed outside the condition behind which they are stored 15.6); rows of 4095 34 (48).
 #pragma once
-#include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 #include <type_traits>
 
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "float_types.cuh"
 
 namespace b200 {
 
 constexpr int E4_GROUP = 128;                    // columns of a scale
 constexpr float E4_TOP = 448.f;                  // the largest number
 constexpr int NORM_MAX_WIDTH = 32768;            // 512 threads of 64 columns
-
-template <typename E> __device__ __forceinline__ float e4_widen(E v);
-template <> __device__ __forceinline__ float e4_widen<float>(float v) { return v; }
-template <> __device__ __forceinline__ float e4_widen<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float e4_widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 // eight values of a thread as they lie in memory.  EIGHTS: neighbours, on a boundary of 16 bytes.  Else: of 256 columns that a warp has, those of each 32 that are its lane's, so that a
 // warp's accesses to rows that start anywhere are runs of 32 columns
@@ -64,7 +59,7 @@ __device__ __forceinline__ void e4_values(const E4Raw<E>& r, float (&v)[8]) {
         E e[8];
         memcpy(e, &r, sizeof(r));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = e4_widen<E>(e[i]);
+        for (int i = 0; i < 8; ++i) v[i] = widened<E>(e[i]);
     }
 }
 // eight values rounded, two at a time
@@ -399,11 +394,11 @@ __global__ void __launch_bounds__(E4_THREADS, EIGHTS && sizeof(E) == 2 ? 4 : 2) 
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(e4_widen<E>(a[i][j])));
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, fabsf(widened<E>(a[i][j])));
         const E4Over over = e4_over(scale_of(most));
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const float v[4] = {e4_widen<E>(a[i][0]), e4_widen<E>(a[i][1]), e4_widen<E>(a[i][2]), e4_widen<E>(a[i][3])};
+            const float v[4] = {widened<E>(a[i][0]), widened<E>(a[i][1]), widened<E>(a[i][2]), widened<E>(a[i][3])};
             if (warp + i * ROWS < rows) e4_put(out + (warp + i * ROWS) * p.out_stride, lane, last + 1, e4_four(v, over));
         }
     }

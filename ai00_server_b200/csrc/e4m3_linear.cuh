@@ -6,10 +6,10 @@
 #pragma once
 #include <cuda.h>
 #include <cudaTypedefs.h>
-#include <cuda_bf16.h>
 
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "float_types.cuh"
 #include "lost_waits.cuh"
 #include "sm_pair.cuh"
 
@@ -105,10 +105,6 @@ __device__ __forceinline__ void e4l_tmem(uint32_t at, float (&v)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
 }
-template <typename O> __device__ __forceinline__ float e4l_widen(O v);
-template <> __device__ __forceinline__ float e4l_widen<float>(float v) { return v; }
-template <> __device__ __forceinline__ float e4l_widen<__half>(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float e4l_widen<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <typename O> __device__ __forceinline__ O e4l_round(float v);
 template <> __device__ __forceinline__ float e4l_round<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half e4l_round<__half>(float v) { return __float2half_rn(v); }
@@ -306,7 +302,7 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
             }
 #pragma unroll
             for (int j = 0; j < BATCH; ++j)
-                if (n < p.N && tb + j * step < nt) out[(size_t)(t0 + tb + j * step) * p.out_stride] = e4l_round<O>(v[j] + e4l_widen<O>(old[j]));
+                if (n < p.N && tb + j * step < nt) out[(size_t)(t0 + tb + j * step) * p.out_stride] = e4l_round<O>(v[j] + widened<O>(old[j]));
         }
     }
     if (split > 1) cluster_sync_all();      // no CTA leaves while another reads its sums
@@ -571,7 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(E4Pair::THREADS, 1) 
                         const uint4 w = *at;
                         memcpy(e, &w, 16);
 #pragma unroll
-                        for (int j = 0; j < PER; ++j) v[j] += e4l_widen<O>(e[j]);
+                        for (int j = 0; j < PER; ++j) v[j] += widened<O>(e[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < PER; ++j) e[j] = e4l_round<O>(v[j]);

@@ -22,8 +22,7 @@
 // Tried: bins' sums from the front alone (half a hundredth of all weights are a tail of thousands of tokens: 410 for the 96 rows, 310 for the 512); rows in the registers or the shared memory of eight CTAs with exact weights in all bins (620 us for the last), steps unrolled four times (fetching their code took longer than
 // running it), a closure that was not inlined (its variables in memory: two to three times as long).
 #pragma once
-#include <cuda_bf16.h>
-
+#include "float_types.cuh"
 #include "sm_pair.cuh"
 #include "token_ops.cuh"
 
@@ -51,12 +50,10 @@ __device__ __forceinline__ float draw_max(float a, float b) {      // NaN where 
 template <typename E> struct DrawRaw;
 template <> struct DrawRaw<float> {
     using Four = float4;
-    static __device__ __forceinline__ float widen(float v) { return v; }
     static __device__ __forceinline__ float4 widen4(float4 v) { return v; }
 };
 template <> struct DrawRaw<__half> {
     using Four = uint2;
-    static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
     static __device__ __forceinline__ float4 widen4(uint2 u) {
         const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
         return make_float4(a.x, a.y, b.x, b.y);
@@ -64,7 +61,6 @@ template <> struct DrawRaw<__half> {
 };
 template <> struct DrawRaw<__nv_bfloat16> {
     using Four = uint2;
-    static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
     static __device__ __forceinline__ float4 widen4(uint2 u) {
         return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
     }
@@ -197,7 +193,7 @@ __global__ void __launch_bounds__(TH, PER_SM) draw_kernel(const __grid_constant_
         const int i = (g * 32 + lane) * 4;
         float x[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[c] = i + c < cnt ? DrawRaw<E>::widen(in[i + c]) : -INFINITY;
+        for (int c = 0; c < 4; ++c) x[c] = i + c < cnt ? widened<E>(in[i + c]) : -INFINITY;
         return make_float4(x[0], x[1], x[2], x[3]);
     };
     // Short steps take four turns' tokens at a time.  Long ones run a few times a CTA only, and fetching their code would take longer than running it were they unrolled: they have

@@ -28,7 +28,7 @@ struct DrawParams {
     int ctas_log, slice;             // CTAs of a row, tokens of each (a multiple of four)
 };
 
-// ctas_log, slice and vec of p are filled in here; V is at most DRAW_MAX_VOCAB
+// ctas_log and slice of p are filled in here; V is at most DRAW_MAX_VOCAB
 B200_HIDDEN void draw_rows(cudaStream_t s, DrawParams p, int rows);
 
 }  // namespace b200
