@@ -5,13 +5,13 @@
 // s and y / s are f32, rounded to nearest, and q is the e4m3 number nearest to that.  (The floor keeps 1 / s a number; a group of zeros is zeros.)
 //
 // Bound: memory, each value read once and written once, as far as the instructions let it: two divisions for every scale in all of its lanes, conversions two values at a time, sixteen columns
-// of a scale to a lane where no row has to stay.  Measured, with inputs larger than L2: rows of 4096 bf16 (14336 of them) 29 us, 6.0 TB/s, as a plain copy of these bytes (sixteen lanes of eight
-// columns, two to a thread: 35); blocks 29 us, 6.0 TB/s (with a test at every load and widened values kept instead of made again: 65).
-// Rows that start anywhere: a lane has every 32nd column, so that a warp's accesses are runs, all asked for at once (14336 rows of 4095 bf16 with a scale a row 88 us and blocks 60, of which
+// of a scale to a lane where no row has to stay.  Measured, with inputs larger than L2: rows of 4096 bf16 (14336 of them) 28 us, 6.3 TB/s, as a plain copy of these bytes (sixteen lanes of eight
+// columns, two to a thread: 35); blocks 28 us, 6.3 TB/s (with a test at every load and widened values kept instead of made again: 65).
+// Rows that start anywhere: a lane has every 32nd column, so that a warp's accesses are runs, all asked for at once (14336 rows of 4095 bf16 with a scale a row 88 us and blocks 62, of which
 // eight neighbours a lane, one value at a time, took 141 and 112; 2539 rows of 1364 f16 6.9 and 12.6).
-// A row of the norm stays in the registers of its CTA between the statistics and the outputs.  Few rows take a thread for every eight columns (latency; one row of 2560 2.0 us).  Many rows: CTAs
-// that stay, sixteen columns a thread, with the next row on its way while one is worked on and the weights kept: 2048 rows of 4096, residual and all in bf16, 12.8 us, 4.6 TB/s (a CTA a row 15.7;
-// a copy of these bytes 12.2; values computed outside the condition behind which they are stored 15.6); rows of 4095 34 (48).
+// A row of the norm stays in the registers of its CTA between the statistics and the outputs.  Few rows take a thread for every eight columns (latency; one row of 2560 1.9 us).  Many rows: CTAs
+// that stay, sixteen columns a thread, with the next row on its way while one is worked on and the weights kept: 2048 rows of 4096, residual and all in bf16, 12.3 us, 4.8 TB/s (a CTA a row 15.7;
+// a copy of as many bytes 11.0; values computed outside the condition behind which they are stored 15.6); rows of 4095 33 (48).
 #pragma once
 #include <cuda_fp8.h>
 
@@ -101,7 +101,7 @@ __device__ __forceinline__ void e4_store(E* p, int first, int width, const float
 // What a group's values are divided by: they become the f32 quotient as a division rounds it, to nearest, and that to nearest e4m3, so that the numbers are those that (y / s), converted
 // anywhere else, has.  The reciprocal comes in two parts, 1 / s = high + low to 2^-45 of itself: with e = 1 - s high, low = high (e + e^2).  A quotient y high + y low is off by 2^-44 before it
 // is rounded: as a division has it for every value of 16 bits (tried out), and for one of f32 but where y / s is that near to the middle of two f32 numbers beside a tie.  (The product with a
-// rounded reciprocal alone lay a step beside it where a value is on a tie of its group: 5 in 10 000 bf16 weights.)  high stays below 1 / s (the unit's is a step off at most): no low is
+// rounded reciprocal alone lay a step beside it where a value is on a tie of its group: 5 in 10 000 bf16 weights; 14336 x 4096 in blocks took 28.8 us with it where these take 29.4, and the norm of 2048 x 4096 12.4 and 12.3.)  high stays below 1 / s (the unit's is a step off at most): no low is
 // negative, and zeros keep their signs.  An infinite scale makes zeros of numbers and NaN of infinities
 struct E4Over { f32x2 high, low; };
 __device__ __forceinline__ E4Over e4_over(float s) {

@@ -113,7 +113,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 e4l_round<__nv_bfloat16>(fl
 // ---- few tokens: the weights' bytes are what a call costs ----
 // 128 weight rows are the rows of the accumulator (a lane an output), up to TT tokens its columns; a cluster of `split` CTAs deals the blocks of inputs among
 // itself, so that all SMs stream weights, and adds its sums in the order of its CTAs: CTA r finishes tokens r, r + split, ...
-// Measured: 16 tokens 4096 -> 14336 14.2 us (58.7 MB of weights: 4.1 TB/s; the start and the end of a launch are 4 of them), 8192 -> 65536 99 us (5.4 TB/s), one token 2560 -> 2560 6;
+// Measured: 16 tokens 4096 -> 14336 14.2 us (58.7 MB of weights: 4.1 TB/s; the start and the end of a launch are 4 of them), 4096 -> 65536 47 us (6.0 TB/s), one token 2560 -> 2560 5.0, or 6.4 with weights from memory;
 // 32 tokens 4096 -> 14336 16, 64 tokens 18, 333 tokens 8960 -> 2560 24.  Of those 24, loads alone take 15.5 and loads with products 21: 32 KB a block of inputs come in and are read by the
 // products at 128 bytes a cycle.  Clusters of five to seven CTAs leave SMs idle (22 us for 14.5); a request for the weights in L2 ahead of the wait for the kernel in
 // front lost (16 to 17 us).
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(E4Few<TT>::THREADS, E4Few<TT>::PER_SM) e4_few_
 // What bounds it: a block of inputs is 512 cycles of the tensor cores and 1 000 of the eight warps that scale its sums, a chain of a wait, four reads of tensor memory and their
 // multiply-adds (without scales, a whole k range summed in tensor memory, 2048 tokens 4096 -> 14336 took 108 us where these took 133).  Those warps have 224 registers, so that a read is in flight
 // beside each quarter's multiply-adds; scales come through shared memory by warps of their own; sums leave through shared memory.
-// Measured: 2048 tokens 4096 -> 14336 118 to 140 us, 1.7 to 2.0 PFLOP/s (140 behind other work, where the power limit shows), with a base 133, to 14337 outputs with a base 166;
+// Measured: 2048 tokens 4096 -> 14336 119 to 141 us, 1.7 to 2.0 PFLOP/s (119 in short runs, 141 for seconds, at the power limit and 1605 MHz), with a base 133, to 14337 outputs with a base 166;
 // 4096 tokens 8192 -> 8192 238 us, 2.3 PFLOP/s; 256 tokens 192 -> 75776 19 us, with a base 26.
 // Tried: sixteen warps for the sums (146 us), a read ahead over the ends of blocks (140: registers spill, and spilled ones are waited for at every arrival), tiles of 128 outputs (160), the
 // last tiles of a launch in halves and quarters (133).

@@ -18,7 +18,7 @@
 // Shape: as many CTAs a row as SMs there are for it, a cluster of sixteen at most; what they tell one another costs a microsecond each time.  Runs that fit stay in shared memory, others are read again
 // from L2 for every step.  More rows than SMs: a CTA a row, two to an SM.  Steps that only a few tokens take part in gather those of 128 first, so that a warp's exponentials are not one lane's.
 // Measured, us: a row of 65536 with top-k 50 and top-p 0.95 12, 16 rows of top-p 0.9 26; 96 rows of 100003 in bf16, top-k 1000 and top-p 0.98 (every fourth top-p alone), 130; 512
-// rows of 65536: the best token 39, top-k 50 59, no limit 108, top-p 0.9 232.
+// rows of 65536: the best token 39, top-k 50 59, no limit 109, top-p 0.9 222 to 233.
 // Tried: bins' sums from the front alone (half a hundredth of all weights are a tail of thousands of tokens: 410 for the 96 rows, 310 for the 512); rows in the registers or the shared memory of eight CTAs with exact weights in all bins (620 us for the last), steps unrolled four times (fetching their code took longer than
 // running it), a closure that was not inlined (its variables in memory: two to three times as long).
 #pragma once

@@ -29,7 +29,7 @@ static void norm_form(cudaStream_t s, const NormParams& p, int rows) {
     // threads of so many times eight values (of which a warp has two groups of 128 columns where rows start anywhere)
     const int eights = EIGHTS ? p.width / 8 : (p.width + 255) / 256 * 32;
     auto threads = [&](int nv) { return ((eights + nv - 1) / nv + 31) / 32 * 32; };
-    // more rows than CTAs that stay (2048 rows of 4096 bf16 12.8 us; a CTA a row 15.7, with 256 threads or 512)
+    // more rows than CTAs that stay (2048 rows of 4096 bf16 12.3 us; a CTA a row 15.7, with 256 threads or 512)
     if (threads(2) <= NORM_MANY_THREADS) {
         const int ctas = sm_count() * (norm_many_per_sm<E, R, EIGHTS>() * NORM_MANY_THREADS / threads(2));
         if (rows > ctas) return launch(rms_norm_kernel<E, R, 2, EIGHTS, true>, dim3(ctas), threads(2), 0, s, p);

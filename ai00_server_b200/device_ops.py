@@ -1,5 +1,5 @@
-"""Operators on tensors in GPU memory (b200rwkv_op_*, include/b200rwkv.h): what the engine runs on its own buffers for the
-requests of a batch, for programs that hold theirs as torch tensors.
+"""Operators on tensors in GPU memory (b200rwkv_op_*, include/b200rwkv.h), for programs that hold theirs as torch tensors: what the engine runs on its own
+buffers for the requests of a batch,
 
   low_rank   low-rank adapters of many requests beside shared projections
   logits     rows of logits adjusted by penalties, biases and grammar masks, as logits, probabilities or log-probabilities
