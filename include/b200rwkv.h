@@ -420,7 +420,8 @@ int32_t b200rwkv_op_logits(int32_t device, void* stream, const b200rwkv_logits* 
  * 128 neighbouring columns of a row (activations) or to a block of 128 rows by 128 columns (weights); the last of a row or column may hold fewer:
  *     scale = max(max |x|, 2^-100) / 448,   out = x / scale
  * Both quotients are f32 numbers, rounded to nearest as a division does it, and out is the e4m3 number nearest to the second (ties to even): the bytes that the same division makes
- * elsewhere.  (The one exception: an f32 x whose quotient lies within 2^-44 of itself at the middle of two f32 numbers, one of them on a tie, may come out on the tie's other side.)  So
+ * elsewhere.  (The one exception: an f32 x whose quotient lies within 2^-44 of itself, or 2^-30 for scales above 2^104, at the middle of two f32 numbers, one of them on a tie, may come out on the tie's
+ * other side.)  So
  * that scale times number is off by 2^-4 of the value at most, or by 2^-10 of a scale where the value is below 2^-6 of it.  A NaN stays with its number; an infinity makes its number NaN, and the scale infinite. */
 typedef struct {
     uint32_t struct_bytes;
